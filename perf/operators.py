@@ -100,12 +100,19 @@ def _generator(seed):
     return g
 
 
+def _places(rows, n, vocab, g):
+    """n tokens a row, none of them twice: one out of every n-th of the vocabulary, in no order."""
+    first = torch.arange(n + 1, device=DEVICE) * vocab // n
+    wide = (first[1:] - first[:-1]).double()
+    at = first[:-1] + (wide * torch.rand(rows, n, generator=g, device=DEVICE, dtype=torch.float64)).long()
+    return at[:, torch.randperm(n, generator=g, device=DEVICE)]
+
+
 def _logits(rows, vocab, g):
     """What a language model says: most of the vocabulary far below a few tokens."""
     x = torch.randn(rows, vocab, generator=g, device=DEVICE) * 2.2
     n = min(24, vocab)
-    at = torch.randint(0, vocab, (rows, n), generator=g, device=DEVICE)
-    x.scatter_(1, at, 4.0 + 9.0 * torch.rand(rows, n, generator=g, device=DEVICE))
+    x.scatter_(1, _places(rows, n, vocab, g), 4.0 + 9.0 * torch.rand(rows, n, generator=g, device=DEVICE))
     return x
 
 
@@ -142,7 +149,7 @@ def _prepare_adjust(case, seed):
         each = torch.randint(0, n + 1, (R,), generator=g, device=DEVICE)        # some rows have none
         start = torch.zeros(R + 1, dtype=torch.int32, device=DEVICE)
         start[1:] = each.cumsum(0)
-        ids = torch.rand(R, V, generator=g, device=DEVICE).topk(n, dim=1).indices       # no token twice in a row
+        ids = _places(R, n, V, g)
         keep = torch.arange(n, device=DEVICE)[None, :] < each[:, None]
         value = torch.randn(R, n, generator=g, device=DEVICE) * 5.0
         value[torch.rand(R, n, generator=g, device=DEVICE) < 0.1] = -math.inf
