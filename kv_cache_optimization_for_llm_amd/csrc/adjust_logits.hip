@@ -1,0 +1,206 @@
+// What a request asks of its logits before a token is taken from them.  With l the logit of a token, m whether the request's row of
+// marks has it, c how often the request has said it:
+//
+//     m:            l <- l > 0 ? l / repetition : l * repetition
+//     m and c > 0:  l <- l - (frequency c + presence)
+//     biases:       l <- l + b, for every one of the row's list that names the token, in the list's order
+//     grammar:      l <- -inf where the token's bit is not set, whatever the logit was
+//
+// One pass: the logits and a byte of marks a token come in 4 tokens a thread and load, a count is looked up only where the mark is
+// set, a grammar is a bit a token.  A row's biases are a list in no order: every workgroup picks out those of its own tokens,
+// 256 at a time, in the list's order, and the threads that hold the tokens add them.  What is computed is 32-bit throughout.
+#include "common.h"
+
+#define AL_THREADS 256
+#define AL_WAVES (AL_THREADS / KVA_WAVE)
+
+typedef float al_f32x4 __attribute__((ext_vector_type(4), aligned(4)));         // (rows start at any multiple of their type)
+typedef uint16_t al_u16x4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint8_t al_u8x4 __attribute__((ext_vector_type(4), aligned(1)));
+
+struct AdjustArgs {
+    const void *logits;
+    float *out;
+    long long in_stride, out_stride;        // elements from a row to the next
+    int vocab;
+    const int *row_seat;                    // -1: no marks
+    int seats;
+    const unsigned char *marks;             // [seats, vocab]
+    const int *counts;                      // [seats, vocab]
+    const float *repetition, *presence, *frequency;
+    const int *bias_start, *bias_token;     // [rows + 1], [biases]
+    const float *bias_value;
+    int biases;
+    const int *allowed_row;                 // -1: everything is allowed
+    const unsigned *allowed;                // [grammars, words]
+    int grammars, words;
+};
+
+// grid (tiles, rows); a tile is UNITS x 1,024 tokens
+template <typename T, int UNITS>
+__global__ void __launch_bounds__(AL_THREADS)
+adjust_logits_kernel(AdjustArgs a) {
+    __shared__ int hit_token[AL_THREADS];
+    __shared__ float hit_value[AL_THREADS];
+    __shared__ int hits_of[AL_WAVES];
+    const int row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, vocab = a.vocab;
+    const int tile0 = blockIdx.x * (UNITS * 4 * AL_THREADS), tile1 = min(vocab, tile0 + UNITS * 4 * AL_THREADS);
+    const T *in = reinterpret_cast<const T *>(a.logits) + row * a.in_stride;
+    float l[UNITS][4];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const int t = tile0 + 4 * (u * AL_THREADS + tid);
+        if (t + 3 < vocab) {
+            if constexpr (sizeof(T) == 4) {
+                const al_f32x4 v = *reinterpret_cast<const al_f32x4 *>(in + t);
+                l[u][0] = v.x, l[u][1] = v.y, l[u][2] = v.z, l[u][3] = v.w;
+            } else {
+                const al_u16x4 v = *reinterpret_cast<const al_u16x4 *>(in + t);
+                l[u][0] = bf16_bits_to_float(v.x), l[u][1] = bf16_bits_to_float(v.y);
+                l[u][2] = bf16_bits_to_float(v.z), l[u][3] = bf16_bits_to_float(v.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[u][i] = t + i < vocab ? to_float(in[t + i]) : 0.f;
+        }
+    }
+    // a row that names a seat or a grammar that is not there gets no token at all
+    bool lost = false;
+    if (a.row_seat != nullptr) {
+        const int seat = a.row_seat[row];
+        if (seat >= a.seats || seat < -1) lost = true;
+        else if (seat >= 0) {
+            const unsigned char *marks = a.marks + (size_t)seat * vocab;
+            const int *counts = a.counts != nullptr ? a.counts + (size_t)seat * vocab : nullptr;
+            const float rep = a.repetition != nullptr ? a.repetition[row] : 1.f;
+            const float pres = a.presence != nullptr ? a.presence[row] : 0.f, freq = a.frequency != nullptr ? a.frequency[row] : 0.f;
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                const int t = tile0 + 4 * (u * AL_THREADS + tid);
+                unsigned m = 0;
+                if (t + 3 < vocab) {
+                    const al_u8x4 v = *reinterpret_cast<const al_u8x4 *>(marks + t);
+                    m = (v.x != 0) | (v.y != 0) << 1 | (v.z != 0) << 2 | (v.w != 0) << 3;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (t + i < vocab && marks[t + i] != 0) m |= 1u << i;
+                }
+                if (m == 0) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(m >> i & 1)) continue;
+                    float x = l[u][i];
+                    if (rep != 1.f) x = x > 0.f ? x / rep : x * rep;
+                    if (counts != nullptr) {
+                        const int c = counts[t + i];
+                        if (c > 0) x -= fmaf(freq, (float)c, pres);
+                    }
+                    l[u][i] = x;
+                }
+            }
+        }
+    }
+    if (a.bias_start != nullptr) {
+        const int from = max(0, a.bias_start[row]), to = min(a.biases, a.bias_start[row + 1]);
+        for (int base = from; base < to; base += AL_THREADS) {
+            const int i = base + tid;
+            const int token = i < to ? a.bias_token[i] : -1;
+            const bool mine = token >= tile0 && token < tile1;
+            const unsigned long long votes = __ballot(mine);
+            if (lane == 0) hits_of[wave] = __popcll(votes);
+            __syncthreads();
+            int before = 0, hits = 0;
+#pragma unroll
+            for (int w = 0; w < AL_WAVES; ++w) {
+                if (w < wave) before += hits_of[w];
+                hits += hits_of[w];
+            }
+            if (mine) {
+                const int at = before + __popcll(votes & ((1ull << lane) - 1));
+                hit_token[at] = token;
+                hit_value[at] = a.bias_value[i];
+            }
+            __syncthreads();
+            for (int h = 0; h < hits; ++h) {
+                const int rel = hit_token[h] - tile0;
+                if ((rel >> 2) % AL_THREADS != tid) continue;
+                const int unit = (rel >> 2) / AL_THREADS, which = rel & 3;
+                const float b = hit_value[h];
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (u == unit && j == which) l[u][j] += b;
+            }
+            __syncthreads();
+        }
+    }
+    const unsigned *allowed = nullptr;
+    if (a.allowed_row != nullptr) {
+        const int g = a.allowed_row[row];
+        if (g >= a.grammars || g < -1) lost = true;
+        else if (g >= 0) allowed = a.allowed + (size_t)g * a.words;
+    }
+    float *out = a.out + row * a.out_stride;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const int t = tile0 + 4 * (u * AL_THREADS + tid);
+        if (t >= vocab) continue;
+        unsigned bits = 15;
+        if (allowed != nullptr) bits = allowed[t / 32] >> t % 32;
+        if (lost) bits = 0;
+        al_f32x4 v;
+        v.x = bits & 1 ? l[u][0] : -INFINITY;
+        v.y = bits & 2 ? l[u][1] : -INFINITY;
+        v.z = bits & 4 ? l[u][2] : -INFINITY;
+        v.w = bits & 8 ? l[u][3] : -INFINITY;
+        if (t + 3 < vocab) *reinterpret_cast<al_f32x4 *>(out + t) = v;
+        else
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (t + i < vocab) out[t + i] = v[i];
+    }
+}
+
+extern "C" int kva_adjust_logits(float *out, long long out_stride, const void *logits, int dtype, long long in_stride, int rows, int vocab,
+                                 const int *row_seat, int seats, const unsigned char *marks, const int *counts, const float *repetition,
+                                 const float *presence, const float *frequency, const int *bias_start, const int *bias_token,
+                                 const float *bias_value, int biases, const int *allowed_row, const int *allowed, int grammars,
+                                 hipStream_t stream) {
+    KVA_REQUIRE(dtype == KVA_F32 || dtype == KVA_BF16, "adjust_logits: dtype %d", dtype);
+    KVA_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab < 1 << 30, "adjust_logits: bad sizes rows=%d vocab=%d", rows, vocab);
+    KVA_REQUIRE(row_seat == nullptr || (marks != nullptr && seats > 0), "adjust_logits: seats without marks");
+    KVA_REQUIRE(allowed_row == nullptr || (allowed != nullptr && grammars > 0), "adjust_logits: grammars are missing");
+    if (rows == 0) return KVA_OK;
+    const AdjustArgs a{logits, out, in_stride, out_stride, vocab, row_seat, seats, marks, counts, repetition, presence, frequency, bias_start,
+                       bias_token, bias_value, biases, allowed_row, (const unsigned *)allowed, grammars, (vocab + 31) / 32};
+    const int tile = 4 * AL_THREADS;
+    const dim3 grid((vocab + tile - 1) / tile, rows), block(AL_THREADS);
+    if (dtype == KVA_F32) hipLaunchKernelGGL((adjust_logits_kernel<float, 1>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((adjust_logits_kernel<bf16_t, 1>), grid, block, 0, stream, a);
+    KVA_CHECK_LAUNCH("adjust_logits");
+    return KVA_OK;
+}
+
+// counts[seat][token] += 1 and marks[seat][token] = 1; additions of whole numbers, so any order gives the same
+__global__ void __launch_bounds__(256)
+count_tokens_kernel(unsigned char *__restrict__ marks, int *__restrict__ counts, int seats, int vocab, const int *__restrict__ of,
+                    const int *__restrict__ tokens, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int seat = of[i], token = tokens[i];
+    if (seat < 0 || seat >= seats || token < 0 || token >= vocab) return;
+    const size_t at = (size_t)seat * vocab + token;
+    marks[at] = 1;
+    if (counts != nullptr) atomicAdd(counts + at, 1);
+}
+
+extern "C" int kva_count_tokens(unsigned char *marks, int *counts, int seats, int vocab, const int *of, const int *tokens, int n,
+                                hipStream_t stream) {
+    KVA_REQUIRE(n >= 0 && seats > 0 && vocab > 0, "count_tokens: bad sizes");
+    if (n == 0) return KVA_OK;
+    hipLaunchKernelGGL(count_tokens_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, marks, counts, seats, vocab, of, tokens, n);
+    KVA_CHECK_LAUNCH("count_tokens");
+    return KVA_OK;
+}

@@ -23,6 +23,7 @@
 // 12.4, 64 rows (33 MB) 8.6 / 17.3, 128 rows 14.8 / 24.0.  With 128 workgroups a row whose threads took four tokens each, one by
 // one, and a single wavefront that walked its spans of the chunk: 64 rows 13.8 / 35.2.
 #include "common.h"
+#include "counter_uniform.h"
 #include <string.h>
 #include <math.h>
 
@@ -142,16 +143,6 @@ struct Online {
 };
 
 } // namespace
-
-__host__ __device__ inline float counter_uniform(unsigned int seed, unsigned int key, unsigned int step) {
-    unsigned long long z = ((unsigned long long)key << 32) ^ (unsigned long long)step;
-    z ^= (unsigned long long)seed * 0x9E3779B97F4A7C15ULL;
-    z += 0x9E3779B97F4A7C15ULL;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ULL;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBULL;
-    z = z ^ (z >> 31);
-    return (float)(z >> 40) * (1.0f / 16777216.0f);
-}
 
 // One record per (row, chunk): the chunk's best (value, id), and for temperature rows the chunk's
 // maximum and its sum of exp((l - maximum) / T).

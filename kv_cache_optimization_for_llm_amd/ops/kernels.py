@@ -1195,6 +1195,203 @@ def mark_tokens(mask: torch.Tensor, seats: torch.Tensor, tokens: torch.Tensor) -
           "mark_tokens")
 
 
+def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The launch goes to the current device's stream: everything it takes has to be there."""
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != _RAW_DEVICE():
+            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{_RAW_DEVICE()}")
+
+
+def _rows_of(what: str, t: torch.Tensor, name: str) -> int:
+    """Elements from a row of ``[rows, columns]`` to the next; the elements of a row lie next to each other."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise KernelError(f"{what}: {name} must be [rows, vocabulary]")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise KernelError(f"{what}: the elements of a row of {name} must lie next to each other")
+    if rows > 1 and t.stride(0) < cols:
+        raise KernelError(f"{what}: rows of {name} overlap")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _per_row(what: str, rows: int, dtype: torch.dtype, **arrays: Optional[torch.Tensor]) -> list:
+    out = []
+    for name, t in arrays.items():
+        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != (rows,)):
+            raise KernelError(f"{what}: {name} must have an element per row")
+        out.append(_opt(t, name, dtype))
+    return out
+
+
+def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional[torch.Tensor] = None,
+                  marks: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                  repetition: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                  frequency: Optional[torch.Tensor] = None, bias: Optional[tuple] = None, allowed: Optional[torch.Tensor] = None,
+                  allowed_row: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What requests ask of their logits ``[rows, vocab]`` (fp32 or bf16; rows may be apart), into the fp32 ``out`` (which may be
+    the fp32 logits themselves), in this order:
+
+    * ``marks`` uint8 ``[seats, vocab]`` with ``row_seat`` (-1: none): a marked token's logit ``l`` becomes ``l / r`` if it is
+      above 0 and ``l * r`` else, ``r`` the row's ``repetition``; and where the seat's ``counts`` (int32 ``[seats, vocab]``) of
+      it, ``c``, is above 0, ``l - (frequency * c + presence)`` with the row's two numbers.  Counts of tokens that are not
+      marked are not read (:func:`count_tokens` keeps both);
+    * ``bias`` = (start int32 ``[rows + 1]``, token int32 ``[n]``, value fp32 ``[n]``): row ``i`` adds ``value[start[i] :
+      start[i + 1]]`` to the logits of those tokens, one after the other; tokens outside the vocabulary are passed over;
+    * ``allowed`` int32 ``[grammars, ceil(vocab / 32)]`` with ``allowed_row`` (-1: everything): the logit of a token whose bit
+      (``token % 32`` of word ``token / 32``) is not set becomes -inf.
+
+    A row that names a seat or a grammar that is not there gets -inf everywhere: no token can be taken from it."""
+    what = "adjust_logits"
+    in_stride, out_stride = _rows_of(what, logits, "logits"), _rows_of(what, out, "out")
+    rows, vocab = logits.shape
+    if out.shape != logits.shape:
+        raise KernelError(f"{what}: out {tuple(out.shape)} does not fit logits {tuple(logits.shape)}")
+    p_in, p_out = _dev(logits, "logits", contiguous=False), _dev(out, "out", torch.float32, contiguous=False)
+    code = dtype_code(logits.dtype)
+    if rows and vocab and not (p_in == p_out and logits.dtype == out.dtype and in_stride == out_stride):
+        size = logits.element_size()
+        if p_in < p_out + 4 * ((rows - 1) * out_stride + vocab) and p_out < p_in + size * ((rows - 1) * in_stride + vocab):
+            raise KernelError(f"{what}: out overlaps the logits without being them")
+    if (marks is None) != (row_seat is None):
+        raise KernelError(f"{what}: marks and the seats of the rows go together")
+    if marks is None and (counts is not None or repetition is not None):
+        raise KernelError(f"{what}: counts and repetition need marks")
+    if counts is None and (presence is not None or frequency is not None):
+        raise KernelError(f"{what}: presence and frequency need counts")
+    for name, t in (("marks", marks), ("counts", counts)):
+        if t is not None and (t.dim() != 2 or t.shape[1] != vocab or t.shape[0] < 1 or t.shape[0] != marks.shape[0]):
+            raise KernelError(f"{what}: {name} must be [seats, {vocab}]")
+    if (allowed is None) != (allowed_row is None):
+        raise KernelError(f"{what}: grammars and the rows' numbers of them go together")
+    if allowed is not None and (allowed.dim() != 2 or allowed.shape[0] < 1 or allowed.shape[1] != (vocab + 31) // 32):
+        raise KernelError(f"{what}: allowed must be [grammars, {(vocab + 31) // 32}] words of 32 tokens")
+    start = token = value = None
+    if bias is not None:
+        if len(bias) != 3:
+            raise KernelError(f"{what}: bias is (start, token, value)")
+        start, token, value = bias
+        if start.shape != (rows + 1,) or token.dim() != 1 or value.shape != token.shape:
+            raise KernelError(f"{what}: bias takes rows + 1 starts and a value per token")
+    _here(what, logits, out, row_seat, marks, counts, repetition, presence, frequency, start, token, value, allowed, allowed_row)
+    rep, pres, freq = _per_row(what, rows, torch.float32, repetition=repetition, presence=presence, frequency=frequency)
+    seat, grammar = _per_row(what, rows, torch.int32, row_seat=row_seat, allowed_row=allowed_row)
+    check(hip_lib().kva_adjust_logits(
+        p_out, out_stride, p_in, code, in_stride, rows, vocab, seat, marks.shape[0] if marks is not None else 0,
+        _opt(marks, "marks", torch.uint8), _opt(counts, "counts", torch.int32), rep, pres, freq, _opt(start, "bias start", torch.int32),
+        _opt(token, "bias token", torch.int32), _opt(value, "bias value", torch.float32), token.shape[0] if token is not None else 0,
+        grammar, _opt(allowed, "allowed", torch.int32), allowed.shape[0] if allowed is not None else 0, _stream()), what)
+    return out
+
+
+def count_tokens(marks: torch.Tensor, counts: Optional[torch.Tensor], seats: torch.Tensor, tokens: torch.Tensor) -> None:
+    """``marks[seat, token] = 1`` and, with counts, ``counts[seat, token] += 1`` for every pair of ``seats`` and ``tokens`` (int32,
+    as often as it is there); pairs outside the arrays are passed over."""
+    what = "count_tokens"
+    if marks.dim() != 2 or (counts is not None and counts.shape != marks.shape) or seats.dim() != 1 or tokens.shape != seats.shape:
+        raise KernelError(f"{what}: one seat per token, marks and counts [seats, vocab]")
+    _here(what, marks, counts, seats, tokens)
+    check(hip_lib().kva_count_tokens(
+        _dev(marks, "marks", torch.uint8), _opt(counts, "counts", torch.int32), marks.shape[0], marks.shape[1],
+        _dev(seats, "seats", torch.int32), _dev(tokens, "tokens", torch.int32), seats.shape[0], _stream()), what)
+
+
+def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
+                     top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None, uniform: Optional[torch.Tensor] = None,
+                     seed: int = 0, rng_key: Optional[torch.Tensor] = None, rng_step: Optional[torch.Tensor] = None,
+                     kept: Optional[torch.Tensor] = None, logprob: Optional[torch.Tensor] = None,
+                     host_tokens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A token per row of fp32 logits ``[rows, vocab]`` from the best of the row.  In the order of the logits (the largest first,
+    of equal ones the lowest id; -inf and NaN are not in it) and with ``w = exp((l - max l) * inv_temperature)``:
+
+    1. the first ``top_k`` tokens (int32; <= 0: all);
+    2. of these the shortest beginning that has at least the share ``top_p`` of their weight (>= 1: all of them; at least one token);
+    3. of these the ones with ``w >= min_p`` and the best ones (<= 0: all of them);
+    4. of these the first, by ids, at which the weights up to it exceed ``u`` times all of theirs; ``u`` is ``uniform`` (fp32, in
+       [0, 1)) or, without it, the number that :func:`sample` draws for (``seed``, ``rng_key``, ``rng_step``).
+
+    Weights are held to 2^-45 of the best one's for vocabularies of up to 131,072 (half as finely for every doubling) and added up
+    exactly; tokens of less than half of that keep their place in the order and are never drawn.  Rows whose ``inv_temperature`` is
+    not above 0 take the best token.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability among
+    them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
+    tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
+    what = "sample_truncated"
+    stride = _rows_of(what, logits, "logits")
+    rows, vocab = logits.shape
+    if inv_temperature is None:
+        raise KernelError(f"{what}: inv_temperature is needed")
+    if uniform is None and (rng_key is None or rng_step is None):
+        raise KernelError(f"{what}: random numbers, or a key and a step per row, are needed")
+    if uniform is not None and (rng_key is not None or rng_step is not None):
+        raise KernelError(f"{what}: random numbers are given twice")
+    if host_tokens is not None and (host_tokens.is_cuda or not host_tokens.is_pinned() or host_tokens.dtype != torch.int32
+                                    or host_tokens.dim() != 1 or host_tokens.shape[0] < rows or not host_tokens.is_contiguous()):
+        raise KernelError(f"{what}: host_tokens must be a pinned host int32 vector with a place per row")
+    _here(what, logits, out_tokens, inv_temperature, top_k, top_p, min_p, uniform, rng_key, rng_step, kept, logprob)
+    inv_t, p, least, u, lp = _per_row(what, rows, torch.float32, inv_temperature=inv_temperature, top_p=top_p, min_p=min_p,
+                                      uniform=uniform, logprob=logprob)
+    tok, k, key, step, n = _per_row(what, rows, torch.int32, out_tokens=out_tokens, top_k=top_k, rng_key=rng_key, rng_step=rng_step,
+                                    kept=kept)
+    check(hip_lib().kva_sample_truncated(
+        tok, _dev(logits, "logits", torch.float32, contiguous=False), stride, rows, vocab, inv_t, k, p, least, u, int(seed) & 0xFFFFFFFF,
+        key, step, n, lp, ctypes.c_void_p(host_tokens.data_ptr()) if host_tokens is not None else None, _stream()), what)
+    return out_tokens
+
+
+def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, lengths: torch.Tensor, page_size: int,
+                pages: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Block tables that take the pages their requests need: request ``e`` sits in row ``seats[e]`` of ``table`` (int32 ``[rows,
+    blocks]``), has its first ``held[e]`` blocks mapped and will hold ``lengths[e]`` tokens; blocks ``held[e] .. ceil(lengths[e] /
+    page_size) - 1`` get the next of ``pages`` (int32), request after request.  ``offsets`` (int32 ``[requests + 1]``, made if
+    absent) gets where each one's pages begin and, last, how many all need.  A request whose pages are not all among ``pages``
+    takes none of them and its row stays as it is; one whose seat or blocks are outside the table needs none.  No row may be
+    named by two requests whose blocks overlap.  Up to 4,096 requests."""
+    what = "grow_tables"
+    n = seats.shape[0] if seats.dim() == 1 else -1
+    if n < 0 or held.shape != (n,) or lengths.shape != (n,) or pages.dim() != 1 or table.dim() != 2:
+        raise KernelError(f"{what}: a table [rows, blocks], a seat, held blocks and a length per request, and a row of pages")
+    if offsets is None:
+        offsets = torch.empty(n + 1, dtype=torch.int32, device=table.device)
+    if offsets.shape != (n + 1,):
+        raise KernelError(f"{what}: offsets has a place per request and one more")
+    _here(what, table, seats, held, lengths, pages, offsets)
+    if n == 0:
+        _dev(offsets, "offsets", torch.int32)
+        return offsets.zero_()
+    check(hip_lib().kva_grow_tables(
+        _dev(table, "table", torch.int32), table.shape[0], table.shape[1], _dev(seats, "seats", torch.int32), _dev(held, "held", torch.int32),
+        _dev(lengths, "lengths", torch.int32), n, int(page_size), _dev(pages, "pages", torch.int32), pages.shape[0],
+        _dev(offsets, "offsets", torch.int32), _stream()), what)
+    return offsets
+
+
+def step_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, tables, page_size: int, q_start: torch.Tensor,
+              positions: torch.Tensor, tok_seat: torch.Tensor, slots) -> None:
+    """The index arrays of a step from its entries: entry ``e`` brings ``lengths[e]`` tokens of the request in row ``seats[e]``, from
+    position ``starts[e]`` on.  ``q_start`` ``[entries + 1]`` gets each entry's first row (its last element: the rows of all), and
+    the step's rows get their position (``positions``), seat (``tok_seat``) and, per group of the cache, their slot ``page *
+    page_size + row in the page`` out of the group's block table (``tables``: int32 ``[rows, blocks]``, ``slots``: ``[tokens]``; up
+    to 8 groups), -1 where no page is mapped, or the position or the seat is outside the table.  Rows behind the last entry's are left
+    as they were, and rows that the arrays have no room for are not made.  Everything is int32; up to 4,096 entries."""
+    what = "step_rows"
+    n = lengths.shape[0] if lengths.dim() == 1 else -1
+    if n < 0 or starts.shape != (n,) or seats.shape != (n,) or q_start.shape != (n + 1,):
+        raise KernelError(f"{what}: a length, a start and a seat per entry, and one more place in q_start")
+    tokens = positions.shape[0] if positions.dim() == 1 else -1
+    if tokens < 0 or tok_seat.shape != (tokens,) or len(slots) != len(tables) or any(s.shape != (tokens,) for s in slots):
+        raise KernelError(f"{what}: a position, a seat and a slot per group for every token")
+    if any(t.dim() != 2 for t in tables):
+        raise KernelError(f"{what}: tables are [rows, blocks]")
+    groups = len(tables)
+    _here(what, lengths, starts, seats, q_start, positions, tok_seat, *tables, *slots)
+    pointers, sizes = ctypes.c_void_p * max(1, groups), ctypes.c_int * max(1, groups)
+    check(hip_lib().kva_step_rows(
+        _dev(lengths, "lengths", torch.int32), _dev(starts, "starts", torch.int32), _dev(seats, "seats", torch.int32), n,
+        pointers(*[_dev(t, "table", torch.int32) for t in tables]), sizes(*[t.shape[0] for t in tables]),
+        sizes(*[t.shape[1] for t in tables]), groups, int(page_size), tokens, _dev(q_start, "q_start", torch.int32),
+        _dev(positions, "positions", torch.int32), _dev(tok_seat, "tok_seat", torch.int32),
+        pointers(*[_dev(s, "slots", torch.int32) for s in slots]), _stream()), what)
+
+
 _MAX_SPLITS = None
 
 
