@@ -13,10 +13,20 @@
 // any order: atomics may add them up, and a row draws the same token whoever shares the launch with it.
 //
 // The order is one of 64-bit places, (the logit's bits, descending) above (the id): both cuts are a place, and what stays is what
-// lies in front of it.  A cut is found by counting: the places still in question are cut into 1,024 ranges, their numbers and
-// weights added up in LDS, and the range in which the sum passes what is sought is the next turn's.
+// lies in front of it.
 //
-// sample_truncated_kernel: a workgroup a row, which reads the row again in every turn.
+// Vocabularies of up to 262,144 take four launches, the first three of them with many workgroups a row, each of some steps of
+// 1,024 tokens:
+//   1. trunc_best_kernel     the best place of every workgroup's tokens
+//   2. trunc_bins_kernel     1,024 bins by the distance from the best, some 1/22 of a factor of two wide: how many tokens a bin has where
+//                            the row asks for k, their weight where it asks for p alone
+//   3. trunc_collect_kernel  finds the bin in which the cut lies and leaves a list of tokens: where k is asked for those of all bins up to
+//                            it (p's cut is among them), else those of this bin, and the sums of what lies in front of it by 256 ids
+//   4. trunc_pick_kernel     a workgroup a row: the cuts among the list's tokens, what stays by 256 ids, then the token among 256
+// A list has room for 4,096 tokens.  A row with more in the bin of its cut (nearly equal logits), or with a larger k among
+// them, is taken by the last kernel alone, as rows of larger vocabularies are by sample_truncated_kernel: a cut is found by counting, the places still in
+// question are cut into 1,024 ranges, their numbers and weights added up in LDS, and the range in which the sum passes what is
+// sought is the next turn's; the row is read again in every turn.
 #include "common.h"
 #include "counter_uniform.h"
 
@@ -109,14 +119,103 @@ __device__ inline void tr_block_prefix(TruncShared &s, u64 &v, unsigned &c) {
     for (int w = 0; w < wave; ++w) v += s.part[w], c += s.part_count[w];
 }
 
-// grid (rows)
-__global__ void __launch_bounds__(TR_THREADS)
-sample_truncated_kernel(TruncArgs a) {
-    __shared__ TruncShared s;
-    const int row = blockIdx.x, tid = threadIdx.x, vocab = a.vocab, bits = a.scale_bits;
+// What a row leaves: its token, how many stayed, its log-probability.
+struct TruncResult {
+    int token, kept;
+    float logprob;
+    __device__ inline void store(const TruncArgs &a, int row) const {
+        a.tokens[row] = token;
+        if (a.host_tokens != nullptr) a.host_tokens[row] = token;
+        if (a.kept != nullptr) a.kept[row] = kept;
+        if (a.logprob != nullptr) a.logprob[row] = logprob;
+    }
+};
+
+// A row that no weights decide: without a token, greedy, or without finite weights.  `at`: its best place (all ones: none)
+__device__ inline bool tr_decided(u64 at, float best, float inv_t, TruncResult &r) {
+    const bool none = at == ~0ull;
+    if (!none && inv_t > 0.f && best < INFINITY) return false;
+    if (none || inv_t > 0.f) r = TruncResult{TR_NO_TOKEN, 0, -INFINITY};
+    else r = TruncResult{(int)(unsigned)at, 1, 0.f};
+    return true;
+}
+
+__device__ inline double tr_rate(float inv_t) { return (double)inv_t * 1.4426950408889634; }
+
+// The weight that p's cut has to reach, of `total`.
+__device__ inline u64 tr_share(float p, u64 total) {
+    const double share = ceil((double)p * (double)total);
+    return share >= 1.0 ? min((u64)share, total) : 1ull;
+}
+
+// Whether a token that lies in front of the cuts stays, and its weight (0 if not).
+__device__ inline bool tr_stays(double octaves, double least, int bits, u64 &weight) {
+    const double w = octaves < bits + 1.0 ? exp2((double)bits - octaves) : 0.0;
+    if (least > 0.0 && octaves > 0.0 && !((octaves < bits + 1.0 ? w : exp2((double)bits - octaves)) >= ldexp(least, bits))) {
+        weight = 0;
+        return false;
+    }
+    weight = (u64)__double2ll_rn(w);
+    return true;
+}
+
+__device__ inline u64 tr_target(const TruncArgs &a, int row, u64 all) {
+    const float u = a.uniform != nullptr ? a.uniform[row] : counter_uniform(a.seed, a.key[row], a.step[row]);
+    const u64 target = u > 0.f ? (u64)(fmin((double)u, 1.0) * (double)all) : 0ull;
+    return min(target, all - 1);
+}
+
+__device__ inline float tr_logprob(double octaves, u64 all, int bits) {
+    return (float)(-0.6931471805599453 * (octaves + log2((double)all) - (double)bits));
+}
+
+// Of the places that each(f) hands to f(place, weight), from .. to: the one at which their number (by_count) or weight, with
+// `front` and `front_weight` in front of them, reaches `need`.  There is one.  `upto` gets the weight up to it.
+template <typename EACH>
+__device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u64 front, u64 front_weight, u64 need, u64 &upto, EACH each) {
+    const int tid = threadIdx.x;
+    while (true) {
+        const u64 span = to - from;
+        const int shift = span < TR_DIGITS ? 0 : 64 - __clzll((long long)span) - 10;
+        s.sum[tid] = 0;
+        s.count[tid] = 0;
+        __syncthreads();
+        each([&](u64 at, u64 weight) {
+            if (at < from || at > to) return;
+            const int digit = (int)((at - from) >> shift);
+            atomicAdd(&s.sum[digit], weight);
+            atomicAdd(&s.count[digit], 1u);
+        });
+        __syncthreads();
+        const u64 mine = s.sum[tid];
+        const unsigned n = s.count[tid];
+        u64 sum = mine;
+        unsigned count = n;
+        tr_block_prefix(s, sum, count);
+        const u64 reach = front + (by_count ? (u64)count : sum), behind = reach - (by_count ? (u64)n : mine);
+        if (behind < need && need <= reach) {           // (one thread's range)
+            s.found = tid;
+            s.above = behind;
+            s.lo = front_weight + sum - mine;
+            s.hi = front_weight + sum;
+        }
+        __syncthreads();
+        const int digit = s.found;
+        front = s.above;
+        front_weight = s.lo;
+        upto = s.hi;
+        __syncthreads();
+        from += (u64)digit << shift;
+        if (shift == 0) return from;
+        to = min(to, from + ((1ull << shift) - 1));
+    }
+}
+
+// A row by one workgroup that reads it in every turn.
+__device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s, int row) {
+    const int tid = threadIdx.x, vocab = a.vocab, bits = a.scale_bits;
     const float *rl = a.logits + row * a.stride;
     const float inv_t = a.inv_t[row];
-    const bool sampled = inv_t > 0.f;
     // the best place and the last one
     u64 lo = ~0ull, hi = 0;
     unsigned valid = 0;
@@ -128,144 +227,451 @@ sample_truncated_kernel(TruncArgs a) {
         hi = max(hi, at);
         ++valid;
     }
-    {
-        u64 none = 0;
-        tr_block_prefix(s, none, valid);
-        if (tid == TR_THREADS - 1) s.inside_count = valid;
-        tr_block_range(s, lo, hi);
-        valid = s.inside_count;
+    u64 none = 0;
+    tr_block_prefix(s, none, valid);
+    if (tid == TR_THREADS - 1) s.inside_count = valid;
+    tr_block_range(s, lo, hi);
+    valid = s.inside_count;
+    const float best = valid ? rl[(unsigned)lo] : 0.f;
+    TruncResult r;
+    if (tr_decided(lo, best, inv_t, r)) return r;
+    const double rate = tr_rate(inv_t);
+    auto each = [&](auto f) {
+        for (int t = tid; t < vocab; t += TR_THREADS) {
+            const float l = rl[t];
+            if (l > -INFINITY) f(tr_place(l, t), tr_weight(tr_octaves(best, l, rate), bits));
+        }
+    };
+    u64 last = hi, total = 0;               // the last place that stays, the weight up to it
+    const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+    const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
+    const double least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
+    if (k > 0 && (unsigned)k < valid) last = tr_cut(s, lo, hi, true, 0, 0, (u64)k, total, each);
+    if (p < 1.f) {
+        if (total == 0) {
+            u64 sum = 0;
+            unsigned unused = 0;
+            each([&](u64, u64 w) { sum += w; });
+            tr_block_prefix(s, sum, unused);
+            if (tid == TR_THREADS - 1) s.hi = sum;
+            __syncthreads();
+            total = s.hi;
+            __syncthreads();
+        }
+        last = tr_cut(s, lo, last, false, 0, 0, tr_share(p, total), total, each);
     }
-    const int best_id = (int)(unsigned)lo;
-    const float best = valid ? rl[best_id] : 0.f;
-    int token = valid ? best_id : TR_NO_TOKEN, kept = valid ? 1 : 0;
-    float logprob = valid ? 0.f : -INFINITY;
-    if (sampled && valid && best == INFINITY) token = TR_NO_TOKEN, kept = 0, logprob = -INFINITY;
-    if (sampled && token >= 0) {
-        const double rate = (double)inv_t * 1.4426950408889634;
-        // The place of the order's n-th token (by_count), or of the first at which the weights reach `need`, of those up to
-        // `hi`; `before` gets the weights in front of it, `weight` its own.  There is one.
-        auto cut = [&](u64 from, u64 to, bool by_count, u64 need, u64 &upto) {
-            u64 front = 0;                      // numbers or weights in front of `from`, and the weights alone
-            u64 front_weight = 0;
-            while (true) {
-                const u64 span = to - from;
-                const int shift = span < TR_DIGITS ? 0 : 64 - __clzll((long long)span) - 10;
-                s.sum[tid] = 0;
-                s.count[tid] = 0;
-                __syncthreads();
-                for (int t = tid; t < vocab; t += TR_THREADS) {
-                    const float l = rl[t];
-                    if (!(l > -INFINITY)) continue;
-                    const u64 at = tr_place(l, t);
-                    if (at < from || at > to) continue;
-                    const int digit = (int)((at - from) >> shift);
-                    atomicAdd(&s.sum[digit], tr_weight(tr_octaves(best, l, rate), bits));
-                    atomicAdd(&s.count[digit], 1u);
-                }
-                __syncthreads();
-                const u64 mine = s.sum[tid];
-                const unsigned n = s.count[tid];
-                u64 sum = mine;
-                unsigned count = n;
-                tr_block_prefix(s, sum, count);
-                const u64 reach = front + (by_count ? (u64)count : sum), behind = reach - (by_count ? (u64)n : mine);
-                if (behind < need && need <= reach) {           // (one thread's range)
-                    s.found = tid;
-                    s.above = behind;
-                    s.lo = front_weight + sum - mine;
-                    s.hi = front_weight + sum;
-                }
-                __syncthreads();
-                const int digit = s.found;
-                if (shift == 0) {
-                    upto = s.hi;
-                    const u64 at = from + (u64)digit;
-                    __syncthreads();
-                    return at;
-                }
-                front = s.above;
-                front_weight = s.lo;
-                from += (u64)digit << shift;
-                to = min(to, from + ((1ull << shift) - 1));
-                __syncthreads();
-            }
-        };
-        u64 last = hi, total = 0;               // the last place that stays, the weight up to it
-        const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-        const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
-        const double least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
-        if (k > 0 && (unsigned)k < valid) last = cut(lo, hi, true, (u64)k, total);
-        if (p < 1.f) {
-            if (total == 0) {
-                u64 sum = 0;
-                unsigned none = 0;
-                for (int t = tid; t < vocab; t += TR_THREADS)
-                    if (rl[t] > -INFINITY) sum += tr_weight(tr_octaves(best, rl[t], rate), bits);
-                tr_block_prefix(s, sum, none);
-                if (tid == TR_THREADS - 1) s.hi = sum;
-                __syncthreads();
-                total = s.hi;
-                __syncthreads();
-            }
-            const double share = ceil((double)p * (double)total);
-            const u64 need = share >= 1.0 ? min((u64)share, total) : 1ull;
-            last = cut(lo, last, false, need, total);
-        }
-        // what stays, by ids: ranges of ids first, then the tokens of one
-        const int per = (vocab + TR_THREADS - 1) / TR_THREADS;
-        auto stays = [&](float l, int t, u64 &weight) {
-            weight = 0;
-            if (!(l > -INFINITY) || tr_place(l, t) > last) return false;
-            const double octaves = tr_octaves(best, l, rate);
-            weight = tr_weight(octaves, bits);
-            if (least > 0.0 && octaves > 0.0 && !(exp2(-octaves) >= least)) {
-                weight = 0;
-                return false;
-            }
-            return true;
-        };
-        u64 sum = 0;
-        unsigned count = 0;
-        for (int t = tid * per; t < min(vocab, (tid + 1) * per); ++t) {
-            u64 w;
-            if (stays(rl[t], t, w)) ++count;
-            sum += w;
-        }
-        const u64 mine = sum;
-        tr_block_prefix(s, sum, count);
-        if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
-        __syncthreads();
-        const u64 all = s.hi;
-        kept = (int)s.inside_count;
-        const float u = a.uniform != nullptr ? a.uniform[row] : counter_uniform(a.seed, a.key[row], a.step[row]);
-        u64 target = u > 0.f ? (u64)(fmin((double)u, 1.0) * (double)all) : 0ull;
-        target = min(target, all - 1);
-        if (sum - mine <= target && target < sum) {
-            u64 run = sum - mine, w = 0;
-            int t = tid * per;
-            for (;; ++t) {
-                stays(rl[t], t, w);
-                run += w;
-                if (target < run) break;
-            }
-            s.found = t;
-        }
-        __syncthreads();
-        token = s.found;
-        logprob = (float)(-0.6931471805599453 * (tr_octaves(best, rl[token], rate) + log2((double)all) - (double)bits));
+    // what stays, by ids: a range of them a thread, then the tokens of one
+    const int per = (vocab + TR_THREADS - 1) / TR_THREADS;
+    auto weight = [&](int t, u64 &w) {
+        w = 0;
+        const float l = rl[t];
+        return l > -INFINITY && tr_place(l, t) <= last && tr_stays(tr_octaves(best, l, rate), least, bits, w);
+    };
+    u64 sum = 0;
+    unsigned count = 0;
+    for (int t = tid * per; t < min(vocab, (tid + 1) * per); ++t) {
+        u64 w;
+        if (weight(t, w)) ++count;
+        sum += w;
     }
+    const u64 mine = sum;
+    tr_block_prefix(s, sum, count);
+    if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
+    __syncthreads();
+    const u64 all = s.hi, target = tr_target(a, row, all);
+    if (sum - mine <= target && target < sum) {         // (one thread's)
+        u64 run = sum - mine, w;
+        int t = tid * per;
+        for (;; ++t) {
+            weight(t, w);
+            run += w;
+            if (target < run) break;
+        }
+        s.found = t;
+    }
+    __syncthreads();
+    return TruncResult{s.found, (int)s.inside_count, tr_logprob(tr_octaves(best, rl[s.found], rate), all, bits)};
+}
+
+// grid (rows)
+__global__ void __launch_bounds__(TR_THREADS)
+sample_truncated_kernel(TruncArgs a) {
+    __shared__ TruncShared s;
+    const TruncResult r = trunc_whole_row(a, s, blockIdx.x);
+    if (threadIdx.x == 0) r.store(a, blockIdx.x);
+}
+
+// ---------------------------------------------------------------- many workgroups a row
+#define TR_BINS 1024
+#define TR_LIST 4096
+#define TR_PAIRS 256                    // so many tokens are compared with one another
+#define TR_STEP 1024                    // tokens a workgroup takes at a time: 256 threads, 4 neighbouring tokens each
+#define TR_BUCKET 256                   // ... and a wavefront of them
+#define TR_SPLIT_THREADS 256
+#define TR_MAX_PARTS 128
+#define TR_MAX_VOCAB (TR_BUCKET * TR_THREADS)
+
+struct TruncSpace {                     // of all rows
+    u64 *best;                          // [parts]
+    u64 *bins;                          // [TR_BINS]
+    u64 *sums;                          // [buckets]: what stays for certain, by ids
+    unsigned *counts;                   // [buckets]
+    int *list;                          // [TR_LIST]
+    int *listed;                        // [1]: tokens that asked for a place in the list
+    int parts, part_tokens, buckets;
+};
+
+// What a row's cut is found by: nothing, the number of tokens up to a bin, or their weight.
+enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2 };
+__device__ inline int tr_mode(const TruncArgs &a, int row) {
+    const int k = a.top_k != nullptr ? a.top_k[row] : 0;
+    if (k > 0 && k < a.vocab) return TR_COUNT;
+    return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
+}
+
+// The last bin takes what weighs nothing.
+__device__ inline int tr_bin(double octaves, int bits) {
+    return octaves < bits + 1.0 ? (int)(octaves * ((TR_BINS - 1) / (bits + 1.0))) : TR_BINS - 1;
+}
+
+typedef float tr_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Four neighbouring logits from token t on; what lies behind the vocabulary is -inf.
+__device__ inline void tr_load4(const float *rl, int t, int vocab, float (&l)[4]) {
+    if (t + 3 < vocab) {
+        const tr_f32x4 v = *reinterpret_cast<const tr_f32x4 *>(rl + t);
+        l[0] = v.x, l[1] = v.y, l[2] = v.z, l[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] = t + i < vocab ? rl[t + i] : -INFINITY;
+    }
+}
+
+__device__ inline u64 tr_wave_min(u64 v) {
+#pragma unroll
+    for (int off = KVA_WAVE / 2; off > 0; off >>= 1) v = min(v, (u64)__shfl_xor(v, off, KVA_WAVE));
+    return v;
+}
+
+// The best place of a row, from its parts' (every wavefront for itself).
+__device__ inline u64 tr_best(const TruncSpace &sp, int row) {
+    u64 at = ~0ull;
+    for (int c = threadIdx.x % KVA_WAVE; c < sp.parts; c += KVA_WAVE) at = min(at, sp.best[(size_t)row * sp.parts + c]);
+    return tr_wave_min(at);
+}
+
+// grid (parts, rows)
+__global__ void __launch_bounds__(TR_SPLIT_THREADS)
+trunc_best_kernel(TruncArgs a, TruncSpace sp) {
+    __shared__ u64 of_wave[TR_SPLIT_THREADS / KVA_WAVE];
+    const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
+    const float *rl = a.logits + row * a.stride;
+    // (the next launches add to these)
+    const int per = (TR_BINS + sp.parts - 1) / sp.parts;
+    for (int i = part * per + tid; i < min(TR_BINS, (part + 1) * per); i += TR_SPLIT_THREADS) sp.bins[(size_t)row * TR_BINS + i] = 0;
+    if (part == 0 && tid == 0) sp.listed[row] = 0;
+    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
+    float top = -INFINITY;
+    int id = 0;
+    for (int t = part * sp.part_tokens + 4 * tid; t < end; t += TR_STEP) {
+        float l[4];
+        tr_load4(rl, t, a.vocab, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (l[i] > top) top = l[i], id = t + i;     // (ascending ids: the first of equal ones)
+    }
+    u64 at = tr_wave_min(top > -INFINITY ? tr_place(top, id) : ~0ull);
+    if (tid % KVA_WAVE == 0) of_wave[tid / KVA_WAVE] = at;
+    __syncthreads();
     if (tid == 0) {
-        a.tokens[row] = token;
-        if (a.host_tokens != nullptr) a.host_tokens[row] = token;
-        if (a.kept != nullptr) a.kept[row] = kept;
-        if (a.logprob != nullptr) a.logprob[row] = logprob;
+        for (int w = 1; w < TR_SPLIT_THREADS / KVA_WAVE; ++w) at = min(at, of_wave[w]);
+        sp.best[(size_t)row * sp.parts + part] = at;
     }
+}
+
+// grid (parts, rows)
+__global__ void __launch_bounds__(TR_SPLIT_THREADS)
+trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
+    __shared__ u64 bins[TR_BINS];
+    const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, bits = a.scale_bits;
+    const float inv_t = a.inv_t[row];
+    const int mode = tr_mode(a, row);
+    if (!(inv_t > 0.f) || mode == TR_ALL) return;
+    for (int i = tid; i < TR_BINS; i += TR_SPLIT_THREADS) bins[i] = 0;
+    const float *rl = a.logits + row * a.stride;
+    const u64 at = tr_best(sp, row);
+    if (at == ~0ull) return;
+    const float best = rl[(unsigned)at];
+    const double rate = tr_rate(inv_t);
+    __syncthreads();
+    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
+    for (int t = part * sp.part_tokens + 4 * tid; t < end; t += TR_STEP) {
+        float l[4];
+        tr_load4(rl, t, a.vocab, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (!(l[i] > -INFINITY)) continue;
+            const double octaves = tr_octaves(best, l[i], rate);
+            const int bin = tr_bin(octaves, bits);
+            if (mode == TR_COUNT) atomicAdd(&bins[bin], 1ull);
+            else if (bin < TR_BINS - 1) atomicAdd(&bins[bin], tr_weight(octaves, bits));
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < TR_BINS; i += TR_SPLIT_THREADS)
+        if (bins[i] != 0) atomicAdd(&sp.bins[(size_t)row * TR_BINS + i], bins[i]);
+}
+
+// grid (parts, rows)
+__global__ void __launch_bounds__(TR_SPLIT_THREADS)
+trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
+    __shared__ u64 of_wave[TR_SPLIT_THREADS / KVA_WAVE];
+    __shared__ int cut_bin;
+    const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, bits = a.scale_bits;
+    const float inv_t = a.inv_t[row];
+    if (!(inv_t > 0.f)) return;
+    const int mode = tr_mode(a, row);
+    const float *rl = a.logits + row * a.stride;
+    const u64 at = tr_best(sp, row);
+    if (at == ~0ull) return;
+    const float best = rl[(unsigned)at];
+    if (!(best < INFINITY)) return;
+    int cut = TR_BINS;                      // the bin in which the cut lies; past the last: everything stays
+    if (mode != TR_ALL) {
+        u64 v[TR_BINS / TR_SPLIT_THREADS], mine = 0;
+#pragma unroll
+        for (int i = 0; i < TR_BINS / TR_SPLIT_THREADS; ++i) {
+            v[i] = sp.bins[(size_t)row * TR_BINS + tid * (TR_BINS / TR_SPLIT_THREADS) + i];
+            mine += v[i];
+        }
+        u64 upto = tr_wave_prefix(mine);
+        if (lane == KVA_WAVE - 1) of_wave[wave] = upto;
+        if (tid == 0) cut_bin = TR_BINS - 1;            // (fewer tokens than k: all of them)
+        __syncthreads();
+        u64 total = 0;
+#pragma unroll
+        for (int w = 0; w < TR_SPLIT_THREADS / KVA_WAVE; ++w) {
+            if (w < wave) upto += of_wave[w];
+            total += of_wave[w];
+        }
+        const u64 need = mode == TR_COUNT ? (u64)a.top_k[row] : tr_share(a.top_p[row], total);
+        u64 run = upto - mine;
+        if (run < need && need <= upto) {
+#pragma unroll
+            for (int i = 0; i < TR_BINS / TR_SPLIT_THREADS; ++i) {
+                if (run < need && need <= run + v[i]) cut_bin = tid * (TR_BINS / TR_SPLIT_THREADS) + i;
+                run += v[i];
+            }
+        }
+        __syncthreads();
+        cut = cut_bin;
+    }
+    const double rate = tr_rate(inv_t), least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
+    int *list = sp.list + (size_t)row * TR_LIST;
+    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
+    for (int t0 = part * sp.part_tokens; t0 < end; t0 += TR_STEP) {
+        const int t = t0 + 4 * tid;
+        float l[4];
+        tr_load4(rl, t, a.vocab, l);
+        u64 sum = 0;
+        unsigned count = 0, asks = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (!(l[i] > -INFINITY)) continue;
+            const double octaves = tr_octaves(best, l[i], rate);
+            const int bin = mode == TR_ALL ? 0 : tr_bin(octaves, bits);
+            if (bin > cut) continue;
+            if (mode == TR_COUNT || bin == cut) {
+                asks |= 1u << i;
+            } else {
+                u64 w;
+                if (tr_stays(octaves, least, bits, w)) ++count;
+                sum += w;
+            }
+        }
+        if (mode != TR_COUNT) {
+            // 256 ids of this wavefront
+#pragma unroll
+            for (int off = KVA_WAVE / 2; off > 0; off >>= 1) {
+                sum += __shfl_xor(sum, off, KVA_WAVE);
+                count += __shfl_xor(count, off, KVA_WAVE);
+            }
+            const int bucket = t0 / TR_BUCKET + wave;
+            if (lane == 0 && bucket < sp.buckets) {
+                sp.sums[(size_t)row * sp.buckets + bucket] = sum;
+                sp.counts[(size_t)row * sp.buckets + bucket] = count;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned long long votes = __ballot(asks >> i & 1);
+            if (votes == 0) continue;
+            int from = 0;
+            if (lane == 0) from = atomicAdd(&sp.listed[row], (int)__popcll(votes));
+            from = __shfl(from, 0, KVA_WAVE) + (int)__popcll(votes & ((1ull << lane) - 1));
+            if ((asks >> i & 1) && from < TR_LIST) list[from] = t + i;
+        }
+    }
+}
+
+// grid (rows)
+__global__ void __launch_bounds__(TR_THREADS)
+trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
+    __shared__ TruncShared s;
+    __shared__ u64 place[TR_LIST], heavy[TR_PAIRS];
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid % KVA_WAVE, bits = a.scale_bits, vocab = a.vocab;
+    const float *rl = a.logits + row * a.stride;
+    const float inv_t = a.inv_t[row];
+    const u64 first = tr_best(sp, row);
+    const float best = first == ~0ull ? 0.f : rl[(unsigned)first];
+    TruncResult r;
+    if (tr_decided(first, best, inv_t, r)) {
+        if (tid == 0) r.store(a, row);
+        return;
+    }
+    const int mode = tr_mode(a, row), n = mode == TR_ALL ? 0 : sp.listed[row];
+    if (n > TR_LIST) {
+        r = trunc_whole_row(a, s, row);
+        if (tid == 0) r.store(a, row);
+        return;
+    }
+    const double rate = tr_rate(inv_t), least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
+    const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
+    u64 last = ~0ull;                       // the last place that stays
+    for (int i = tid; i < n; i += TR_THREADS) {
+        const int id = sp.list[(size_t)row * TR_LIST + i];
+        place[i] = tr_place(rl[id], id);
+    }
+    auto octaves_of = [&](u64 at) { return tr_octaves(best, rl[(unsigned)at], rate); };
+    if (mode != TR_ALL) {
+        // what lies in front of the list's tokens, and what is sought
+        u64 front = 0, need = 0;
+        if (mode == TR_WEIGHT) {
+            const u64 mine = sp.bins[(size_t)row * TR_BINS + tid];
+            u64 upto = mine;
+            unsigned unused = 0;
+            tr_block_prefix(s, upto, unused);
+            if (tid == TR_THREADS - 1) s.hi = upto;
+            __syncthreads();
+            need = tr_share(p, s.hi);
+            if (upto - mine < need && need <= upto) s.above = upto - mine;
+            __syncthreads();
+            front = s.above;
+        } else {
+            need = (u64)min(a.top_k[row], n);
+        }
+        if (n <= TR_PAIRS) {
+            // four threads a token add up what lies in front of it
+            const int j = tid / 4;
+            if (tid < n) heavy[tid] = tr_weight(octaves_of(place[tid]), bits);
+            __syncthreads();
+            u64 upto = front;
+            int rank = 0;
+            const u64 me = j < n ? place[j] : 0;
+            for (int i = tid % 4; i < n; i += 4) {
+                if (place[i] <= me) upto += heavy[i], ++rank;
+            }
+            upto -= tid % 4 ? front : 0;
+#pragma unroll
+            for (int off = 1; off < 4; off <<= 1) {
+                upto += __shfl_xor(upto, off, KVA_WAVE);
+                rank += __shfl_xor(rank, off, KVA_WAVE);
+            }
+            if (tid == 0) s.lo = ~0ull;
+            if (mode == TR_COUNT) {
+                if (j < n && tid % 4 == 0 && (u64)rank == need) s.hi = upto, s.above = me;       // (ranks are 1 .. n, one each)
+                __syncthreads();
+                last = s.above;
+                need = p < 1.f ? tr_share(p, s.hi) : ~0ull;
+            } else {
+                __syncthreads();
+            }
+            if (need != ~0ull) {
+                if (j < n && tid % 4 == 0 && upto >= need) atomicMin(&s.lo, me);
+                __syncthreads();
+                last = s.lo;
+            }
+        } else {
+            __syncthreads();
+            u64 from = ~0ull, to = 0, total = 0;
+            for (int i = tid; i < n; i += TR_THREADS) from = min(from, place[i]), to = max(to, place[i]);
+            tr_block_range(s, from, to);
+            auto each = [&](auto f) {
+                for (int i = tid; i < n; i += TR_THREADS) f(place[i], tr_weight(octaves_of(place[i]), bits));
+            };
+            last = tr_cut(s, from, to, mode == TR_COUNT, front, front, need, total, each);
+            if (mode == TR_COUNT && p < 1.f) last = tr_cut(s, from, last, false, 0, 0, tr_share(p, total), total, each);
+        }
+    }
+    // what stays, by 256 ids: a thread each
+    __syncthreads();
+    const bool inside = tid < sp.buckets && mode != TR_COUNT;
+    s.sum[tid] = inside ? sp.sums[(size_t)row * sp.buckets + tid] : 0;
+    s.count[tid] = inside ? sp.counts[(size_t)row * sp.buckets + tid] : 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += TR_THREADS) {
+        u64 w;
+        if (place[i] > last || !tr_stays(octaves_of(place[i]), least, bits, w)) continue;
+        atomicAdd(&s.sum[(unsigned)place[i] / TR_BUCKET], w);
+        atomicAdd(&s.count[(unsigned)place[i] / TR_BUCKET], 1u);
+    }
+    __syncthreads();
+    const u64 mine = s.sum[tid];
+    u64 sum = mine;
+    unsigned count = s.count[tid];
+    tr_block_prefix(s, sum, count);
+    if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
+    __syncthreads();
+    const u64 all = s.hi, target = tr_target(a, row, all);
+    if (sum - mine <= target && target < sum) s.found = tid, s.above = sum - mine;
+    __syncthreads();
+    if (tid >= KVA_WAVE) return;
+    // the token: four neighbouring ones a lane
+    const int t = s.found * TR_BUCKET + 4 * lane;
+    float l[4];
+    u64 w[4];
+    tr_load4(rl, t, vocab, l);
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = 0;
+        if (l[i] > -INFINITY && tr_place(l[i], t + i) <= last) tr_stays(tr_octaves(best, l[i], rate), least, bits, w[i]);
+        sum += w[i];
+    }
+    u64 run = s.above + tr_wave_prefix(sum) - sum;
+    if (run <= target && target < run + sum) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (run <= target && target < run + w[i])
+                TruncResult{t + i, (int)s.inside_count, tr_logprob(tr_octaves(best, l[i], rate), all, bits)}.store(a, row);
+            run += w[i];
+        }
+    }
+}
+
+// How many workgroups a row gets in the first three launches, and their tokens.
+static int trunc_parts(int rows, int vocab, int *part_tokens) {
+    const int steps = (vocab + TR_STEP - 1) / TR_STEP;
+    int parts = (2048 + rows - 1) / rows;
+    parts = parts < 1 ? 1 : parts > TR_MAX_PARTS ? TR_MAX_PARTS : parts;
+    parts = parts > steps ? steps : parts;
+    *part_tokens = (steps + parts - 1) / parts * TR_STEP;
+    return (vocab + *part_tokens - 1) / *part_tokens;
+}
+
+static bool trunc_split(int vocab) { return vocab > 4096 && vocab <= TR_MAX_VOCAB; }
+
+extern "C" long long kva_sample_truncated_workspace_bytes(int rows, int vocab) {
+    if (rows <= 0 || !trunc_split(vocab)) return 0;
+    int part_tokens;
+    const long long parts = trunc_parts(rows, vocab, &part_tokens), buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
+    return rows * (8 * (parts + TR_BINS + buckets) + 4 * (buckets + TR_LIST + 1));
 }
 
 extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long stride, int rows, int vocab, const float *inv_t,
                                     const int *top_k, const float *top_p, const float *min_p, const float *uniform, unsigned seed,
                                     const unsigned *key, const unsigned *step, int *kept, float *logprob, int *host_tokens,
-                                    hipStream_t stream) {
+                                    void *workspace, hipStream_t stream) {
     int *host_mapped = nullptr;
     if (host_tokens != nullptr) {
         void *dev = nullptr;
@@ -283,7 +689,26 @@ extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long 
     while ((1 << log_vocab) < vocab) ++log_vocab;
     const int bits = log_vocab > 16 ? 62 - log_vocab : 46;
     const TruncArgs a{logits, stride, vocab, bits, inv_t, top_k, top_p, min_p, uniform, seed, key, step, tokens, host_mapped, kept, logprob};
-    hipLaunchKernelGGL(sample_truncated_kernel, dim3(rows), dim3(TR_THREADS), 0, stream, a);
+    if (!trunc_split(vocab)) {
+        hipLaunchKernelGGL(sample_truncated_kernel, dim3(rows), dim3(TR_THREADS), 0, stream, a);
+        KVA_CHECK_LAUNCH("sample_truncated");
+        return KVA_OK;
+    }
+    KVA_REQUIRE(workspace != nullptr && (uintptr_t)workspace % 8 == 0, "sample_truncated: a workspace of kva_sample_truncated_workspace_bytes is needed");
+    TruncSpace sp;
+    sp.parts = trunc_parts(rows, vocab, &sp.part_tokens);
+    sp.buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
+    sp.best = (u64 *)workspace;
+    sp.bins = sp.best + (size_t)rows * sp.parts;
+    sp.sums = sp.bins + (size_t)rows * TR_BINS;
+    sp.counts = (unsigned *)(sp.sums + (size_t)rows * sp.buckets);
+    sp.list = (int *)(sp.counts + (size_t)rows * sp.buckets);
+    sp.listed = sp.list + (size_t)rows * TR_LIST;
+    const dim3 grid(sp.parts, rows), block(TR_SPLIT_THREADS);
+    hipLaunchKernelGGL(trunc_best_kernel, grid, block, 0, stream, a, sp);
+    hipLaunchKernelGGL(trunc_bins_kernel, grid, block, 0, stream, a, sp);
+    hipLaunchKernelGGL(trunc_collect_kernel, grid, block, 0, stream, a, sp);
+    hipLaunchKernelGGL(trunc_pick_kernel, dim3(rows), dim3(TR_THREADS), 0, stream, a, sp);
     KVA_CHECK_LAUNCH("sample_truncated");
     return KVA_OK;
 }

@@ -1331,9 +1331,13 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
                                       uniform=uniform, logprob=logprob)
     tok, k, key, step, n = _per_row(what, rows, torch.int32, out_tokens=out_tokens, top_k=top_k, rng_key=rng_key, rng_step=rng_step,
                                     kept=kept)
-    check(hip_lib().kva_sample_truncated(
+    lib = hip_lib()
+    size = lib.kva_sample_truncated_workspace_bytes(rows, vocab)
+    space = torch.empty(size // 4, dtype=torch.int32, device=logits.device) if size else None
+    check(lib.kva_sample_truncated(
         tok, _dev(logits, "logits", torch.float32, contiguous=False), stride, rows, vocab, inv_t, k, p, least, u, int(seed) & 0xFFFFFFFF,
-        key, step, n, lp, ctypes.c_void_p(host_tokens.data_ptr()) if host_tokens is not None else None, _stream()), what)
+        key, step, n, lp, ctypes.c_void_p(host_tokens.data_ptr()) if host_tokens is not None else None,
+        space.data_ptr() if space is not None else None, _stream()), what)
     return out_tokens
 
 

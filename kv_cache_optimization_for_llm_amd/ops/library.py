@@ -102,7 +102,7 @@ _HIP_SIGNATURES = {
     "kva_event_synchronize": [P],
     "kva_event_destroy": [P],
     "kva_mark_tokens": [P, P, P, I, I, P],
-    "kva_sample_truncated": [P, P, LL, I, I, P, P, P, P, P, U, P, P, P, P, P, P],
+    "kva_sample_truncated": [P, P, LL, I, I, P, P, P, P, P, U, P, P, P, P, P, P, P],
     "kva_adjust_logits": [P, LL, P, I, LL, I, I, P, I, P, P, P, P, P, P, P, P, I, P, P, I, P],
     "kva_count_tokens": [P, P, I, I, P, P, I, P],
     "kva_grow_tables": [P, I, I, P, P, P, I, I, P, I, P, P],
@@ -177,6 +177,8 @@ def hip_lib():
         lib.kva_last_error.restype = c_char_p
         lib.kva_sample_workspace_bytes.argtypes = [I, I]
         lib.kva_sample_workspace_bytes.restype = LL
+        lib.kva_sample_truncated_workspace_bytes.argtypes = [I, I]
+        lib.kva_sample_truncated_workspace_bytes.restype = LL
         lib.kva_state_space_workspace.argtypes = [I, I, I, I, I]
         lib.kva_state_space_workspace.restype = LL
         lib.kva_recurrent_chunks_workspace.argtypes = [I, I, I, I]
