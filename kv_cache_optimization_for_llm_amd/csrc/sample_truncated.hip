@@ -58,49 +58,92 @@ __device__ inline unsigned tr_falling(float l) {
 }
 __device__ inline u64 tr_place(float l, int id) { return (u64)tr_falling(l) << 32 | (unsigned)id; }
 
-// how far below the best one a logit lies, in units of log2(weight)
-__device__ inline double tr_octaves(float best, float l, double octaves_per_unit) {
-    const double d = (double)best - (double)l;
-    return d == 0.0 ? 0.0 : d * octaves_per_unit;
-}
-// round(2^bits 2^-octaves)
-__device__ inline u64 tr_weight(double octaves, int bits) {
-    return octaves < bits + 1.0 ? (u64)__double2ll_rn(exp2((double)bits - octaves)) : 0ull;
+// ... and back
+__device__ inline float tr_logit(u64 place) {
+    const unsigned k = (unsigned)(place >> 32);
+    return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu);
 }
 
-__device__ inline u64 tr_wave_prefix(u64 v) {
-    const int lane = threadIdx.x % KVA_WAVE;
-#pragma unroll
-    for (int off = 1; off < KVA_WAVE; off <<= 1) {
-        const u64 below = __shfl_up(v, off, KVA_WAVE);
-        if (lane >= off) v += below;
-    }
-    return v;
+// how far below the best one a logit lies, in units of log2(weight)
+__device__ inline double tr_octaves(float best, float l, double rate) {
+    const double d = (double)best - (double)l;
+    return d == 0.0 ? 0.0 : d * rate;
 }
+
+// round(2^bits 2^-octaves).  2^f for f from -1/2 to 1/2 by a polynomial through the eleven Chebyshev nodes (4e-16 off, 1 at 0); a number
+// below 2^52 and 2^52 add up to one whose last bits are the number's whole part, rounded.
+__device__ inline u64 tr_weight(double octaves, int bits) {
+    const double z = fmax((double)bits - octaves, -4.0), n = rint(z), f = z - n;
+    double p = 7.072585949269224e-09;
+    p = fma(p, f, 1.0208690299958306e-07);
+    p = fma(p, f, 1.321544258792169e-06);
+    p = fma(p, f, 1.5252657260200837e-05);
+    p = fma(p, f, 0.0001540353044173605);
+    p = fma(p, f, 0.0013333558230164974);
+    p = fma(p, f, 0.009618129107606888);
+    p = fma(p, f, 0.05550410866444772);
+    p = fma(p, f, 0.24022650695910097);
+    p = fma(p, f, 0.69314718055995);
+    p = fma(p, f, 1.0);
+    const double w = ldexp(p, (int)n) + 4503599627370496.0;
+    return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+}
+
+// Numbers from lanes in front of this one, or `none` where there is no such lane.
+template <int CTRL, int ROWS>
+__device__ inline unsigned tr_from(unsigned v, unsigned none) {
+    return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ inline u64 tr_from(u64 v, u64 none) {
+    return (u64)tr_from<CTRL, ROWS>((unsigned)(v >> 32), (unsigned)(none >> 32)) << 32 | tr_from<CTRL, ROWS>((unsigned)v, (unsigned)none);
+}
+// Inclusive prefix of the wavefront in the vector ALU: 1, 2, 4 and 8 lanes up inside rows of 16, then the last lane of a row to the
+// next one, then that of the first half to the second.
+template <typename T, typename OP>
+__device__ inline T tr_wave_scan(T v, T none, OP op) {
+    v = op(v, tr_from<0x111, 0xf>(v, none));
+    v = op(v, tr_from<0x112, 0xf>(v, none));
+    v = op(v, tr_from<0x114, 0xf>(v, none));
+    v = op(v, tr_from<0x118, 0xf>(v, none));
+    v = op(v, tr_from<0x142, 0xa>(v, none));
+    return op(v, tr_from<0x143, 0xc>(v, none));
+}
+template <typename T>
+__device__ inline T tr_wave_prefix(T v) {
+    return tr_wave_scan(v, (T)0, [](T a, T b) { return a + b; });
+}
+__device__ inline unsigned tr_last_lane(unsigned v) { return __builtin_amdgcn_readlane(v, KVA_WAVE - 1); }
+__device__ inline u64 tr_last_lane(u64 v) { return (u64)tr_last_lane((unsigned)(v >> 32)) << 32 | tr_last_lane((unsigned)v); }
+__device__ inline u64 tr_wave_min(u64 v) {
+    return tr_last_lane(tr_wave_scan(v, ~0ull, [](u64 a, u64 b) { return a < b ? a : b; }));
+}
+__device__ inline u64 tr_wave_max(u64 v) {
+    return tr_last_lane(tr_wave_scan(v, 0ull, [](u64 a, u64 b) { return a > b ? a : b; }));
+}
+
+#define TR_PAIRS 256                    // so many tokens are compared with one another
 
 struct TruncShared {
     u64 sum[TR_DIGITS];
     unsigned count[TR_DIGITS];
     u64 part[TR_WAVES];
     unsigned part_count[TR_WAVES];
+    u64 place[TR_PAIRS], weight[TR_PAIRS];
     u64 lo, hi, above;
-    unsigned above_count, inside_count;
+    unsigned inside_count, gathered;
     int found;
 };
 
 // The smallest of all threads' numbers and the largest.
 __device__ inline void tr_block_range(TruncShared &s, u64 &lo, u64 &hi) {
-#pragma unroll
-    for (int off = KVA_WAVE / 2; off > 0; off >>= 1) {
-        const u64 a = __shfl_xor(lo, off, KVA_WAVE), b = __shfl_xor(hi, off, KVA_WAVE);
-        lo = min(lo, a);
-        hi = max(hi, b);
-    }
+    lo = tr_wave_min(lo);
+    hi = tr_wave_max(hi);
     __syncthreads();
     if (threadIdx.x % KVA_WAVE == 0) s.sum[threadIdx.x / KVA_WAVE] = lo, s.part[threadIdx.x / KVA_WAVE] = hi;
     __syncthreads();
-    lo = s.sum[0], hi = s.part[0];
-    for (int w = 1; w < TR_WAVES; ++w) lo = min(lo, s.sum[w]), hi = max(hi, s.part[w]);
+#pragma unroll
+    for (int w = 0; w < TR_WAVES; ++w) lo = min(lo, s.sum[w]), hi = max(hi, s.part[w]);
     __syncthreads();
 }
 
@@ -108,15 +151,54 @@ __device__ inline void tr_block_range(TruncShared &s, u64 &lo, u64 &hi) {
 __device__ inline void tr_block_prefix(TruncShared &s, u64 &v, unsigned &c) {
     const int lane = threadIdx.x % KVA_WAVE, wave = threadIdx.x / KVA_WAVE;
     v = tr_wave_prefix(v);
-#pragma unroll
-    for (int off = 1; off < KVA_WAVE; off <<= 1) {
-        const unsigned below = __shfl_up(c, off, KVA_WAVE);
-        if (lane >= off) c += below;
-    }
+    c = tr_wave_prefix(c);
     __syncthreads();
     if (lane == KVA_WAVE - 1) s.part[wave] = v, s.part_count[wave] = c;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) v += s.part[w], c += s.part_count[w];
+#pragma unroll
+    for (int w = 0; w < TR_WAVES - 1; ++w) {
+        const u64 part = s.part[w];
+        const unsigned part_count = s.part_count[w];
+        if (w < wave) v += part, c += part_count;
+    }
+}
+
+// Up to 256 tokens, their places in s.place: how many of them and what weight (beside `front`) lies up to each of them, itself
+// included.  Four threads a token, which all get it.
+struct PairSums {
+    bool on;
+    u64 place, upto;
+    unsigned rank;
+};
+template <typename WEIGHT>
+__device__ inline PairSums tr_pairs(TruncShared &s, int n, u64 front, WEIGHT weight) {
+    const int tid = threadIdx.x, j = tid / 4;
+    if (tid < n) s.weight[tid] = weight(s.place[tid]);
+    if (tid == 0) s.lo = ~0ull;
+    __syncthreads();
+    PairSums r{j < n, j < n ? s.place[j] : 0, 0, 0};
+    for (int i = tid % 4; i < n; i += 4)
+        if (s.place[i] <= r.place) r.upto += s.weight[i], ++r.rank;
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+        r.upto += __shfl_xor(r.upto, off, KVA_WAVE);
+        r.rank += __shfl_xor(r.rank, off, KVA_WAVE);
+    }
+    r.upto += front;
+    return r;
+}
+// The place of the need-th of them, and the weight up to it.
+__device__ inline u64 tr_pair_by_count(TruncShared &s, const PairSums &r, unsigned need, u64 &upto) {
+    if (r.on && r.rank == need) s.above = r.place, s.hi = r.upto;       // (four threads, the same)
+    __syncthreads();
+    upto = s.hi;
+    return s.above;
+}
+// The first place up to which the weight reaches `need` (once after tr_pairs).
+__device__ inline u64 tr_pair_by_weight(TruncShared &s, const PairSums &r, u64 need) {
+    if (r.on && threadIdx.x % 4 == 0 && r.upto >= need) atomicMin(&s.lo, r.place);
+    __syncthreads();
+    return s.lo;
 }
 
 // What a row leaves: its token, how many stayed, its log-probability.
@@ -148,15 +230,10 @@ __device__ inline u64 tr_share(float p, u64 total) {
     return share >= 1.0 ? min((u64)share, total) : 1ull;
 }
 
-// Whether a token that lies in front of the cuts stays, and its weight (0 if not).
-__device__ inline bool tr_stays(double octaves, double least, int bits, u64 &weight) {
-    const double w = octaves < bits + 1.0 ? exp2((double)bits - octaves) : 0.0;
-    if (least > 0.0 && octaves > 0.0 && !((octaves < bits + 1.0 ? w : exp2((double)bits - octaves)) >= ldexp(least, bits))) {
-        weight = 0;
-        return false;
-    }
-    weight = (u64)__double2ll_rn(w);
-    return true;
+// How far below the best one a token may lie to stay (the best ones stay in any case).
+__device__ inline double tr_limit(const TruncArgs &a, int row) {
+    const float least = a.min_p != nullptr ? a.min_p[row] : 0.f;
+    return least > 0.f ? fmax(-log2((double)least), 0.0) : INFINITY;
 }
 
 __device__ inline u64 tr_target(const TruncArgs &a, int row, u64 all) {
@@ -169,21 +246,23 @@ __device__ inline float tr_logprob(double octaves, u64 all, int bits) {
     return (float)(-0.6931471805599453 * (octaves + log2((double)all) - (double)bits));
 }
 
-// Of the places that each(f) hands to f(place, weight), from .. to: the one at which their number (by_count) or weight, with
-// `front` and `front_weight` in front of them, reaches `need`.  There is one.  `upto` gets the weight up to it.
-template <typename EACH>
-__device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u64 front, u64 front_weight, u64 need, u64 &upto, EACH each) {
+// Of the places that each(f) hands to f(place), from .. to: the one at which their number (by_count) or weight, with
+// `front` in front of them, reaches `need`.  There is one.  By count `upto` gets the weight up to it.
+template <typename EACH, typename WEIGHT>
+__device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u64 front, u64 need, u64 &upto, EACH each, WEIGHT weight) {
     const int tid = threadIdx.x;
+    u64 front_weight = by_count ? 0 : front;
     while (true) {
         const u64 span = to - from;
         const int shift = span < TR_DIGITS ? 0 : 64 - __clzll((long long)span) - 10;
         s.sum[tid] = 0;
         s.count[tid] = 0;
+        if (tid == 0) s.gathered = 0;
         __syncthreads();
-        each([&](u64 at, u64 weight) {
+        each([&](u64 at) {
             if (at < from || at > to) return;
             const int digit = (int)((at - from) >> shift);
-            atomicAdd(&s.sum[digit], weight);
+            atomicAdd(&s.sum[digit], weight(at));
             atomicAdd(&s.count[digit], 1u);
         });
         __syncthreads();
@@ -198,9 +277,11 @@ __device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u6
             s.above = behind;
             s.lo = front_weight + sum - mine;
             s.hi = front_weight + sum;
+            s.inside_count = n;
         }
         __syncthreads();
         const int digit = s.found;
+        const unsigned inside = s.inside_count;
         front = s.above;
         front_weight = s.lo;
         upto = s.hi;
@@ -208,6 +289,15 @@ __device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u6
         from += (u64)digit << shift;
         if (shift == 0) return from;
         to = min(to, from + ((1ull << shift) - 1));
+        if (inside > TR_PAIRS) continue;
+        each([&](u64 at) {
+            if (at >= from && at <= to) s.place[atomicAdd(&s.gathered, 1u)] = at;
+        });
+        __syncthreads();
+        const PairSums r = tr_pairs(s, inside, front_weight, weight);
+        const u64 at = by_count ? tr_pair_by_count(s, r, (unsigned)(need - front), upto) : tr_pair_by_weight(s, r, need);
+        __syncthreads();
+        return at;
     }
 }
 
@@ -235,43 +325,47 @@ __device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s
     const float best = valid ? rl[(unsigned)lo] : 0.f;
     TruncResult r;
     if (tr_decided(lo, best, inv_t, r)) return r;
-    const double rate = tr_rate(inv_t);
+    const double rate = tr_rate(inv_t), limit = tr_limit(a, row);
     auto each = [&](auto f) {
         for (int t = tid; t < vocab; t += TR_THREADS) {
             const float l = rl[t];
-            if (l > -INFINITY) f(tr_place(l, t), tr_weight(tr_octaves(best, l, rate), bits));
+            if (l > -INFINITY) f(tr_place(l, t));
         }
     };
+    auto weight = [&](u64 at) { return tr_weight(tr_octaves(best, tr_logit(at), rate), bits); };
     u64 last = hi, total = 0;               // the last place that stays, the weight up to it
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
     const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
-    const double least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
-    if (k > 0 && (unsigned)k < valid) last = tr_cut(s, lo, hi, true, 0, 0, (u64)k, total, each);
+    if (k > 0 && (unsigned)k < valid) last = tr_cut(s, lo, hi, true, 0, (u64)k, total, each, weight);
     if (p < 1.f) {
         if (total == 0) {
             u64 sum = 0;
             unsigned unused = 0;
-            each([&](u64, u64 w) { sum += w; });
+            each([&](u64 at) { sum += weight(at); });
             tr_block_prefix(s, sum, unused);
             if (tid == TR_THREADS - 1) s.hi = sum;
             __syncthreads();
             total = s.hi;
             __syncthreads();
         }
-        last = tr_cut(s, lo, last, false, 0, 0, tr_share(p, total), total, each);
+        last = tr_cut(s, lo, last, false, 0, tr_share(p, total), total, each, weight);
     }
     // what stays, by ids: a range of them a thread, then the tokens of one
     const int per = (vocab + TR_THREADS - 1) / TR_THREADS;
-    auto weight = [&](int t, u64 &w) {
+    auto stays = [&](int t, u64 &w) {
         w = 0;
         const float l = rl[t];
-        return l > -INFINITY && tr_place(l, t) <= last && tr_stays(tr_octaves(best, l, rate), least, bits, w);
+        if (!(l > -INFINITY) || tr_place(l, t) > last) return false;
+        const double octaves = tr_octaves(best, l, rate);
+        if (octaves > limit) return false;
+        w = tr_weight(octaves, bits);
+        return true;
     };
     u64 sum = 0;
     unsigned count = 0;
     for (int t = tid * per; t < min(vocab, (tid + 1) * per); ++t) {
         u64 w;
-        if (weight(t, w)) ++count;
+        if (stays(t, w)) ++count;
         sum += w;
     }
     const u64 mine = sum;
@@ -283,7 +377,7 @@ __device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s
         u64 run = sum - mine, w;
         int t = tid * per;
         for (;; ++t) {
-            weight(t, w);
+            stays(t, w);
             run += w;
             if (target < run) break;
         }
@@ -304,7 +398,6 @@ sample_truncated_kernel(TruncArgs a) {
 // ---------------------------------------------------------------- many workgroups a row
 #define TR_BINS 1024
 #define TR_LIST 4096
-#define TR_PAIRS 256                    // so many tokens are compared with one another
 #define TR_STEP 1024                    // tokens a workgroup takes at a time: 256 threads, 4 neighbouring tokens each
 #define TR_BUCKET 256                   // ... and a wavefront of them
 #define TR_SPLIT_THREADS 256
@@ -329,9 +422,11 @@ __device__ inline int tr_mode(const TruncArgs &a, int row) {
     return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
 }
 
-// The last bin takes what weighs nothing.
-__device__ inline int tr_bin(double octaves, int bits) {
-    return octaves < bits + 1.0 ? (int)(octaves * ((TR_BINS - 1) / (bits + 1.0))) : TR_BINS - 1;
+// Bins from the best logit down, in 32 bits (any rule that falls with the logit does); the last one takes what weighs nothing.
+__device__ inline float tr_bin_scale(double rate, int bits) { return (float)(rate * ((TR_BINS - 1) / (bits + 1.0))); }
+__device__ inline int tr_bin(float best, float l, float scale) {
+    const float d = best - l;
+    return d > 0.f ? (int)fminf(d * scale, (float)(TR_BINS - 1)) : 0;
 }
 
 typedef float tr_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -345,12 +440,6 @@ __device__ inline void tr_load4(const float *rl, int t, int vocab, float (&l)[4]
 #pragma unroll
         for (int i = 0; i < 4; ++i) l[i] = t + i < vocab ? rl[t + i] : -INFINITY;
     }
-}
-
-__device__ inline u64 tr_wave_min(u64 v) {
-#pragma unroll
-    for (int off = KVA_WAVE / 2; off > 0; off >>= 1) v = min(v, (u64)__shfl_xor(v, off, KVA_WAVE));
-    return v;
 }
 
 // The best place of a row, from its parts' (every wavefront for itself).
@@ -389,61 +478,81 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
     }
 }
 
-// grid (parts, rows)
+// grid (parts, rows).  Four sets of bins, a lane's by its number: most of a row's tokens lie in some tens of bins, and additions to the
+// same one wait for each other.
+#define TR_SETS 4
 __global__ void __launch_bounds__(TR_SPLIT_THREADS)
 trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
-    __shared__ u64 bins[TR_BINS];
+    __shared__ u64 bins[TR_BINS * TR_SETS];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
     const int mode = tr_mode(a, row);
     if (!(inv_t > 0.f) || mode == TR_ALL) return;
-    for (int i = tid; i < TR_BINS; i += TR_SPLIT_THREADS) bins[i] = 0;
     const float *rl = a.logits + row * a.stride;
+    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
+    int t = part * sp.part_tokens + 4 * tid;
+    float l[4];
+    tr_load4(rl, t, a.vocab, l);
+    for (int i = tid; i < TR_BINS * TR_SETS; i += TR_SPLIT_THREADS) bins[i] = 0;
     const u64 at = tr_best(sp, row);
     if (at == ~0ull) return;
-    const float best = rl[(unsigned)at];
+    const float best = tr_logit(at);
     const double rate = tr_rate(inv_t);
+    const float scale = tr_bin_scale(rate, bits);
     __syncthreads();
-    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
-    for (int t = part * sp.part_tokens + 4 * tid; t < end; t += TR_STEP) {
-        float l[4];
-        tr_load4(rl, t, a.vocab, l);
+    for (; t < end; t += TR_STEP) {
+        float next[4];
+        tr_load4(rl, t + TR_STEP, a.vocab, next);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (!(l[i] > -INFINITY)) continue;
-            const double octaves = tr_octaves(best, l[i], rate);
-            const int bin = tr_bin(octaves, bits);
-            if (mode == TR_COUNT) atomicAdd(&bins[bin], 1ull);
-            else if (bin < TR_BINS - 1) atomicAdd(&bins[bin], tr_weight(octaves, bits));
+            const int bin = tr_bin(best, l[i], scale);
+            u64 *to = &bins[bin * TR_SETS + tid % TR_SETS];
+            if (mode == TR_COUNT) atomicAdd(to, 1ull);
+            else if (bin < TR_BINS - 1) atomicAdd(to, tr_weight(tr_octaves(best, l[i], rate), bits));
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] = next[i];
     }
     __syncthreads();
-    for (int i = tid; i < TR_BINS; i += TR_SPLIT_THREADS)
-        if (bins[i] != 0) atomicAdd(&sp.bins[(size_t)row * TR_BINS + i], bins[i]);
+    for (int i = tid; i < TR_BINS; i += TR_SPLIT_THREADS) {
+        u64 v = 0;
+#pragma unroll
+        for (int j = 0; j < TR_SETS; ++j) v += bins[i * TR_SETS + j];
+        if (v != 0) atomicAdd(&sp.bins[(size_t)row * TR_BINS + i], v);
+    }
 }
 
 // grid (parts, rows)
 __global__ void __launch_bounds__(TR_SPLIT_THREADS)
 trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
+    constexpr int PER = TR_BINS / TR_SPLIT_THREADS;
     __shared__ u64 of_wave[TR_SPLIT_THREADS / KVA_WAVE];
-    __shared__ int cut_bin;
+    __shared__ int found[TR_LIST], cut_bin, asked, base;
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
     if (!(inv_t > 0.f)) return;
     const int mode = tr_mode(a, row);
     const float *rl = a.logits + row * a.stride;
+    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
+    int t0 = part * sp.part_tokens;
+    float l[4];
+    tr_load4(rl, t0 + 4 * tid, a.vocab, l);
+    u64 v[PER] = {};
+    if (mode != TR_ALL) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = sp.bins[(size_t)row * TR_BINS + tid * PER + i];
+    }
     const u64 at = tr_best(sp, row);
     if (at == ~0ull) return;
-    const float best = rl[(unsigned)at];
+    const float best = tr_logit(at);
     if (!(best < INFINITY)) return;
     int cut = TR_BINS;                      // the bin in which the cut lies; past the last: everything stays
+    if (tid == 0) asked = 0;
     if (mode != TR_ALL) {
-        u64 v[TR_BINS / TR_SPLIT_THREADS], mine = 0;
+        u64 mine = 0;
 #pragma unroll
-        for (int i = 0; i < TR_BINS / TR_SPLIT_THREADS; ++i) {
-            v[i] = sp.bins[(size_t)row * TR_BINS + tid * (TR_BINS / TR_SPLIT_THREADS) + i];
-            mine += v[i];
-        }
+        for (int i = 0; i < PER; ++i) mine += v[i];
         u64 upto = tr_wave_prefix(mine);
         if (lane == KVA_WAVE - 1) of_wave[wave] = upto;
         if (tid == 0) cut_bin = TR_BINS - 1;            // (fewer tokens than k: all of them)
@@ -458,167 +567,150 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
         u64 run = upto - mine;
         if (run < need && need <= upto) {
 #pragma unroll
-            for (int i = 0; i < TR_BINS / TR_SPLIT_THREADS; ++i) {
-                if (run < need && need <= run + v[i]) cut_bin = tid * (TR_BINS / TR_SPLIT_THREADS) + i;
+            for (int i = 0; i < PER; ++i) {
+                if (run < need && need <= run + v[i]) cut_bin = tid * PER + i;
                 run += v[i];
             }
         }
-        __syncthreads();
-        cut = cut_bin;
     }
-    const double rate = tr_rate(inv_t), least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
-    int *list = sp.list + (size_t)row * TR_LIST;
-    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
-    for (int t0 = part * sp.part_tokens; t0 < end; t0 += TR_STEP) {
+    __syncthreads();
+    if (mode != TR_ALL) cut = cut_bin;
+    const double rate = tr_rate(inv_t), limit = tr_limit(a, row);
+    const float scale = tr_bin_scale(rate, bits);
+    for (; t0 < end; t0 += TR_STEP) {
         const int t = t0 + 4 * tid;
-        float l[4];
-        tr_load4(rl, t, a.vocab, l);
+        float next[4];
+        tr_load4(rl, t + TR_STEP, a.vocab, next);
         u64 sum = 0;
         unsigned count = 0, asks = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (!(l[i] > -INFINITY)) continue;
-            const double octaves = tr_octaves(best, l[i], rate);
-            const int bin = mode == TR_ALL ? 0 : tr_bin(octaves, bits);
+            const int bin = mode == TR_ALL ? 0 : tr_bin(best, l[i], scale);
             if (bin > cut) continue;
             if (mode == TR_COUNT || bin == cut) {
                 asks |= 1u << i;
             } else {
-                u64 w;
-                if (tr_stays(octaves, least, bits, w)) ++count;
-                sum += w;
+                const double octaves = tr_octaves(best, l[i], rate);
+                if (octaves <= limit) sum += tr_weight(octaves, bits), ++count;
             }
         }
         if (mode != TR_COUNT) {
             // 256 ids of this wavefront
-#pragma unroll
-            for (int off = KVA_WAVE / 2; off > 0; off >>= 1) {
-                sum += __shfl_xor(sum, off, KVA_WAVE);
-                count += __shfl_xor(count, off, KVA_WAVE);
-            }
+            sum = tr_wave_prefix(sum);
+            count = tr_wave_prefix(count);
             const int bucket = t0 / TR_BUCKET + wave;
-            if (lane == 0 && bucket < sp.buckets) {
+            if (lane == KVA_WAVE - 1 && bucket < sp.buckets) {
                 sp.sums[(size_t)row * sp.buckets + bucket] = sum;
                 sp.counts[(size_t)row * sp.buckets + bucket] = count;
             }
         }
+        if (asks != 0) {
+            int to = atomicAdd(&asked, __popc(asks));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned long long votes = __ballot(asks >> i & 1);
-            if (votes == 0) continue;
-            int from = 0;
-            if (lane == 0) from = atomicAdd(&sp.listed[row], (int)__popcll(votes));
-            from = __shfl(from, 0, KVA_WAVE) + (int)__popcll(votes & ((1ull << lane) - 1));
-            if ((asks >> i & 1) && from < TR_LIST) list[from] = t + i;
+            for (int i = 0; i < 4; ++i)
+                if ((asks >> i & 1) && to < TR_LIST) found[to++] = t + i;
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] = next[i];
     }
+    __syncthreads();
+    const int n = asked;
+    if (n == 0) return;
+    if (tid == 0) base = atomicAdd(&sp.listed[row], n);
+    __syncthreads();
+    for (int i = tid; i < min(n, TR_LIST - base); i += TR_SPLIT_THREADS) sp.list[(size_t)row * TR_LIST + base + i] = found[i];
 }
 
 // grid (rows)
 __global__ void __launch_bounds__(TR_THREADS)
 trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ TruncShared s;
-    __shared__ u64 place[TR_LIST], heavy[TR_PAIRS];
+    __shared__ u64 place[TR_LIST];
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid % KVA_WAVE, bits = a.scale_bits, vocab = a.vocab;
     const float *rl = a.logits + row * a.stride;
     const float inv_t = a.inv_t[row];
+    const int mode = tr_mode(a, row);
+    // everything that hangs on nothing else is asked for at once
+    const bool drawn = inv_t > 0.f, inside = tid < sp.buckets && mode != TR_COUNT && drawn;
+    const u64 bin = mode == TR_WEIGHT && drawn ? sp.bins[(size_t)row * TR_BINS + tid] : 0;
+    const int n = drawn ? sp.listed[row] : 0, id0 = sp.list[(size_t)row * TR_LIST + tid];
+    u64 mine = inside ? sp.sums[(size_t)row * sp.buckets + tid] : 0;
+    unsigned count = inside ? sp.counts[(size_t)row * sp.buckets + tid] : 0;
     const u64 first = tr_best(sp, row);
-    const float best = first == ~0ull ? 0.f : rl[(unsigned)first];
+    const float best = first == ~0ull ? 0.f : tr_logit(first);
     TruncResult r;
     if (tr_decided(first, best, inv_t, r)) {
         if (tid == 0) r.store(a, row);
         return;
     }
-    const int mode = tr_mode(a, row), n = mode == TR_ALL ? 0 : sp.listed[row];
     if (n > TR_LIST) {
         r = trunc_whole_row(a, s, row);
         if (tid == 0) r.store(a, row);
         return;
     }
-    const double rate = tr_rate(inv_t), least = a.min_p != nullptr ? (double)a.min_p[row] : 0.0;
+    const double rate = tr_rate(inv_t), limit = tr_limit(a, row);
     const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
     u64 last = ~0ull;                       // the last place that stays
     for (int i = tid; i < n; i += TR_THREADS) {
-        const int id = sp.list[(size_t)row * TR_LIST + i];
-        place[i] = tr_place(rl[id], id);
+        const int id = i == tid ? id0 : sp.list[(size_t)row * TR_LIST + i];
+        const u64 at = tr_place(rl[id], id);
+        place[i] = at;
+        if (n <= TR_PAIRS) s.place[i] = at;
     }
-    auto octaves_of = [&](u64 at) { return tr_octaves(best, rl[(unsigned)at], rate); };
+    auto weight = [&](u64 at) { return tr_weight(tr_octaves(best, tr_logit(at), rate), bits); };
     if (mode != TR_ALL) {
         // what lies in front of the list's tokens, and what is sought
-        u64 front = 0, need = 0;
+        u64 front = 0, need = 0, total = 0;
         if (mode == TR_WEIGHT) {
-            const u64 mine = sp.bins[(size_t)row * TR_BINS + tid];
-            u64 upto = mine;
+            u64 upto = bin;
             unsigned unused = 0;
             tr_block_prefix(s, upto, unused);
             if (tid == TR_THREADS - 1) s.hi = upto;
             __syncthreads();
             need = tr_share(p, s.hi);
-            if (upto - mine < need && need <= upto) s.above = upto - mine;
+            if (upto - bin < need && need <= upto) s.above = upto - bin;
             __syncthreads();
             front = s.above;
         } else {
             need = (u64)min(a.top_k[row], n);
         }
+        __syncthreads();
         if (n <= TR_PAIRS) {
-            // four threads a token add up what lies in front of it
-            const int j = tid / 4;
-            if (tid < n) heavy[tid] = tr_weight(octaves_of(place[tid]), bits);
-            __syncthreads();
-            u64 upto = front;
-            int rank = 0;
-            const u64 me = j < n ? place[j] : 0;
-            for (int i = tid % 4; i < n; i += 4) {
-                if (place[i] <= me) upto += heavy[i], ++rank;
-            }
-            upto -= tid % 4 ? front : 0;
-#pragma unroll
-            for (int off = 1; off < 4; off <<= 1) {
-                upto += __shfl_xor(upto, off, KVA_WAVE);
-                rank += __shfl_xor(rank, off, KVA_WAVE);
-            }
-            if (tid == 0) s.lo = ~0ull;
+            const PairSums pairs = tr_pairs(s, n, front, weight);
             if (mode == TR_COUNT) {
-                if (j < n && tid % 4 == 0 && (u64)rank == need) s.hi = upto, s.above = me;       // (ranks are 1 .. n, one each)
-                __syncthreads();
-                last = s.above;
-                need = p < 1.f ? tr_share(p, s.hi) : ~0ull;
+                last = tr_pair_by_count(s, pairs, (unsigned)need, total);
+                if (p < 1.f) last = tr_pair_by_weight(s, pairs, tr_share(p, total));
             } else {
-                __syncthreads();
-            }
-            if (need != ~0ull) {
-                if (j < n && tid % 4 == 0 && upto >= need) atomicMin(&s.lo, me);
-                __syncthreads();
-                last = s.lo;
+                last = tr_pair_by_weight(s, pairs, need);
             }
         } else {
-            __syncthreads();
-            u64 from = ~0ull, to = 0, total = 0;
+            u64 from = ~0ull, to = 0;
             for (int i = tid; i < n; i += TR_THREADS) from = min(from, place[i]), to = max(to, place[i]);
             tr_block_range(s, from, to);
             auto each = [&](auto f) {
-                for (int i = tid; i < n; i += TR_THREADS) f(place[i], tr_weight(octaves_of(place[i]), bits));
+                for (int i = tid; i < n; i += TR_THREADS) f(place[i]);
             };
-            last = tr_cut(s, from, to, mode == TR_COUNT, front, front, need, total, each);
-            if (mode == TR_COUNT && p < 1.f) last = tr_cut(s, from, last, false, 0, 0, tr_share(p, total), total, each);
+            last = tr_cut(s, from, to, mode == TR_COUNT, front, need, total, each, weight);
+            if (mode == TR_COUNT && p < 1.f) last = tr_cut(s, from, last, false, 0, tr_share(p, total), total, each, weight);
         }
     }
     // what stays, by 256 ids: a thread each
     __syncthreads();
-    const bool inside = tid < sp.buckets && mode != TR_COUNT;
-    s.sum[tid] = inside ? sp.sums[(size_t)row * sp.buckets + tid] : 0;
-    s.count[tid] = inside ? sp.counts[(size_t)row * sp.buckets + tid] : 0;
+    s.sum[tid] = mine;
+    s.count[tid] = count;
     __syncthreads();
     for (int i = tid; i < n; i += TR_THREADS) {
-        u64 w;
-        if (place[i] > last || !tr_stays(octaves_of(place[i]), least, bits, w)) continue;
-        atomicAdd(&s.sum[(unsigned)place[i] / TR_BUCKET], w);
-        atomicAdd(&s.count[(unsigned)place[i] / TR_BUCKET], 1u);
+        const u64 at = place[i];
+        const double octaves = tr_octaves(best, tr_logit(at), rate);
+        if (at > last || octaves > limit) continue;
+        atomicAdd(&s.sum[(unsigned)at / TR_BUCKET], tr_weight(octaves, bits));
+        atomicAdd(&s.count[(unsigned)at / TR_BUCKET], 1u);
     }
     __syncthreads();
-    const u64 mine = s.sum[tid];
+    mine = s.sum[tid];
     u64 sum = mine;
-    unsigned count = s.count[tid];
+    count = s.count[tid];
     tr_block_prefix(s, sum, count);
     if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
     __syncthreads();
@@ -635,7 +727,10 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         w[i] = 0;
-        if (l[i] > -INFINITY && tr_place(l[i], t + i) <= last) tr_stays(tr_octaves(best, l[i], rate), least, bits, w[i]);
+        if (l[i] > -INFINITY && tr_place(l[i], t + i) <= last) {
+            const double octaves = tr_octaves(best, l[i], rate);
+            if (octaves <= limit) w[i] = tr_weight(octaves, bits);
+        }
         sum += w[i];
     }
     u64 run = s.above + tr_wave_prefix(sum) - sum;

@@ -176,20 +176,19 @@ step_rows_kernel(RowsArgs a) {
     }
 }
 
-// table [groups] of rows x blocks each, slots [groups]; the arrays of pointers and sizes are the host's
-extern "C" int kva_step_rows(const int *lengths, const int *starts, const int *seats, int entries, const void *const *tables,
-                             const int *rows, const int *blocks, int groups, int page_size, int tokens, int *q_start, int *positions,
-                             int *tok_seat, void *const *slots, hipStream_t stream) {
+// group [groups][4], the host's: a table's address, its rows and blocks, and the address of the group's slots
+extern "C" int kva_step_rows(const int *lengths, const int *starts, const int *seats, int entries, const long long *group, int groups,
+                             int page_size, int tokens, int *q_start, int *positions, int *tok_seat, hipStream_t stream) {
     KVA_REQUIRE(entries >= 0 && entries <= ST_MAX_ENTRIES, "step_rows: %d entries are not in 0..%d", entries, ST_MAX_ENTRIES);
     KVA_REQUIRE(groups >= 0 && groups <= ST_MAX_GROUPS, "step_rows: %d groups are not in 0..%d", groups, ST_MAX_GROUPS);
     KVA_REQUIRE(tokens >= 0 && page_size > 0, "step_rows: bad sizes tokens=%d page_size=%d", tokens, page_size);
     RowsArgs a{lengths, starts, seats, q_start, positions, tok_seat, entries, tokens, page_size, groups, {}, {}, {}, {}};
-    for (int g = 0; g < groups; ++g) {
-        KVA_REQUIRE(rows[g] > 0 && blocks[g] > 0, "step_rows: table %d is %d x %d", g, rows[g], blocks[g]);
-        a.table[g] = (const int *)tables[g];
-        a.slots[g] = (int *)slots[g];
-        a.rows[g] = rows[g];
-        a.blocks[g] = blocks[g];
+    for (int g = 0; g < groups; ++g, group += 4) {
+        KVA_REQUIRE(group[1] > 0 && group[2] > 0 && group[1] <= INT_MAX && group[2] <= INT_MAX, "step_rows: table %d is %lld x %lld", g, group[1], group[2]);
+        a.table[g] = (const int *)group[0];
+        a.rows[g] = (int)group[1];
+        a.blocks[g] = (int)group[2];
+        a.slots[g] = (int *)group[3];
     }
     const int grid = max(1, (int)(((long long)tokens + 4 * ST_THREADS - 1) / (4 * ST_THREADS)));
     hipLaunchKernelGGL(step_rows_kernel, dim3(grid), dim3(ST_THREADS), 0, stream, a);

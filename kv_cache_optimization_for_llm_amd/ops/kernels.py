@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from typing import Optional
 
 import torch
@@ -1195,32 +1196,42 @@ def mark_tokens(mask: torch.Tensor, seats: torch.Tensor, tokens: torch.Tensor) -
           "mark_tokens")
 
 
-def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """The launch goes to the current device's stream: everything it takes has to be there."""
-    for t in tensors:
-        if t is not None and t.is_cuda and t.device.index != _RAW_DEVICE():
-            raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{_RAW_DEVICE()}")
+def _at(what: str, name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: tuple, device: int) -> Optional[int]:
+    """The address of a contiguous tensor of this type and shape on the device that the launch goes to; ``None`` for no tensor.  (What
+    it looks at first takes a fifth of the time of the reasons it gives: these launches are a few microseconds long.)"""
+    if t is None:
+        return None
+    try:
+        if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        raise KernelError(f"{what}: {name}: expected a tensor, got {type(t).__name__}") from None
+    if t.shape != shape:
+        raise KernelError(f"{what}: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
+    _dev(t, f"{what}: {name}", dtype)
+    raise KernelError(f"{what}: {name} is on {t.device}, the launch goes to cuda:{device}")
 
 
-def _rows_of(what: str, t: torch.Tensor, name: str) -> int:
+def _launch_device(what: str, t: torch.Tensor) -> int:
+    """The current device, which has to be the tensor's: the launch goes to its stream."""
+    if not t.is_cuda:
+        raise KernelError(f"{what}: tensor is on {t.device}; the kernels run on the GPU only")
+    device = _RAW_DEVICE()
+    if t.get_device() != device:
+        raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
+    return device
+
+
+def _rows_of(what: str, name: str, t: torch.Tensor) -> int:
     """Elements from a row of ``[rows, columns]`` to the next; the elements of a row lie next to each other."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise KernelError(f"{what}: {name} must be [rows, vocabulary]")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    (rows, cols), (stride, one) = t.shape, t.stride()
+    if cols > 1 and one != 1:
         raise KernelError(f"{what}: the elements of a row of {name} must lie next to each other")
-    if rows > 1 and t.stride(0) < cols:
+    if rows > 1 and stride < cols:
         raise KernelError(f"{what}: rows of {name} overlap")
-    return t.stride(0) if rows > 1 else cols
-
-
-def _per_row(what: str, rows: int, dtype: torch.dtype, **arrays: Optional[torch.Tensor]) -> list:
-    out = []
-    for name, t in arrays.items():
-        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != (rows,)):
-            raise KernelError(f"{what}: {name} must have an element per row")
-        out.append(_opt(t, name, dtype))
-    return out
+    return stride if rows > 1 else cols
 
 
 def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional[torch.Tensor] = None,
@@ -1242,44 +1253,52 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional
 
     A row that names a seat or a grammar that is not there gets -inf everywhere: no token can be taken from it."""
     what = "adjust_logits"
-    in_stride, out_stride = _rows_of(what, logits, "logits"), _rows_of(what, out, "out")
+    in_stride, out_stride = _rows_of(what, "logits", logits), _rows_of(what, "out", out)
     rows, vocab = logits.shape
     if out.shape != logits.shape:
         raise KernelError(f"{what}: out {tuple(out.shape)} does not fit logits {tuple(logits.shape)}")
-    p_in, p_out = _dev(logits, "logits", contiguous=False), _dev(out, "out", torch.float32, contiguous=False)
-    code = dtype_code(logits.dtype)
-    if rows and vocab and not (p_in == p_out and logits.dtype == out.dtype and in_stride == out_stride):
-        size = logits.element_size()
-        if p_in < p_out + 4 * ((rows - 1) * out_stride + vocab) and p_out < p_in + size * ((rows - 1) * in_stride + vocab):
-            raise KernelError(f"{what}: out overlaps the logits without being them")
     if (marks is None) != (row_seat is None):
         raise KernelError(f"{what}: marks and the seats of the rows go together")
     if marks is None and (counts is not None or repetition is not None):
         raise KernelError(f"{what}: counts and repetition need marks")
     if counts is None and (presence is not None or frequency is not None):
         raise KernelError(f"{what}: presence and frequency need counts")
-    for name, t in (("marks", marks), ("counts", counts)):
-        if t is not None and (t.dim() != 2 or t.shape[1] != vocab or t.shape[0] < 1 or t.shape[0] != marks.shape[0]):
-            raise KernelError(f"{what}: {name} must be [seats, {vocab}]")
     if (allowed is None) != (allowed_row is None):
         raise KernelError(f"{what}: grammars and the rows' numbers of them go together")
-    if allowed is not None and (allowed.dim() != 2 or allowed.shape[0] < 1 or allowed.shape[1] != (vocab + 31) // 32):
-        raise KernelError(f"{what}: allowed must be [grammars, {(vocab + 31) // 32}] words of 32 tokens")
+    seats = grammars = biases = 0
     start = token = value = None
+    if marks is not None:
+        seats = marks.shape[0] if marks.dim() == 2 else 0
+        if seats < 1:
+            raise KernelError(f"{what}: marks must be [seats, {vocab}]")
+    if allowed is not None:
+        grammars = allowed.shape[0] if allowed.dim() == 2 else 0
+        if grammars < 1:
+            raise KernelError(f"{what}: allowed must be [grammars, {(vocab + 31) // 32}] words of 32 tokens")
     if bias is not None:
         if len(bias) != 3:
             raise KernelError(f"{what}: bias is (start, token, value)")
         start, token, value = bias
-        if start.shape != (rows + 1,) or token.dim() != 1 or value.shape != token.shape:
-            raise KernelError(f"{what}: bias takes rows + 1 starts and a value per token")
-    _here(what, logits, out, row_seat, marks, counts, repetition, presence, frequency, start, token, value, allowed, allowed_row)
-    rep, pres, freq = _per_row(what, rows, torch.float32, repetition=repetition, presence=presence, frequency=frequency)
-    seat, grammar = _per_row(what, rows, torch.int32, row_seat=row_seat, allowed_row=allowed_row)
-    check(hip_lib().kva_adjust_logits(
-        p_out, out_stride, p_in, code, in_stride, rows, vocab, seat, marks.shape[0] if marks is not None else 0,
-        _opt(marks, "marks", torch.uint8), _opt(counts, "counts", torch.int32), rep, pres, freq, _opt(start, "bias start", torch.int32),
-        _opt(token, "bias token", torch.int32), _opt(value, "bias value", torch.float32), token.shape[0] if token is not None else 0,
-        grammar, _opt(allowed, "allowed", torch.int32), allowed.shape[0] if allowed is not None else 0, _stream()), what)
+        biases = token.shape[0] if token.dim() == 1 else -1
+    per_row = (rows,)
+    f32, i32 = torch.float32, torch.int32
+    # (shapes first: they are refused without a device, too)
+    device = logits.get_device() if logits.is_cuda else -1
+    args = (_at(what, "row_seat", row_seat, i32, per_row, device), seats, _at(what, "marks", marks, torch.uint8, (seats, vocab), device),
+            _at(what, "counts", counts, i32, (seats, vocab), device), _at(what, "repetition", repetition, f32, per_row, device),
+            _at(what, "presence", presence, f32, per_row, device), _at(what, "frequency", frequency, f32, per_row, device),
+            _at(what, "bias start", start, i32, (rows + 1,), device), _at(what, "bias token", token, i32, (biases,), device),
+            _at(what, "bias value", value, f32, (biases,), device), biases, _at(what, "allowed_row", allowed_row, i32, per_row, device),
+            _at(what, "allowed", allowed, i32, (grammars, (vocab + 31) // 32), device), grammars)
+    _launch_device(what, logits)
+    if out.dtype is not f32 or out.get_device() != device:
+        raise KernelError(f"{what}: out must be float32 on the logits' device")
+    p_in, p_out, code = logits.data_ptr(), out.data_ptr(), dtype_code(logits.dtype)
+    if rows and vocab and not (p_in == p_out and code == F32 and in_stride == out_stride):
+        size = 4 if code == F32 else 2
+        if p_in < p_out + 4 * ((rows - 1) * out_stride + vocab) and p_out < p_in + size * ((rows - 1) * in_stride + vocab):
+            raise KernelError(f"{what}: out overlaps the logits without being them")
+    check(hip_lib().kva_adjust_logits(p_out, out_stride, p_in, code, in_stride, rows, vocab, *args, _stream()), what)
     return out
 
 
@@ -1287,12 +1306,13 @@ def count_tokens(marks: torch.Tensor, counts: Optional[torch.Tensor], seats: tor
     """``marks[seat, token] = 1`` and, with counts, ``counts[seat, token] += 1`` for every pair of ``seats`` and ``tokens`` (int32,
     as often as it is there); pairs outside the arrays are passed over."""
     what = "count_tokens"
-    if marks.dim() != 2 or (counts is not None and counts.shape != marks.shape) or seats.dim() != 1 or tokens.shape != seats.shape:
+    if marks.dim() != 2 or tokens.dim() != 1:
         raise KernelError(f"{what}: one seat per token, marks and counts [seats, vocab]")
-    _here(what, marks, counts, seats, tokens)
-    check(hip_lib().kva_count_tokens(
-        _dev(marks, "marks", torch.uint8), _opt(counts, "counts", torch.int32), marks.shape[0], marks.shape[1],
-        _dev(seats, "seats", torch.int32), _dev(tokens, "tokens", torch.int32), seats.shape[0], _stream()), what)
+    rows, n, i32, device = marks.shape, tokens.shape, torch.int32, marks.get_device() if marks.is_cuda else -1
+    args = (_at(what, "marks", marks, torch.uint8, rows, device), _at(what, "counts", counts, i32, rows, device), rows[0], rows[1],
+            _at(what, "seats", seats, i32, n, device), _at(what, "tokens", tokens, i32, n, device), n[0])
+    _launch_device(what, marks)
+    check(hip_lib().kva_count_tokens(*args, _stream()), what)
 
 
 def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
@@ -1315,7 +1335,7 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
     tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
     what = "sample_truncated"
-    stride = _rows_of(what, logits, "logits")
+    stride = _rows_of(what, "logits", logits)
     rows, vocab = logits.shape
     if inv_temperature is None:
         raise KernelError(f"{what}: inv_temperature is needed")
@@ -1326,18 +1346,21 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     if host_tokens is not None and (host_tokens.is_cuda or not host_tokens.is_pinned() or host_tokens.dtype != torch.int32
                                     or host_tokens.dim() != 1 or host_tokens.shape[0] < rows or not host_tokens.is_contiguous()):
         raise KernelError(f"{what}: host_tokens must be a pinned host int32 vector with a place per row")
-    _here(what, logits, out_tokens, inv_temperature, top_k, top_p, min_p, uniform, rng_key, rng_step, kept, logprob)
-    inv_t, p, least, u, lp = _per_row(what, rows, torch.float32, inv_temperature=inv_temperature, top_p=top_p, min_p=min_p,
-                                      uniform=uniform, logprob=logprob)
-    tok, k, key, step, n = _per_row(what, rows, torch.int32, out_tokens=out_tokens, top_k=top_k, rng_key=rng_key, rng_step=rng_step,
-                                    kept=kept)
+    device = logits.get_device() if logits.is_cuda else -1
+    n, f32, i32 = (rows,), torch.float32, torch.int32
+    args = (_at(what, "inv_temperature", inv_temperature, f32, n, device), _at(what, "top_k", top_k, i32, n, device),
+            _at(what, "top_p", top_p, f32, n, device), _at(what, "min_p", min_p, f32, n, device), _at(what, "uniform", uniform, f32, n, device),
+            int(seed) & 0xFFFFFFFF, _at(what, "rng_key", rng_key, i32, n, device), _at(what, "rng_step", rng_step, i32, n, device),
+            _at(what, "kept", kept, i32, n, device), _at(what, "logprob", logprob, f32, n, device),
+            host_tokens.data_ptr() if host_tokens is not None else None)
+    tokens = _at(what, "out_tokens", out_tokens, i32, n, device)
+    _launch_device(what, logits)
+    if logits.dtype is not f32:
+        raise KernelError(f"{what}: logits are {logits.dtype}, expected torch.float32")
     lib = hip_lib()
     size = lib.kva_sample_truncated_workspace_bytes(rows, vocab)
-    space = torch.empty(size // 4, dtype=torch.int32, device=logits.device) if size else None
-    check(lib.kva_sample_truncated(
-        tok, _dev(logits, "logits", torch.float32, contiguous=False), stride, rows, vocab, inv_t, k, p, least, u, int(seed) & 0xFFFFFFFF,
-        key, step, n, lp, ctypes.c_void_p(host_tokens.data_ptr()) if host_tokens is not None else None,
-        space.data_ptr() if space is not None else None, _stream()), what)
+    space = torch.empty(size // 4, dtype=i32, device=logits.device) if size else None
+    check(lib.kva_sample_truncated(tokens, logits.data_ptr(), stride, rows, vocab, *args, space.data_ptr() if size else None, _stream()), what)
     return out_tokens
 
 
@@ -1350,21 +1373,20 @@ def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, le
     takes none of them and its row stays as it is; one whose seat or blocks are outside the table needs none.  No row may be
     named by two requests whose blocks overlap.  Up to 4,096 requests."""
     what = "grow_tables"
-    n = seats.shape[0] if seats.dim() == 1 else -1
-    if n < 0 or held.shape != (n,) or lengths.shape != (n,) or pages.dim() != 1 or table.dim() != 2:
+    if seats.dim() != 1 or pages.dim() != 1 or table.dim() != 2:
         raise KernelError(f"{what}: a table [rows, blocks], a seat, held blocks and a length per request, and a row of pages")
+    n, i32, device = seats.shape, torch.int32, table.get_device() if table.is_cuda else -1
+    entries = n[0]
     if offsets is None:
-        offsets = torch.empty(n + 1, dtype=torch.int32, device=table.device)
-    if offsets.shape != (n + 1,):
-        raise KernelError(f"{what}: offsets has a place per request and one more")
-    _here(what, table, seats, held, lengths, pages, offsets)
-    if n == 0:
-        _dev(offsets, "offsets", torch.int32)
+        offsets = torch.empty(entries + 1, dtype=i32, device=table.device)
+    size = table.shape
+    args = (_at(what, "table", table, i32, size, device), size[0], size[1], _at(what, "seats", seats, i32, n, device),
+            _at(what, "held", held, i32, n, device), _at(what, "lengths", lengths, i32, n, device), entries, int(page_size),
+            _at(what, "pages", pages, i32, pages.shape, device), pages.shape[0], _at(what, "offsets", offsets, i32, (entries + 1,), device))
+    _launch_device(what, table)
+    if entries == 0:
         return offsets.zero_()
-    check(hip_lib().kva_grow_tables(
-        _dev(table, "table", torch.int32), table.shape[0], table.shape[1], _dev(seats, "seats", torch.int32), _dev(held, "held", torch.int32),
-        _dev(lengths, "lengths", torch.int32), n, int(page_size), _dev(pages, "pages", torch.int32), pages.shape[0],
-        _dev(offsets, "offsets", torch.int32), _stream()), what)
+    check(hip_lib().kva_grow_tables(*args, _stream()), what)
     return offsets
 
 
@@ -1377,23 +1399,18 @@ def step_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, 
     to 8 groups), -1 where no page is mapped, or the position or the seat is outside the table.  Rows behind the last entry's are left
     as they were, and rows that the arrays have no room for are not made.  Everything is int32; up to 4,096 entries."""
     what = "step_rows"
-    n = lengths.shape[0] if lengths.dim() == 1 else -1
-    if n < 0 or starts.shape != (n,) or seats.shape != (n,) or q_start.shape != (n + 1,):
-        raise KernelError(f"{what}: a length, a start and a seat per entry, and one more place in q_start")
-    tokens = positions.shape[0] if positions.dim() == 1 else -1
-    if tokens < 0 or tok_seat.shape != (tokens,) or len(slots) != len(tables) or any(s.shape != (tokens,) for s in slots):
-        raise KernelError(f"{what}: a position, a seat and a slot per group for every token")
-    if any(t.dim() != 2 for t in tables):
-        raise KernelError(f"{what}: tables are [rows, blocks]")
-    groups = len(tables)
-    _here(what, lengths, starts, seats, q_start, positions, tok_seat, *tables, *slots)
-    pointers, sizes = ctypes.c_void_p * max(1, groups), ctypes.c_int * max(1, groups)
-    check(hip_lib().kva_step_rows(
-        _dev(lengths, "lengths", torch.int32), _dev(starts, "starts", torch.int32), _dev(seats, "seats", torch.int32), n,
-        pointers(*[_dev(t, "table", torch.int32) for t in tables]), sizes(*[t.shape[0] for t in tables]),
-        sizes(*[t.shape[1] for t in tables]), groups, int(page_size), tokens, _dev(q_start, "q_start", torch.int32),
-        _dev(positions, "positions", torch.int32), _dev(tok_seat, "tok_seat", torch.int32),
-        pointers(*[_dev(s, "slots", torch.int32) for s in slots]), _stream()), what)
+    if lengths.dim() != 1 or positions.dim() != 1 or len(slots) != len(tables) or any(t.dim() != 2 for t in tables):
+        raise KernelError(f"{what}: a length per entry, a position per token, tables [rows, blocks] and as many arrays of slots")
+    n, tokens, i32, device = lengths.shape, positions.shape, torch.int32, lengths.get_device() if lengths.is_cuda else -1
+    groups = []
+    for t, s in zip(tables, slots):
+        groups += (_at(what, "table", t, i32, t.shape, device), *t.shape, _at(what, "slots", s, i32, tokens, device))
+    args = (_at(what, "q_start", q_start, i32, (n[0] + 1,), device), _at(what, "positions", positions, i32, tokens, device),
+            _at(what, "tok_seat", tok_seat, i32, tokens, device))
+    first = (_at(what, "lengths", lengths, i32, n, device), _at(what, "starts", starts, i32, n, device), _at(what, "seats", seats, i32, n, device))
+    _launch_device(what, lengths)
+    groups = array("q", groups)
+    check(hip_lib().kva_step_rows(*first, n[0], groups.buffer_info()[0], len(tables), int(page_size), tokens[0], *args, _stream()), what)
 
 
 _MAX_SPLITS = None

@@ -106,7 +106,7 @@ _HIP_SIGNATURES = {
     "kva_adjust_logits": [P, LL, P, I, LL, I, I, P, I, P, P, P, P, P, P, P, P, I, P, P, I, P],
     "kva_count_tokens": [P, P, I, I, P, P, I, P],
     "kva_grow_tables": [P, I, I, P, P, P, I, I, P, I, P, P],
-    "kva_step_rows": [P, P, P, I, P, P, P, I, I, I, P, P, P, P, P],
+    "kva_step_rows": [P, P, P, I, P, I, I, I, P, P, P, P],
     "kva_delta_token": [I, P, I, I, I, P, I, P, LL, I, I, I, I, P, P, P, I, F, P, F, P, I, I, I, I, P, I, I, I, F, P, P, I, I, I, I, I, P],
     "kva_linear_token": [I, P, I, I, I, I, I, I, I, P, I, P, F, F, P, LL, I, P, F, P, I, I, I, I, P, I, I, I, F, P, P, I, I, I, I, P],
     "kva_space_token": [I, P, I, I, I, P, P, I, P, LL, I, I, I, P, P, P, P, F, I, P, I, I, I, F, P, P, I, I, I, I, I, I, P],
