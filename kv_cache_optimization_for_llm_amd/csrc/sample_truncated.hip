@@ -17,12 +17,13 @@
 //
 // Vocabularies of up to 262,144 take four launches, the first three of them with many workgroups a row, each of some steps of
 // 1,024 tokens:
-//   1. trunc_best_kernel     the best place of every workgroup's tokens
+//   1. trunc_best_kernel     the best place of every workgroup's tokens; for a small k also of every 256 ids
 //   2. trunc_bins_kernel     1,024 bins by the distance from the best, some 1/22 of a factor of two wide: how many tokens a bin has where
 //                            the row asks for k, their weight where it asks for p alone
 //   3. trunc_collect_kernel  finds the bin in which the cut lies and leaves a list of tokens: where k is asked for those of all bins up to
 //                            it (p's cut is among them), else those of this bin, and the sums of what lies in front of it by 256 ids
-//   4. trunc_pick_kernel     a workgroup a row: the cuts among the list's tokens, what stays by 256 ids, then the token among 256
+//   4. trunc_pick_kernel     a workgroup a row: for a small k its list from the 256s that can hold the k best (such rows pass 2 and 3 by);
+//                            the cuts among the list's tokens, what stays by 256 ids, then the token among 256
 // A list has room for 4,096 tokens.  A row with more in the bin of its cut (nearly equal logits), or with a larger k among
 // them, is taken by the last kernel alone, as rows of larger vocabularies are by sample_truncated_kernel: a cut is found by counting, the places still in
 // question are cut into 1,024 ranges, their numbers and weights added up in LDS, and the range in which the sum passes what is
@@ -64,29 +65,33 @@ __device__ inline float tr_logit(u64 place) {
     return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu);
 }
 
-// how far below the best one a logit lies, in units of log2(weight)
-__device__ inline double tr_octaves(float best, float l, double rate) {
-    const double d = (double)best - (double)l;
-    return d == 0.0 ? 0.0 : d * rate;
-}
-
-// round(2^bits 2^-octaves).  2^f for f from -1/2 to 1/2 by a polynomial through the eleven Chebyshev nodes (4e-16 off, 1 at 0); a number
-// below 2^52 and 2^52 add up to one whose last bits are the number's whole part, rounded.
-__device__ inline u64 tr_weight(double octaves, int bits) {
-    const double z = fmax((double)bits - octaves, -4.0), n = rint(z), f = z - n;
-    double p = 7.072585949269224e-09;
-    p = fma(p, f, 1.0208690299958306e-07);
-    p = fma(p, f, 1.321544258792169e-06);
-    p = fma(p, f, 1.5252657260200837e-05);
-    p = fma(p, f, 0.0001540353044173605);
-    p = fma(p, f, 0.0013333558230164974);
-    p = fma(p, f, 0.009618129107606888);
-    p = fma(p, f, 0.05550410866444772);
-    p = fma(p, f, 0.24022650695910097);
-    p = fma(p, f, 0.69314718055995);
-    p = fma(p, f, 1.0);
-    const double w = ldexp(p, (int)n) + 4503599627370496.0;
-    return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+// How a row weighs its logits.  With x = 128 (s - (best - l) / (T ln 2)) and m its nearest whole number, W = 2^(m / 128) 2^((x - m) / 128):
+// the first from a table of 2^(j / 128) and an exponent, the second, 1 + q with |q| < 0.0028, by three terms of its series (2e-12 off).  A number below 2^52 and
+// 2^52 add up to one whose last bits are the number's whole part, rounded.  Ten terms without a table: 256 rows' bins 58 us instead of 42.
+#define TR_TABLE 128
+struct TruncWeights {
+    double best, rate;                  // 128 / (T ln 2)
+    int bits;
+    const double *table;
+    __device__ inline double scaled(float l) const { return fma(best - (double)l, -rate, (double)TR_TABLE * bits); }
+    __device__ inline u64 of(float l) const { return of(scaled(l)); }
+    __device__ inline u64 of(double scaled) const {
+        const double x = fmax(scaled, -4.0 * TR_TABLE), m = rint(x), y = x - m;     // (at least a number whose weight rounds to none)
+        const int n = (int)m;
+        // (ln 2 / 128)^i / i!
+        double q = fma(y, 2.646642144433097e-08, 1.4662262387640425e-05);
+        q = y * fma(y, q, 0.0054152123481245725);
+        const double t = table[n & (TR_TABLE - 1)];
+        return (u64)__double_as_longlong(ldexp(fma(t, q, t), n >> 7) + 4503599627370496.0) & 0xfffffffffffffull;
+    }
+    __device__ inline u64 of(u64 place) const { return of(tr_logit(place)); }
+    // how far below the best one, in units of log2(weight)
+    __device__ inline double octaves(float l) const { return (best - (double)l) * (rate / TR_TABLE); }
+};
+// (a temperature of nothing has no infinite rate: 0 times it is 0)
+__device__ inline double tr_rate(float inv_t) { return fmin((double)inv_t, 1e300) * (TR_TABLE * 1.4426950408889634); }
+__device__ inline void tr_fill_table(double *table) {
+    if (threadIdx.x < TR_TABLE) table[threadIdx.x] = exp2((double)threadIdx.x / TR_TABLE);
 }
 
 // Numbers from lanes in front of this one, or `none` where there is no such lane.
@@ -222,18 +227,16 @@ __device__ inline bool tr_decided(u64 at, float best, float inv_t, TruncResult &
     return true;
 }
 
-__device__ inline double tr_rate(float inv_t) { return (double)inv_t * 1.4426950408889634; }
-
 // The weight that p's cut has to reach, of `total`.
 __device__ inline u64 tr_share(float p, u64 total) {
     const double share = ceil((double)p * (double)total);
     return share >= 1.0 ? min((u64)share, total) : 1ull;
 }
 
-// How far below the best one a token may lie to stay (the best ones stay in any case).
-__device__ inline double tr_limit(const TruncArgs &a, int row) {
+// The x of TruncWeights that a token needs to stay (the best ones stay in any case).
+__device__ inline double tr_least(const TruncArgs &a, int row) {
     const float least = a.min_p != nullptr ? a.min_p[row] : 0.f;
-    return least > 0.f ? fmax(-log2((double)least), 0.0) : INFINITY;
+    return least > 0.f ? TR_TABLE * (a.scale_bits + fmin(log2((double)least), 0.0)) : -INFINITY;
 }
 
 __device__ inline u64 tr_target(const TruncArgs &a, int row, u64 all) {
@@ -302,7 +305,7 @@ __device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u6
 }
 
 // A row by one workgroup that reads it in every turn.
-__device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s, int row) {
+__device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s, const double *table, int row) {
     const int tid = threadIdx.x, vocab = a.vocab, bits = a.scale_bits;
     const float *rl = a.logits + row * a.stride;
     const float inv_t = a.inv_t[row];
@@ -325,14 +328,15 @@ __device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s
     const float best = valid ? rl[(unsigned)lo] : 0.f;
     TruncResult r;
     if (tr_decided(lo, best, inv_t, r)) return r;
-    const double rate = tr_rate(inv_t), limit = tr_limit(a, row);
+    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    const double least = tr_least(a, row);
     auto each = [&](auto f) {
         for (int t = tid; t < vocab; t += TR_THREADS) {
             const float l = rl[t];
             if (l > -INFINITY) f(tr_place(l, t));
         }
     };
-    auto weight = [&](u64 at) { return tr_weight(tr_octaves(best, tr_logit(at), rate), bits); };
+    auto weight = [&](u64 at) { return weigh.of(at); };
     u64 last = hi, total = 0;               // the last place that stays, the weight up to it
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
     const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
@@ -356,9 +360,9 @@ __device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s
         w = 0;
         const float l = rl[t];
         if (!(l > -INFINITY) || tr_place(l, t) > last) return false;
-        const double octaves = tr_octaves(best, l, rate);
-        if (octaves > limit) return false;
-        w = tr_weight(octaves, bits);
+        const double x = weigh.scaled(l);
+        if (x < least) return false;
+        w = weigh.of(x);
         return true;
     };
     u64 sum = 0;
@@ -384,14 +388,16 @@ __device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s
         s.found = t;
     }
     __syncthreads();
-    return TruncResult{s.found, (int)s.inside_count, tr_logprob(tr_octaves(best, rl[s.found], rate), all, bits)};
+    return TruncResult{s.found, (int)s.inside_count, tr_logprob(weigh.octaves(rl[s.found]), all, bits)};
 }
 
 // grid (rows)
 __global__ void __launch_bounds__(TR_THREADS)
 sample_truncated_kernel(TruncArgs a) {
     __shared__ TruncShared s;
-    const TruncResult r = trunc_whole_row(a, s, blockIdx.x);
+    __shared__ double table[TR_TABLE];
+    tr_fill_table(table);               // (the first barrier comes before its first use)
+    const TruncResult r = trunc_whole_row(a, s, table, blockIdx.x);
     if (threadIdx.x == 0) r.store(a, blockIdx.x);
 }
 
@@ -401,12 +407,15 @@ sample_truncated_kernel(TruncArgs a) {
 #define TR_STEP 1024                    // tokens a workgroup takes at a time: 256 threads, 4 neighbouring tokens each
 #define TR_BUCKET 256                   // ... and a wavefront of them
 #define TR_SPLIT_THREADS 256
-#define TR_MAX_PARTS 128
+#define TR_MAX_PARTS 64
+#define TR_FEW_MOST 256
 #define TR_MAX_VOCAB (TR_BUCKET * TR_THREADS)
 
 struct TruncSpace {                     // of all rows
     u64 *best;                          // [parts]
+    u64 *tops;                          // [buckets]: the best place of every 256 ids
     u64 *bins;                          // [TR_BINS]
+    u64 *sought;                        // [2]: the weight in front of the cut's bin, and the one the cut has to reach
     u64 *sums;                          // [buckets]: what stays for certain, by ids
     unsigned *counts;                   // [buckets]
     int *list;                          // [TR_LIST]
@@ -414,18 +423,19 @@ struct TruncSpace {                     // of all rows
     int parts, part_tokens, buckets;
 };
 
-// What a row's cut is found by: nothing, the number of tokens up to a bin, or their weight.
-enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2 };
+// What a row's cut is found by: nothing, the number of tokens up to a bin, their weight, or the best tokens of every 256 ids (a k of up
+// to half as many as there are of those: 64 rows of 128,256 and k up to 50, us: 24 instead of 37).
+enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2, TR_FEW = 3 };
 __device__ inline int tr_mode(const TruncArgs &a, int row) {
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    if (k > 0 && k < a.vocab) return TR_COUNT;
+    if (k > 0 && k < a.vocab) return k <= min(TR_FEW_MOST, (a.vocab + TR_BUCKET - 1) / TR_BUCKET / 2) ? TR_FEW : TR_COUNT;
     return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
 }
 
 // Bins from the best logit down, in 32 bits (any rule that falls with the logit does); the last one takes what weighs nothing.
-__device__ inline float tr_bin_scale(double rate, int bits) { return (float)(rate * ((TR_BINS - 1) / (bits + 1.0))); }
+__device__ inline float tr_bin_scale(double rate, int bits) { return (float)(rate / TR_TABLE * ((TR_BINS - 1) / (bits + 1.0))); }
 __device__ inline int tr_bin(float best, float l, float scale) {
-    const float d = best - l;
+    const float d = fminf(best - l, 3.402823466e38f);
     return d > 0.f ? (int)fminf(d * scale, (float)(TR_BINS - 1)) : 0;
 }
 
@@ -440,6 +450,15 @@ __device__ inline void tr_load4(const float *rl, int t, int vocab, float (&l)[4]
 #pragma unroll
         for (int i = 0; i < 4; ++i) l[i] = t + i < vocab ? rl[t + i] : -INFINITY;
     }
+}
+
+// The best place of a wavefront whose lanes' ids ascend.
+__device__ inline u64 tr_wave_first(float top, int id) {
+    const unsigned mine = top > -INFINITY ? tr_falling(top) : ~0u;
+    const unsigned best = tr_last_lane(tr_wave_scan(mine, ~0u, [](unsigned a, unsigned b) { return a < b ? a : b; }));
+    if (best == ~0u) return ~0ull;
+    const int lane = __ffsll((long long)__ballot(mine == best)) - 1;
+    return (u64)best << 32 | (unsigned)__builtin_amdgcn_readlane(id, lane);
 }
 
 // The best place of a row, from its parts' (every wavefront for itself).
@@ -459,18 +478,31 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
     const int per = (TR_BINS + sp.parts - 1) / sp.parts;
     for (int i = part * per + tid; i < min(TR_BINS, (part + 1) * per); i += TR_SPLIT_THREADS) sp.bins[(size_t)row * TR_BINS + i] = 0;
     if (part == 0 && tid == 0) sp.listed[row] = 0;
-    const int end = min(a.vocab, (part + 1) * sp.part_tokens);
-    float top = -INFINITY;
+    const int end = min(a.vocab, (part + 1) * sp.part_tokens), lane = tid % KVA_WAVE, wave = tid / KVA_WAVE;
+    const bool few = tr_mode(a, row) == TR_FEW;
+    float l[4], top = -INFINITY;
+    tr_load4(rl, part * sp.part_tokens + 4 * tid, a.vocab, l);
     int id = 0;
-    for (int t = part * sp.part_tokens + 4 * tid; t < end; t += TR_STEP) {
-        float l[4];
-        tr_load4(rl, t, a.vocab, l);
+    u64 at = ~0ull;
+    for (int t0 = part * sp.part_tokens; t0 < end; t0 += TR_STEP) {
+        const int t = t0 + 4 * tid;
+        float next[4];
+        tr_load4(rl, t + TR_STEP, a.vocab, next);
+        if (few) top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (l[i] > top) top = l[i], id = t + i;     // (ascending ids: the first of equal ones)
+        if (few) {
+            const u64 of = tr_wave_first(top, id);
+            const int bucket = t0 / TR_BUCKET + wave;
+            if (lane == 0 && bucket < sp.buckets) sp.tops[(size_t)row * sp.buckets + bucket] = of;
+            at = min(at, of);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] = next[i];
     }
-    u64 at = tr_wave_min(top > -INFINITY ? tr_place(top, id) : ~0ull);
-    if (tid % KVA_WAVE == 0) of_wave[tid / KVA_WAVE] = at;
+    if (!few) at = tr_wave_min(top > -INFINITY ? tr_place(top, id) : ~0ull);     // (a lane's ids are no run: the lowest of all)
+    if (lane == 0) of_wave[wave] = at;
     __syncthreads();
     if (tid == 0) {
         for (int w = 1; w < TR_SPLIT_THREADS / KVA_WAVE; ++w) at = min(at, of_wave[w]);
@@ -478,38 +510,48 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
     }
 }
 
-// grid (parts, rows).  Four sets of bins, a lane's by its number: most of a row's tokens lie in some tens of bins, and additions to the
+// grid (parts, rows).  Two sets of bins, a lane's by its number: most of a row's tokens lie in some tens of bins, and additions to the
 // same one wait for each other.
-#define TR_SETS 4
+#define TR_SETS 2
 __global__ void __launch_bounds__(TR_SPLIT_THREADS)
 trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ u64 bins[TR_BINS * TR_SETS];
+    __shared__ double table[TR_TABLE];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
     const int mode = tr_mode(a, row);
-    if (!(inv_t > 0.f) || mode == TR_ALL) return;
+    if (!(inv_t > 0.f) || mode == TR_ALL || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
     int t = part * sp.part_tokens + 4 * tid;
     float l[4];
     tr_load4(rl, t, a.vocab, l);
     for (int i = tid; i < TR_BINS * TR_SETS; i += TR_SPLIT_THREADS) bins[i] = 0;
+    tr_fill_table(table);
     const u64 at = tr_best(sp, row);
     if (at == ~0ull) return;
     const float best = tr_logit(at);
-    const double rate = tr_rate(inv_t);
-    const float scale = tr_bin_scale(rate, bits);
+    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    const float scale = tr_bin_scale(weigh.rate, bits);
     __syncthreads();
     for (; t < end; t += TR_STEP) {
         float next[4];
         tr_load4(rl, t + TR_STEP, a.vocab, next);
+        // (a logit that is not in the order lies in the last bin with no weight)
+        int bin[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (!(l[i] > -INFINITY)) continue;
-            const int bin = tr_bin(best, l[i], scale);
-            u64 *to = &bins[bin * TR_SETS + tid % TR_SETS];
-            if (mode == TR_COUNT) atomicAdd(to, 1ull);
-            else if (bin < TR_BINS - 1) atomicAdd(to, tr_weight(tr_octaves(best, l[i], rate), bits));
+        for (int i = 0; i < 4; ++i) bin[i] = l[i] > -INFINITY ? tr_bin(best, l[i], scale) : TR_BINS;
+        if (mode == TR_COUNT) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (bin[i] < TR_BINS) atomicAdd(&bins[bin[i] * TR_SETS + tid % TR_SETS], 1ull);
+        } else {
+            u64 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = weigh.of(l[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (bin[i] < TR_BINS - 1) atomicAdd(&bins[bin[i] * TR_SETS + tid % TR_SETS], w[i]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) l[i] = next[i];
@@ -529,10 +571,11 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     constexpr int PER = TR_BINS / TR_SPLIT_THREADS;
     __shared__ u64 of_wave[TR_SPLIT_THREADS / KVA_WAVE];
     __shared__ int found[TR_LIST], cut_bin, asked, base;
+    __shared__ double table[TR_TABLE];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
-    if (!(inv_t > 0.f)) return;
     const int mode = tr_mode(a, row);
+    if (!(inv_t > 0.f) || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
     int t0 = part * sp.part_tokens;
@@ -549,6 +592,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     if (!(best < INFINITY)) return;
     int cut = TR_BINS;                      // the bin in which the cut lies; past the last: everything stays
     if (tid == 0) asked = 0;
+    tr_fill_table(table);
     if (mode != TR_ALL) {
         u64 mine = 0;
 #pragma unroll
@@ -568,37 +612,47 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
         if (run < need && need <= upto) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                if (run < need && need <= run + v[i]) cut_bin = tid * PER + i;
+                if (run < need && need <= run + v[i]) {
+                    cut_bin = tid * PER + i;
+                    if (part == 0) sp.sought[2 * row] = run, sp.sought[2 * row + 1] = need;
+                }
                 run += v[i];
             }
         }
     }
     __syncthreads();
     if (mode != TR_ALL) cut = cut_bin;
-    const double rate = tr_rate(inv_t), limit = tr_limit(a, row);
-    const float scale = tr_bin_scale(rate, bits);
+    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    const double least = tr_least(a, row);
+    const float scale = tr_bin_scale(weigh.rate, bits);
     for (; t0 < end; t0 += TR_STEP) {
         const int t = t0 + 4 * tid;
         float next[4];
         tr_load4(rl, t + TR_STEP, a.vocab, next);
-        u64 sum = 0;
-        unsigned count = 0, asks = 0;
+        unsigned asks = 0, sure = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (!(l[i] > -INFINITY)) continue;
-            const int bin = mode == TR_ALL ? 0 : tr_bin(best, l[i], scale);
-            if (bin > cut) continue;
-            if (mode == TR_COUNT || bin == cut) {
-                asks |= 1u << i;
-            } else {
-                const double octaves = tr_octaves(best, l[i], rate);
-                if (octaves <= limit) sum += tr_weight(octaves, bits), ++count;
-            }
+            const int bin = l[i] > -INFINITY ? (mode == TR_ALL ? 0 : tr_bin(best, l[i], scale)) : TR_BINS + 1;
+            if (bin == cut || (mode == TR_COUNT && bin < cut)) asks |= 1u << i;
+            else if (bin < cut) sure |= 1u << i;
         }
         if (mode != TR_COUNT) {
             // 256 ids of this wavefront
-            sum = tr_wave_prefix(sum);
-            count = tr_wave_prefix(count);
+            u64 sum = 0;
+            unsigned count = 0;
+            if (__any(sure != 0)) {
+                // (no branch around a weight: the four run side by side)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double x = weigh.scaled(l[i]);
+                    const u64 w = weigh.of(x);
+                    const bool stays = (sure >> i & 1) && x >= least;
+                    sum += stays ? w : 0;
+                    count += stays ? 1 : 0;
+                }
+                sum = tr_wave_prefix(sum);
+                count = tr_wave_prefix(count);
+            }
             const int bucket = t0 / TR_BUCKET + wave;
             if (lane == KVA_WAVE - 1 && bucket < sp.buckets) {
                 sp.sums[(size_t)row * sp.buckets + bucket] = sum;
@@ -627,16 +681,23 @@ __global__ void __launch_bounds__(TR_THREADS)
 trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ TruncShared s;
     __shared__ u64 place[TR_LIST];
+    __shared__ double table[TR_TABLE];
+    __shared__ u64 bucket_sum[TR_THREADS];
+    __shared__ unsigned bucket_count[TR_THREADS];
+    __shared__ unsigned short bucket_of[TR_THREADS];
+    __shared__ int asked, buckets_in;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid % KVA_WAVE, bits = a.scale_bits, vocab = a.vocab;
     const float *rl = a.logits + row * a.stride;
     const float inv_t = a.inv_t[row];
     const int mode = tr_mode(a, row);
     // everything that hangs on nothing else is asked for at once
-    const bool drawn = inv_t > 0.f, inside = tid < sp.buckets && mode != TR_COUNT && drawn;
-    const u64 bin = mode == TR_WEIGHT && drawn ? sp.bins[(size_t)row * TR_BINS + tid] : 0;
-    const int n = drawn ? sp.listed[row] : 0, id0 = sp.list[(size_t)row * TR_LIST + tid];
-    u64 mine = inside ? sp.sums[(size_t)row * sp.buckets + tid] : 0;
-    unsigned count = inside ? sp.counts[(size_t)row * sp.buckets + tid] : 0;
+    const bool drawn = inv_t > 0.f, sums = tid < sp.buckets && drawn && (mode == TR_ALL || mode == TR_WEIGHT);
+    const u64 front = mode == TR_WEIGHT && drawn ? sp.sought[2 * row] : 0, sought = mode == TR_WEIGHT && drawn ? sp.sought[2 * row + 1] : 0;
+    int n = drawn ? sp.listed[row] : 0;
+    const int id0 = sp.list[(size_t)row * TR_LIST + tid];
+    bucket_sum[tid] = sums ? sp.sums[(size_t)row * sp.buckets + tid] : 0;
+    bucket_count[tid] = sums ? sp.counts[(size_t)row * sp.buckets + tid] : 0;
+    const u64 my_top = drawn && mode == TR_FEW && tid < sp.buckets ? sp.tops[(size_t)row * sp.buckets + tid] : ~0ull;
     const u64 first = tr_best(sp, row);
     const float best = first == ~0ull ? 0.f : tr_logit(first);
     TruncResult r;
@@ -644,41 +705,78 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         if (tid == 0) r.store(a, row);
         return;
     }
+    tr_fill_table(table);
+    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    const double least = tr_least(a, row);
+    const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
+    const unsigned k = mode == TR_FEW || mode == TR_COUNT ? (unsigned)a.top_k[row] : 0;
+    u64 last = ~0ull, total = 0;            // the last place that stays
+    auto weight = [&](u64 at) { return weigh.of(at); };
+    if (mode == TR_FEW) {
+        // The k-th best of the best tokens of every 256 ids is no better than the k-th best token: what is sought lies among the
+        // tokens that are no worse than it, and those in the k times 256 ids it came from.
+        // (The end of one of 1,024 ranges between the best of them and the last: no better than the k-th, and soon found.)
+        u64 reach = ~0ull, from = my_top, to = my_top == ~0ull ? 0 : my_top;
+        s.count[tid] = 0;
+        if (tid == 0) asked = buckets_in = 0, s.lo = ~0ull;
+        tr_block_range(s, from, to);
+        const u64 span = to - from;
+        const int shift = span < TR_DIGITS ? 0 : 64 - __clzll((long long)span) - 10;
+        if (my_top != ~0ull) atomicAdd(&s.count[(my_top - from) >> shift], 1u);
+        __syncthreads();
+        const unsigned mine = s.count[tid];
+        unsigned upto = mine;
+        u64 none = 0;
+        tr_block_prefix(s, none, upto);
+        if (upto - mine < k && k <= upto) s.lo = from + ((u64)(tid + 1) << shift) - 1;
+        __syncthreads();
+        reach = s.lo;                       // (fewer than k: all of them)
+        if (my_top != ~0ull && my_top <= reach) bucket_of[atomicAdd(&buckets_in, 1)] = (unsigned short)tid;
+        __syncthreads();
+        // (a wavefront a bucket, two of them on their way)
+        const int in = buckets_in;
+        float l[4], next[4];
+        int w = tid / KVA_WAVE, t = 0;
+        if (w < in) tr_load4(rl, t = bucket_of[w] * TR_BUCKET + 4 * lane, vocab, l);
+        for (; w < in; w += TR_WAVES) {
+            int after = 0;
+            if (w + TR_WAVES < in) tr_load4(rl, after = bucket_of[w + TR_WAVES] * TR_BUCKET + 4 * lane, vocab, next);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!(l[i] > -INFINITY)) continue;
+                const u64 at = tr_place(l[i], t + i);
+                if (at > reach) continue;
+                const int to = atomicAdd(&asked, 1);
+                if (to < TR_LIST) place[to] = at;
+                if (to < TR_PAIRS) s.place[to] = at;
+            }
+            t = after;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[i] = next[i];
+        }
+        __syncthreads();
+        n = asked;
+    }
     if (n > TR_LIST) {
-        r = trunc_whole_row(a, s, row);
+        __syncthreads();
+        r = trunc_whole_row(a, s, table, row);
         if (tid == 0) r.store(a, row);
         return;
     }
-    const double rate = tr_rate(inv_t), limit = tr_limit(a, row);
-    const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
-    u64 last = ~0ull;                       // the last place that stays
-    for (int i = tid; i < n; i += TR_THREADS) {
-        const int id = i == tid ? id0 : sp.list[(size_t)row * TR_LIST + i];
-        const u64 at = tr_place(rl[id], id);
-        place[i] = at;
-        if (n <= TR_PAIRS) s.place[i] = at;
-    }
-    auto weight = [&](u64 at) { return tr_weight(tr_octaves(best, tr_logit(at), rate), bits); };
-    if (mode != TR_ALL) {
-        // what lies in front of the list's tokens, and what is sought
-        u64 front = 0, need = 0, total = 0;
-        if (mode == TR_WEIGHT) {
-            u64 upto = bin;
-            unsigned unused = 0;
-            tr_block_prefix(s, upto, unused);
-            if (tid == TR_THREADS - 1) s.hi = upto;
-            __syncthreads();
-            need = tr_share(p, s.hi);
-            if (upto - bin < need && need <= upto) s.above = upto - bin;
-            __syncthreads();
-            front = s.above;
-        } else {
-            need = (u64)min(a.top_k[row], n);
+    if (mode != TR_FEW)
+        for (int i = tid; i < n; i += TR_THREADS) {
+            const int id = i == tid ? id0 : sp.list[(size_t)row * TR_LIST + i];
+            const u64 at = tr_place(rl[id], id);
+            place[i] = at;
+            if (i < TR_PAIRS) s.place[i] = at;
         }
+    if (mode != TR_ALL) {
+        const u64 need = mode == TR_WEIGHT ? sought : (u64)min(k, (unsigned)n);
         __syncthreads();
+        const bool by_count = mode != TR_WEIGHT;
         if (n <= TR_PAIRS) {
             const PairSums pairs = tr_pairs(s, n, front, weight);
-            if (mode == TR_COUNT) {
+            if (by_count) {
                 last = tr_pair_by_count(s, pairs, (unsigned)need, total);
                 if (p < 1.f) last = tr_pair_by_weight(s, pairs, tr_share(p, total));
             } else {
@@ -691,26 +789,23 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
             auto each = [&](auto f) {
                 for (int i = tid; i < n; i += TR_THREADS) f(place[i]);
             };
-            last = tr_cut(s, from, to, mode == TR_COUNT, front, need, total, each, weight);
-            if (mode == TR_COUNT && p < 1.f) last = tr_cut(s, from, last, false, 0, tr_share(p, total), total, each, weight);
+            last = tr_cut(s, from, to, by_count, front, need, total, each, weight);
+            if (by_count && p < 1.f) last = tr_cut(s, from, last, false, 0, tr_share(p, total), total, each, weight);
         }
     }
     // what stays, by 256 ids: a thread each
-    __syncthreads();
-    s.sum[tid] = mine;
-    s.count[tid] = count;
-    __syncthreads();
+    if (mode == TR_ALL) __syncthreads();
     for (int i = tid; i < n; i += TR_THREADS) {
         const u64 at = place[i];
-        const double octaves = tr_octaves(best, tr_logit(at), rate);
-        if (at > last || octaves > limit) continue;
-        atomicAdd(&s.sum[(unsigned)at / TR_BUCKET], tr_weight(octaves, bits));
-        atomicAdd(&s.count[(unsigned)at / TR_BUCKET], 1u);
+        const double x = weigh.scaled(tr_logit(at));
+        if (at > last || x < least) continue;
+        atomicAdd(&bucket_sum[(unsigned)at / TR_BUCKET], weigh.of(x));
+        atomicAdd(&bucket_count[(unsigned)at / TR_BUCKET], 1u);
     }
     __syncthreads();
-    mine = s.sum[tid];
+    const u64 mine = bucket_sum[tid];
     u64 sum = mine;
-    count = s.count[tid];
+    unsigned count = bucket_count[tid];
     tr_block_prefix(s, sum, count);
     if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
     __syncthreads();
@@ -727,10 +822,8 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         w[i] = 0;
-        if (l[i] > -INFINITY && tr_place(l[i], t + i) <= last) {
-            const double octaves = tr_octaves(best, l[i], rate);
-            if (octaves <= limit) w[i] = tr_weight(octaves, bits);
-        }
+        const double x = weigh.scaled(l[i]);
+        if (l[i] > -INFINITY && tr_place(l[i], t + i) <= last && x >= least) w[i] = weigh.of(x);
         sum += w[i];
     }
     u64 run = s.above + tr_wave_prefix(sum) - sum;
@@ -738,7 +831,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (run <= target && target < run + w[i])
-                TruncResult{t + i, (int)s.inside_count, tr_logprob(tr_octaves(best, l[i], rate), all, bits)}.store(a, row);
+                TruncResult{t + i, (int)s.inside_count, tr_logprob(weigh.octaves(l[i]), all, bits)}.store(a, row);
             run += w[i];
         }
     }
@@ -747,7 +840,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
 // How many workgroups a row gets in the first three launches, and their tokens.
 static int trunc_parts(int rows, int vocab, int *part_tokens) {
     const int steps = (vocab + TR_STEP - 1) / TR_STEP;
-    int parts = (2048 + rows - 1) / rows;
+    int parts = (1024 + rows - 1) / rows;
     parts = parts < 1 ? 1 : parts > TR_MAX_PARTS ? TR_MAX_PARTS : parts;
     parts = parts > steps ? steps : parts;
     *part_tokens = (steps + parts - 1) / parts * TR_STEP;
@@ -760,7 +853,7 @@ extern "C" long long kva_sample_truncated_workspace_bytes(int rows, int vocab) {
     if (rows <= 0 || !trunc_split(vocab)) return 0;
     int part_tokens;
     const long long parts = trunc_parts(rows, vocab, &part_tokens), buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
-    return rows * (8 * (parts + TR_BINS + buckets) + 4 * (buckets + TR_LIST + 1));
+    return rows * (8 * (parts + TR_BINS + 2 * buckets) + 4 * (buckets + TR_LIST + 1) + 16);
 }
 
 extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long stride, int rows, int vocab, const float *inv_t,
@@ -795,7 +888,9 @@ extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long 
     sp.buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
     sp.best = (u64 *)workspace;
     sp.bins = sp.best + (size_t)rows * sp.parts;
-    sp.sums = sp.bins + (size_t)rows * TR_BINS;
+    sp.tops = sp.bins + (size_t)rows * TR_BINS;
+    sp.sought = sp.tops + (size_t)rows * sp.buckets;
+    sp.sums = sp.sought + (size_t)rows * 2;
     sp.counts = (unsigned *)(sp.sums + (size_t)rows * sp.buckets);
     sp.list = (int *)(sp.counts + (size_t)rows * sp.buckets);
     sp.listed = sp.list + (size_t)rows * TR_LIST;
