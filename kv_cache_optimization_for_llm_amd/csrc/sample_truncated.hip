@@ -17,12 +17,12 @@
 //
 // Vocabularies of up to 262,144 take four launches, the first three of them with many workgroups a row, each of some steps of
 // 1,024 tokens:
-//   1. trunc_best_kernel     the best place of every workgroup's tokens; for a small k also of every 256 ids
-//   2. trunc_bins_kernel     1,024 bins by the distance from the best, some 1/22 of a factor of two wide: how many tokens a bin has where
+//   1. trunc_best_kernel     the best place of every workgroup's tokens; for a small k also of groups of some 32 to 512
+//   2. trunc_bins_kernel     bins by the distance from the best, 1/32 of a factor of two wide: how many tokens a bin has where
 //                            the row asks for k, their weight where it asks for p alone
 //   3. trunc_collect_kernel  finds the bin in which the cut lies and leaves a list of tokens: where k is asked for those of all bins up to
 //                            it (p's cut is among them), else those of this bin, and the sums of what lies in front of it by 256 ids
-//   4. trunc_pick_kernel     a workgroup a row: for a small k its list from the 256s that can hold the k best (such rows pass 2 and 3 by);
+//   4. trunc_pick_kernel     a workgroup a row: for a small k its list from the groups that can hold the k best (such rows pass 2 and 3 by);
 //                            the cuts among the list's tokens, what stays by 256 ids, then the token among 256
 // A list has room for 4,096 tokens.  A row with more in the bin of its cut (nearly equal logits), or with a larger k among
 // them, is taken by the last kernel alone, as rows of larger vocabularies are by sample_truncated_kernel: a cut is found by counting, the places still in
@@ -31,10 +31,14 @@
 #include "common.h"
 #include "counter_uniform.h"
 
-#define TR_THREADS 1024
+#include <type_traits>
+
+#define TR_THREADS 256
 #define TR_WAVES (TR_THREADS / KVA_WAVE)
 #define TR_NO_TOKEN (-1)
 #define TR_DIGITS 1024
+#define TR_PER (TR_DIGITS / TR_THREADS)
+#define TR_BUCKETS 1024                 // ranges of ids, in which what stays is added up
 
 typedef unsigned long long u64;
 
@@ -65,31 +69,59 @@ __device__ inline float tr_logit(u64 place) {
     return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu);
 }
 
+typedef float tr_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Four neighbouring logits from token t on; what lies behind the vocabulary is -inf.
+__device__ inline void tr_load4(const float *rl, int t, int vocab, float (&l)[4]) {
+    if (t + 3 < vocab) {
+        const tr_f32x4 v = *reinterpret_cast<const tr_f32x4 *>(rl + t);
+        l[0] = v.x, l[1] = v.y, l[2] = v.z, l[3] = v.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] = t + i < vocab ? rl[t + i] : -INFINITY;
+    }
+}
+
 // How a row weighs its logits.  With x = 128 (s - (best - l) / (T ln 2)) and m its nearest whole number, W = 2^(m / 128) 2^((x - m) / 128):
-// the first from a table of 2^(j / 128) and an exponent, the second, 1 + q with |q| < 0.0028, by three terms of its series (2e-12 off).  A number below 2^52 and
-// 2^52 add up to one whose last bits are the number's whole part, rounded.  Ten terms without a table: 256 rows' bins 58 us instead of 42.
+// the first from a table of 2^(j / 128) and an exponent, the second, 1 + q with |q| < 0.0028, by three terms of its series (2e-12 off).
+// A number below 2^51 and 1.5 2^52 (2^52) add up to one whose last bits are the number's whole part, rounded.  A logit that weighs
+// less than 1/8, and one that is none, has the x of 1/8 and the weight 0.  What bounds the kernels that weigh a whole row is the number of
+// instructions: 64-bit ones take as long as others, and these are eleven; a polynomial of ten terms without a table took 58 us where
+// this takes 30 (256 rows' bins).
 #define TR_TABLE 128
 struct TruncWeights {
     double best, rate;                  // 128 / (T ln 2)
     int bits;
     const double *table;
-    __device__ inline double scaled(float l) const { return fma(best - (double)l, -rate, (double)TR_TABLE * bits); }
-    __device__ inline u64 of(float l) const { return of(scaled(l)); }
-    __device__ inline u64 of(double scaled) const {
-        const double x = fmax(scaled, -4.0 * TR_TABLE), m = rint(x), y = x - m;     // (at least a number whose weight rounds to none)
-        const int n = (int)m;
+
+    __device__ inline TruncWeights(float best_, float inv_t, int bits_, const double *table_) : best(best_), bits(bits_), table(table_) {
+        // (a temperature of nothing has no infinite rate: 0 times it is 0)
+        rate = fmin((double)inv_t, 1e300) * (TR_TABLE * 1.4426950408889634);
+    }
+    // x, at least that of a weight of 1/8
+    __device__ inline double scaled(float l) const { return fmax(fma(best - (double)l, -rate, (double)TR_TABLE * bits), -3.0 * TR_TABLE); }
+    __device__ inline u64 of(double x) const {
+        const double shifted = x + 6755399441055744.0, y = x - (shifted - 6755399441055744.0);
+        const int m = (int)(unsigned)__double_as_longlong(shifted);
         // (ln 2 / 128)^i / i!
         double q = fma(y, 2.646642144433097e-08, 1.4662262387640425e-05);
         q = y * fma(y, q, 0.0054152123481245725);
-        const double t = table[n & (TR_TABLE - 1)];
-        return (u64)__double_as_longlong(ldexp(fma(t, q, t), n >> 7) + 4503599627370496.0) & 0xfffffffffffffull;
+        const u64 from_table = (u64)__double_as_longlong(table[m & (TR_TABLE - 1)]);
+        const double t = __longlong_as_double((long long)(from_table + ((u64)((unsigned)(m >> 7) << 20) << 32)));
+        return (u64)__double_as_longlong(fma(t, q, t) + 4503599627370496.0) & 0xfffffffffffffull;
     }
+    __device__ inline u64 of(float l) const { return of(scaled(l)); }
     __device__ inline u64 of(u64 place) const { return of(tr_logit(place)); }
+    // Bins from the best logit down, 1/32 of an octave wide: what lies within half a 128th of the same four 128ths; the last one
+    // takes all that weighs 1/8 and less.
+    __device__ inline int last_bin() const { return TR_TABLE / 4 * (bits + 3); }
+    __device__ inline int bin(double x) const {
+        const int m = (int)(unsigned)__double_as_longlong(x + 6755399441055744.0);
+        return (TR_TABLE * bits - m) >> 2;
+    }
     // how far below the best one, in units of log2(weight)
     __device__ inline double octaves(float l) const { return (best - (double)l) * (rate / TR_TABLE); }
 };
-// (a temperature of nothing has no infinite rate: 0 times it is 0)
-__device__ inline double tr_rate(float inv_t) { return fmin((double)inv_t, 1e300) * (TR_TABLE * 1.4426950408889634); }
 __device__ inline void tr_fill_table(double *table) {
     if (threadIdx.x < TR_TABLE) table[threadIdx.x] = exp2((double)threadIdx.x / TR_TABLE);
 }
@@ -120,6 +152,11 @@ __device__ inline T tr_wave_prefix(T v) {
 }
 __device__ inline unsigned tr_last_lane(unsigned v) { return __builtin_amdgcn_readlane(v, KVA_WAVE - 1); }
 __device__ inline u64 tr_last_lane(u64 v) { return (u64)tr_last_lane((unsigned)(v >> 32)) << 32 | tr_last_lane((unsigned)v); }
+// Sum of numbers below 2^48 over the wavefront, in the last lane: 24 bits at a time, so that no step carries.
+__device__ inline u64 tr_wave_sum48(u64 v) {
+    const unsigned lo = tr_wave_prefix((unsigned)v & 0xffffffu), hi = tr_wave_prefix((unsigned)(v >> 24));
+    return ((u64)hi << 24) + lo;
+}
 __device__ inline u64 tr_wave_min(u64 v) {
     return tr_last_lane(tr_wave_scan(v, ~0ull, [](u64 a, u64 b) { return a < b ? a : b; }));
 }
@@ -127,14 +164,17 @@ __device__ inline u64 tr_wave_max(u64 v) {
     return tr_last_lane(tr_wave_scan(v, 0ull, [](u64 a, u64 b) { return a > b ? a : b; }));
 }
 
-#define TR_PAIRS 256                    // so many tokens are compared with one another
+#define TR_PAIRS 128                    // so many tokens are compared with one another
 
 struct TruncShared {
     u64 sum[TR_DIGITS];
     unsigned count[TR_DIGITS];
-    u64 part[TR_WAVES];
+    u64 bucket_sum[TR_BUCKETS];
+    unsigned bucket_count[TR_BUCKETS];
+    u64 part[2 * TR_WAVES];
     unsigned part_count[TR_WAVES];
     u64 place[TR_PAIRS], weight[TR_PAIRS];
+    double table[TR_TABLE];
     u64 lo, hi, above;
     unsigned inside_count, gathered;
     int found;
@@ -145,11 +185,10 @@ __device__ inline void tr_block_range(TruncShared &s, u64 &lo, u64 &hi) {
     lo = tr_wave_min(lo);
     hi = tr_wave_max(hi);
     __syncthreads();
-    if (threadIdx.x % KVA_WAVE == 0) s.sum[threadIdx.x / KVA_WAVE] = lo, s.part[threadIdx.x / KVA_WAVE] = hi;
+    if (threadIdx.x % KVA_WAVE == 0) s.part[threadIdx.x / KVA_WAVE] = lo, s.part[TR_WAVES + threadIdx.x / KVA_WAVE] = hi;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < TR_WAVES; ++w) lo = min(lo, s.sum[w]), hi = max(hi, s.part[w]);
-    __syncthreads();
+    for (int w = 0; w < TR_WAVES; ++w) lo = min(lo, s.part[w]), hi = max(hi, s.part[TR_WAVES + w]);
 }
 
 // Inclusive prefix sums of a number and a count a thread over the workgroup.
@@ -161,31 +200,47 @@ __device__ inline void tr_block_prefix(TruncShared &s, u64 &v, unsigned &c) {
     if (lane == KVA_WAVE - 1) s.part[wave] = v, s.part_count[wave] = c;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < TR_WAVES - 1; ++w) {
-        const u64 part = s.part[w];
-        const unsigned part_count = s.part_count[w];
-        if (w < wave) v += part, c += part_count;
-    }
+    for (int w = 0; w < TR_WAVES - 1; ++w)
+        if (w < wave) v += s.part[w], c += s.part_count[w];
 }
 
-// Up to 256 tokens, their places in s.place: how many of them and what weight (beside `front`) lies up to each of them, itself
-// included.  Four threads a token, which all get it.
+// The sums of the threads' four numbers and counts of an array of 1,024 each, up to and with the thread's.
+struct FourSums {
+    u64 v[TR_PER], upto;
+    unsigned c[TR_PER], count;
+};
+__device__ inline FourSums tr_four(TruncShared &s, const u64 *sum, const unsigned *count) {
+    FourSums r;
+    r.upto = 0, r.count = 0;
+#pragma unroll
+    for (int i = 0; i < TR_PER; ++i) {
+        r.v[i] = sum[threadIdx.x * TR_PER + i], r.c[i] = count[threadIdx.x * TR_PER + i];
+        r.upto += r.v[i], r.count += r.c[i];
+    }
+    tr_block_prefix(s, r.upto, r.count);
+    return r;
+}
+
+// Up to 128 tokens, their places in s.place: how many of them and what weight (beside `front`) lies up to each of them, itself
+// included.  Four threads a token, or two of more than 64, which all get it.
 struct PairSums {
     bool on;
-    u64 place, upto;
+    u64 place, own, upto;
     unsigned rank;
 };
 template <typename WEIGHT>
 __device__ inline PairSums tr_pairs(TruncShared &s, int n, u64 front, WEIGHT weight) {
-    const int tid = threadIdx.x, j = tid / 4;
+    const int tid = threadIdx.x, share = n <= TR_THREADS / 4 ? 4 : 2, j = tid / share;
     if (tid < n) s.weight[tid] = weight(s.place[tid]);
-    if (tid == 0) s.lo = ~0ull;
     __syncthreads();
-    PairSums r{j < n, j < n ? s.place[j] : 0, 0, 0};
-    for (int i = tid % 4; i < n; i += 4)
-        if (s.place[i] <= r.place) r.upto += s.weight[i], ++r.rank;
-#pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
+    PairSums r{j < n, j < n ? s.place[j] : 0, j < n ? s.weight[j] : 0, 0, 0};
+#pragma unroll 4
+    for (int i = tid % share; i < n; i += share) {
+        const bool in = s.place[i] <= r.place;
+        r.upto += in ? s.weight[i] : 0;
+        r.rank += in ? 1 : 0;
+    }
+    for (int off = 1; off < share; off <<= 1) {
         r.upto += __shfl_xor(r.upto, off, KVA_WAVE);
         r.rank += __shfl_xor(r.rank, off, KVA_WAVE);
     }
@@ -194,14 +249,14 @@ __device__ inline PairSums tr_pairs(TruncShared &s, int n, u64 front, WEIGHT wei
 }
 // The place of the need-th of them, and the weight up to it.
 __device__ inline u64 tr_pair_by_count(TruncShared &s, const PairSums &r, unsigned need, u64 &upto) {
-    if (r.on && r.rank == need) s.above = r.place, s.hi = r.upto;       // (four threads, the same)
+    if (r.on && r.rank == need) s.above = r.place, s.hi = r.upto;       // (the threads of one token, the same)
     __syncthreads();
     upto = s.hi;
     return s.above;
 }
-// The first place up to which the weight reaches `need` (once after tr_pairs).
+// The place at which the weight reaches `need`.
 __device__ inline u64 tr_pair_by_weight(TruncShared &s, const PairSums &r, u64 need) {
-    if (r.on && threadIdx.x % 4 == 0 && r.upto >= need) atomicMin(&s.lo, r.place);
+    if (r.on && r.upto - r.own < need && need <= r.upto) s.lo = r.place;
     __syncthreads();
     return s.lo;
 }
@@ -245,10 +300,6 @@ __device__ inline u64 tr_target(const TruncArgs &a, int row, u64 all) {
     return min(target, all - 1);
 }
 
-__device__ inline float tr_logprob(double octaves, u64 all, int bits) {
-    return (float)(-0.6931471805599453 * (octaves + log2((double)all) - (double)bits));
-}
-
 // Of the places that each(f) hands to f(place), from .. to: the one at which their number (by_count) or weight, with
 // `front` in front of them, reaches `need`.  There is one.  By count `upto` gets the weight up to it.
 template <typename EACH, typename WEIGHT>
@@ -258,8 +309,8 @@ __device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u6
     while (true) {
         const u64 span = to - from;
         const int shift = span < TR_DIGITS ? 0 : 64 - __clzll((long long)span) - 10;
-        s.sum[tid] = 0;
-        s.count[tid] = 0;
+#pragma unroll
+        for (int i = 0; i < TR_PER; ++i) s.sum[tid + i * TR_THREADS] = 0, s.count[tid + i * TR_THREADS] = 0;
         if (tid == 0) s.gathered = 0;
         __syncthreads();
         each([&](u64 at) {
@@ -269,18 +320,20 @@ __device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u6
             atomicAdd(&s.count[digit], 1u);
         });
         __syncthreads();
-        const u64 mine = s.sum[tid];
-        const unsigned n = s.count[tid];
-        u64 sum = mine;
-        unsigned count = n;
-        tr_block_prefix(s, sum, count);
-        const u64 reach = front + (by_count ? (u64)count : sum), behind = reach - (by_count ? (u64)n : mine);
-        if (behind < need && need <= reach) {           // (one thread's range)
-            s.found = tid;
-            s.above = behind;
-            s.lo = front_weight + sum - mine;
-            s.hi = front_weight + sum;
-            s.inside_count = n;
+        const FourSums sums = tr_four(s, s.sum, s.count);
+        u64 run = sums.upto;
+        unsigned seen = sums.count;
+#pragma unroll
+        for (int i = TR_PER - 1; i >= 0; --i) {
+            const u64 reach = front + (by_count ? (u64)seen : run), behind = reach - (by_count ? (u64)sums.c[i] : sums.v[i]);
+            run -= sums.v[i], seen -= sums.c[i];
+            if (behind < need && need <= reach) {       // (one range of them all)
+                s.found = tid * TR_PER + i;
+                s.above = behind;
+                s.lo = front_weight + run;
+                s.hi = front_weight + run + sums.v[i];
+                s.inside_count = sums.c[i];
+            }
         }
         __syncthreads();
         const int digit = s.found;
@@ -304,42 +357,100 @@ __device__ inline u64 tr_cut(TruncShared &s, u64 from, u64 to, bool by_count, u6
     }
 }
 
-// A row by one workgroup that reads it in every turn.
-__device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s, const double *table, int row) {
-    const int tid = threadIdx.x, vocab = a.vocab, bits = a.scale_bits;
-    const float *rl = a.logits + row * a.stride;
+// Four neighbouring tokens: the weight of those that stay up to `last`, and how many they are.
+__device__ inline void tr_stay4(const float (&l)[4], int t, const TruncWeights &weigh, u64 last, double least, u64 (&w)[4], unsigned &count) {
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double x = weigh.scaled(l[i]);
+        const bool stays = l[i] > -INFINITY && tr_place(l[i], t + i) <= last && x >= least;
+        w[i] = stays ? weigh.of(x) : 0;
+        count += stays ? 1 : 0;
+    }
+}
+
+// The token of a row, from what stays by ranges of `per` ids (a multiple of 256), in s.bucket_sum and s.bucket_count.
+__device__ inline void tr_draw(const TruncArgs &a, TruncShared &s, const float *rl, int row, int per, const TruncWeights &weigh, u64 last, double least) {
+    const int tid = threadIdx.x, lane = tid % KVA_WAVE;
+    const FourSums sums = tr_four(s, s.bucket_sum, s.bucket_count);
+    if (tid == TR_THREADS - 1) s.hi = sums.upto, s.inside_count = sums.count;
+    __syncthreads();
+    const u64 all = s.hi, target = tr_target(a, row, all);
+    u64 run = sums.upto;
+#pragma unroll
+    for (int i = TR_PER - 1; i >= 0; --i) {
+        run -= sums.v[i];
+        if (run <= target && target < run + sums.v[i]) s.found = tid * TR_PER + i, s.above = run;
+    }
+    __syncthreads();
+    if (tid >= KVA_WAVE) return;
+    run = s.above;
+    for (int t0 = s.found * per; t0 < a.vocab; t0 += 4 * KVA_WAVE) {
+        const int t = t0 + 4 * lane;
+        float l[4];
+        u64 w[4];
+        unsigned unused;
+        tr_load4(rl, t, a.vocab, l);
+        tr_stay4(l, t, weigh, last, least, w, unused);
+        const u64 mine = w[0] + w[1] + w[2] + w[3], upto = tr_wave_prefix(mine), whole = tr_last_lane(upto);
+        if (target >= run + whole) {            // (the same in all lanes; a range's sum is its tokens')
+            run += whole;
+            continue;
+        }
+        u64 at = run + upto - mine;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (at <= target && target < at + w[i])
+                TruncResult{t + i, (int)s.inside_count, (float)(-0.6931471805599453 * (weigh.octaves(l[i]) + log2((double)all) - (double)weigh.bits))}.store(a, row);
+            at += w[i];
+        }
+        return;
+    }
+}
+
+// A row (`rl`: its logits) by one workgroup that reads it in every turn; s.table is filled, or will be with the next barrier.
+__device__ inline void trunc_whole_row(const TruncArgs &a, TruncShared &s, const float *rl, int row) {
+    const int tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, vocab = a.vocab, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
+    auto each = [&](auto f) {
+        float l[4];
+        tr_load4(rl, 4 * tid, vocab, l);
+        for (int t = 4 * tid; t < vocab; t += 4 * TR_THREADS) {
+            float next[4];
+            tr_load4(rl, t + 4 * TR_THREADS, vocab, next);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (l[i] > -INFINITY) f(tr_place(l[i], t + i));
+                l[i] = next[i];
+            }
+        }
+    };
     // the best place and the last one
     u64 lo = ~0ull, hi = 0;
     unsigned valid = 0;
-    for (int t = tid; t < vocab; t += TR_THREADS) {
-        const float l = rl[t];
-        if (!(l > -INFINITY)) continue;
-        const u64 at = tr_place(l, t);
+    each([&](u64 at) {
         lo = min(lo, at);
         hi = max(hi, at);
         ++valid;
-    }
+    });
     u64 none = 0;
     tr_block_prefix(s, none, valid);
     if (tid == TR_THREADS - 1) s.inside_count = valid;
     tr_block_range(s, lo, hi);
     valid = s.inside_count;
-    const float best = valid ? rl[(unsigned)lo] : 0.f;
+    const float best = valid ? tr_logit(lo) : 0.f;
     TruncResult r;
-    if (tr_decided(lo, best, inv_t, r)) return r;
-    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    if (tr_decided(lo, best, inv_t, r)) {
+        if (tid == 0) r.store(a, row);
+        return;
+    }
+    const TruncWeights weigh(best, inv_t, bits, s.table);
     const double least = tr_least(a, row);
-    auto each = [&](auto f) {
-        for (int t = tid; t < vocab; t += TR_THREADS) {
-            const float l = rl[t];
-            if (l > -INFINITY) f(tr_place(l, t));
-        }
-    };
     auto weight = [&](u64 at) { return weigh.of(at); };
     u64 last = hi, total = 0;               // the last place that stays, the weight up to it
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
     const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
+    __syncthreads();
     if (k > 0 && (unsigned)k < valid) last = tr_cut(s, lo, hi, true, 0, (u64)k, total, each, weight);
     if (p < 1.f) {
         if (total == 0) {
@@ -354,66 +465,69 @@ __device__ inline TruncResult trunc_whole_row(const TruncArgs &a, TruncShared &s
         }
         last = tr_cut(s, lo, last, false, 0, tr_share(p, total), total, each, weight);
     }
-    // what stays, by ids: a range of them a thread, then the tokens of one
-    const int per = (vocab + TR_THREADS - 1) / TR_THREADS;
-    auto stays = [&](int t, u64 &w) {
-        w = 0;
-        const float l = rl[t];
-        if (!(l > -INFINITY) || tr_place(l, t) > last) return false;
-        const double x = weigh.scaled(l);
-        if (x < least) return false;
-        w = weigh.of(x);
-        return true;
-    };
-    u64 sum = 0;
-    unsigned count = 0;
-    for (int t = tid * per; t < min(vocab, (tid + 1) * per); ++t) {
-        u64 w;
-        if (stays(t, w)) ++count;
-        sum += w;
-    }
-    const u64 mine = sum;
-    tr_block_prefix(s, sum, count);
-    if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
+    // what stays, a wavefront a range of ids
+    const int per = (vocab + TR_BUCKETS * 4 * KVA_WAVE - 1) / (TR_BUCKETS * 4 * KVA_WAVE) * (4 * KVA_WAVE);
+#pragma unroll
+    for (int i = 0; i < TR_BUCKETS / TR_THREADS; ++i) s.bucket_sum[tid + i * TR_THREADS] = 0, s.bucket_count[tid + i * TR_THREADS] = 0;
     __syncthreads();
-    const u64 all = s.hi, target = tr_target(a, row, all);
-    if (sum - mine <= target && target < sum) {         // (one thread's)
-        u64 run = sum - mine, w;
-        int t = tid * per;
-        for (;; ++t) {
-            stays(t, w);
-            run += w;
-            if (target < run) break;
+    for (int b = wave; b * per < vocab; b += TR_WAVES) {
+        u64 sum = 0;
+        unsigned count = 0;
+        float l[4];
+        tr_load4(rl, b * per + 4 * lane, vocab, l);
+        for (int t0 = b * per; t0 < min(vocab, (b + 1) * per); t0 += 4 * KVA_WAVE) {
+            float next[4];
+            u64 w[4];
+            unsigned n;
+            tr_load4(rl, t0 + 4 * KVA_WAVE + 4 * lane, vocab, next);
+            tr_stay4(l, t0 + 4 * lane, weigh, last, least, w, n);
+            sum += tr_wave_sum48(w[0] + w[1] + w[2] + w[3]);
+            count += n;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[i] = next[i];
         }
-        s.found = t;
+        count = tr_wave_prefix(count);
+        if (lane == KVA_WAVE - 1) s.bucket_sum[b] = sum, s.bucket_count[b] = count;
     }
     __syncthreads();
-    return TruncResult{s.found, (int)s.inside_count, tr_logprob(weigh.octaves(rl[s.found]), all, bits)};
+    tr_draw(a, s, rl, row, per, weigh, last, least);
 }
 
-// grid (rows)
+// grid (rows).  HELD: the row stands in LDS.
+#define TR_HELD_VOCAB 16384
+template <bool HELD>
 __global__ void __launch_bounds__(TR_THREADS)
 sample_truncated_kernel(TruncArgs a) {
     __shared__ TruncShared s;
-    __shared__ double table[TR_TABLE];
-    tr_fill_table(table);               // (the first barrier comes before its first use)
-    const TruncResult r = trunc_whole_row(a, s, table, blockIdx.x);
-    if (threadIdx.x == 0) r.store(a, blockIdx.x);
+    __shared__ __attribute__((aligned(16))) float held[HELD ? TR_HELD_VOCAB : 4];
+    tr_fill_table(s.table);             // (the first barrier comes before its first use)
+    const float *rl = a.logits + blockIdx.x * a.stride;
+    if (HELD) {
+        for (int t = 4 * threadIdx.x; t < a.vocab; t += 4 * TR_THREADS) {
+            float l[4];
+            tr_load4(rl, t, a.vocab, l);
+            *reinterpret_cast<float4 *>(held + t) = make_float4(l[0], l[1], l[2], l[3]);       // (each thread its own: no barrier yet)
+        }
+    }
+    trunc_whole_row(a, s, HELD ? held : rl, blockIdx.x);
 }
 
 // ---------------------------------------------------------------- many workgroups a row
-#define TR_BINS 1024
+#define TR_BINS 2048                    // (TruncWeights::last_bin is below 1,600)
 #define TR_LIST 4096
 #define TR_STEP 1024                    // tokens a workgroup takes at a time: 256 threads, 4 neighbouring tokens each
 #define TR_BUCKET 256                   // ... and a wavefront of them
 #define TR_SPLIT_THREADS 256
+#define TR_SPLIT_WAVES (TR_SPLIT_THREADS / KVA_WAVE)
+#define TR_WAVE_LIST 1024
 #define TR_MAX_PARTS 64
 #define TR_FEW_MOST 256
-#define TR_MAX_VOCAB (TR_BUCKET * TR_THREADS)
+#define TR_GROUPS 64                    // groups a part
+#define TR_MAX_VOCAB (TR_BUCKET * TR_BUCKETS)
 
 struct TruncSpace {                     // of all rows
     u64 *best;                          // [parts]
-    u64 *tops;                          // [buckets]: the best place of every 256 ids
+    u64 *tops;                          // [parts * 64]: the best place of every group, four neighbouring threads' tokens of a part
     u64 *bins;                          // [TR_BINS]
     u64 *sought;                        // [2]: the weight in front of the cut's bin, and the one the cut has to reach
     u64 *sums;                          // [buckets]: what stays for certain, by ids
@@ -423,42 +537,24 @@ struct TruncSpace {                     // of all rows
     int parts, part_tokens, buckets;
 };
 
-// What a row's cut is found by: nothing, the number of tokens up to a bin, their weight, or the best tokens of every 256 ids (a k of up
-// to half as many as there are of those: 64 rows of 128,256 and k up to 50, us: 24 instead of 37).
+// What a row's cut is found by: nothing, the number of tokens up to a bin, their weight, or the best tokens of the groups (a k of up to
+// half as many as there are of those: 64 rows of 128,256 and k up to 50, us: 22 instead of 37).
 enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2, TR_FEW = 3 };
-__device__ inline int tr_mode(const TruncArgs &a, int row) {
+__device__ inline int tr_mode(const TruncArgs &a, const TruncSpace &sp, int row) {
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    if (k > 0 && k < a.vocab) return k <= min(TR_FEW_MOST, (a.vocab + TR_BUCKET - 1) / TR_BUCKET / 2) ? TR_FEW : TR_COUNT;
+    if (k > 0 && k < a.vocab) return k <= min(TR_FEW_MOST, sp.parts * TR_GROUPS / 2) ? TR_FEW : TR_COUNT;
     return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
 }
 
-// Bins from the best logit down, in 32 bits (any rule that falls with the logit does); the last one takes what weighs nothing.
-__device__ inline float tr_bin_scale(double rate, int bits) { return (float)(rate / TR_TABLE * ((TR_BINS - 1) / (bits + 1.0))); }
-__device__ inline int tr_bin(float best, float l, float scale) {
-    const float d = fminf(best - l, 3.402823466e38f);
-    return d > 0.f ? (int)fminf(d * scale, (float)(TR_BINS - 1)) : 0;
-}
-
-typedef float tr_f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-
-// Four neighbouring logits from token t on; what lies behind the vocabulary is -inf.
-__device__ inline void tr_load4(const float *rl, int t, int vocab, float (&l)[4]) {
-    if (t + 3 < vocab) {
+// The four tokens of a thread in the step that begins at t0 (the same in all threads: a whole step needs no test a token).
+__device__ inline void tr_load_step(const float *rl, int t0, int vocab, float (&l)[4]) {
+    const int t = t0 + 4 * threadIdx.x;
+    if (t0 + TR_STEP <= vocab) {
         const tr_f32x4 v = *reinterpret_cast<const tr_f32x4 *>(rl + t);
         l[0] = v.x, l[1] = v.y, l[2] = v.z, l[3] = v.w;
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[i] = t + i < vocab ? rl[t + i] : -INFINITY;
+        tr_load4(rl, t, vocab, l);
     }
-}
-
-// The best place of a wavefront whose lanes' ids ascend.
-__device__ inline u64 tr_wave_first(float top, int id) {
-    const unsigned mine = top > -INFINITY ? tr_falling(top) : ~0u;
-    const unsigned best = tr_last_lane(tr_wave_scan(mine, ~0u, [](unsigned a, unsigned b) { return a < b ? a : b; }));
-    if (best == ~0u) return ~0ull;
-    const int lane = __ffsll((long long)__ballot(mine == best)) - 1;
-    return (u64)best << 32 | (unsigned)__builtin_amdgcn_readlane(id, lane);
 }
 
 // The best place of a row, from its parts' (every wavefront for itself).
@@ -471,7 +567,7 @@ __device__ inline u64 tr_best(const TruncSpace &sp, int row) {
 // grid (parts, rows)
 __global__ void __launch_bounds__(TR_SPLIT_THREADS)
 trunc_best_kernel(TruncArgs a, TruncSpace sp) {
-    __shared__ u64 of_wave[TR_SPLIT_THREADS / KVA_WAVE];
+    __shared__ u64 of_wave[TR_SPLIT_WAVES];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     const float *rl = a.logits + row * a.stride;
     // (the next launches add to these)
@@ -479,33 +575,30 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
     for (int i = part * per + tid; i < min(TR_BINS, (part + 1) * per); i += TR_SPLIT_THREADS) sp.bins[(size_t)row * TR_BINS + i] = 0;
     if (part == 0 && tid == 0) sp.listed[row] = 0;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens), lane = tid % KVA_WAVE, wave = tid / KVA_WAVE;
-    const bool few = tr_mode(a, row) == TR_FEW;
     float l[4], top = -INFINITY;
-    tr_load4(rl, part * sp.part_tokens + 4 * tid, a.vocab, l);
+    tr_load_step(rl, part * sp.part_tokens, a.vocab, l);
     int id = 0;
-    u64 at = ~0ull;
     for (int t0 = part * sp.part_tokens; t0 < end; t0 += TR_STEP) {
         const int t = t0 + 4 * tid;
         float next[4];
-        tr_load4(rl, t + TR_STEP, a.vocab, next);
-        if (few) top = -INFINITY;
+        tr_load_step(rl, t0 + TR_STEP, a.vocab, next);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (l[i] > top) top = l[i], id = t + i;     // (ascending ids: the first of equal ones)
-        if (few) {
-            const u64 of = tr_wave_first(top, id);
-            const int bucket = t0 / TR_BUCKET + wave;
-            if (lane == 0 && bucket < sp.buckets) sp.tops[(size_t)row * sp.buckets + bucket] = of;
-            at = min(at, of);
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) l[i] = next[i];
     }
-    if (!few) at = tr_wave_min(top > -INFINITY ? tr_place(top, id) : ~0ull);     // (a lane's ids are no run: the lowest of all)
+    u64 at = top > -INFINITY ? tr_place(top, id) : ~0ull;
+    if (tr_mode(a, sp, row) == TR_FEW) {
+        u64 of = min(at, (u64)__shfl_xor(at, 1, KVA_WAVE));
+        of = min(of, (u64)__shfl_xor(of, 2, KVA_WAVE));
+        if (tid % 4 == 0) sp.tops[((size_t)row * sp.parts + part) * TR_GROUPS + tid / 4] = of;
+    }
+    at = tr_wave_min(at);
     if (lane == 0) of_wave[wave] = at;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < TR_SPLIT_THREADS / KVA_WAVE; ++w) at = min(at, of_wave[w]);
+        for (int w = 1; w < TR_SPLIT_WAVES; ++w) at = min(at, of_wave[w]);
         sp.best[(size_t)row * sp.parts + part] = at;
     }
 }
@@ -519,43 +612,41 @@ trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ double table[TR_TABLE];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
-    const int mode = tr_mode(a, row);
+    const int mode = tr_mode(a, sp, row);
     if (!(inv_t > 0.f) || mode == TR_ALL || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
-    int t = part * sp.part_tokens + 4 * tid;
     float l[4];
-    tr_load4(rl, t, a.vocab, l);
+    tr_load_step(rl, part * sp.part_tokens, a.vocab, l);
     for (int i = tid; i < TR_BINS * TR_SETS; i += TR_SPLIT_THREADS) bins[i] = 0;
     tr_fill_table(table);
     const u64 at = tr_best(sp, row);
     if (at == ~0ull) return;
     const float best = tr_logit(at);
-    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
-    const float scale = tr_bin_scale(weigh.rate, bits);
+    const TruncWeights weigh(best, inv_t, bits, table);
     __syncthreads();
-    for (; t < end; t += TR_STEP) {
-        float next[4];
-        tr_load4(rl, t + TR_STEP, a.vocab, next);
-        // (a logit that is not in the order lies in the last bin with no weight)
-        int bin[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bin[i] = l[i] > -INFINITY ? tr_bin(best, l[i], scale) : TR_BINS;
-        if (mode == TR_COUNT) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (bin[i] < TR_BINS) atomicAdd(&bins[bin[i] * TR_SETS + tid % TR_SETS], 1ull);
-        } else {
+    u64 *mine = bins + tid % TR_SETS;
+    auto run = [&](auto counting) {
+        for (int t0 = part * sp.part_tokens; t0 < end; t0 += TR_STEP) {
+            float next[4];
+            tr_load_step(rl, t0 + TR_STEP, a.vocab, next);
+            double x[4];
             u64 w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = weigh.of(l[i]);
+            for (int i = 0; i < 4; ++i) {
+                x[i] = weigh.scaled(l[i]);
+                // (what is not in the order weighs nothing)
+                w[i] = counting ? (l[i] > -INFINITY ? 1 : 0) : weigh.of(x[i]);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (bin[i] < TR_BINS - 1) atomicAdd(&bins[bin[i] * TR_SETS + tid % TR_SETS], w[i]);
-        }
+                if (w[i] != 0) atomicAdd(mine + weigh.bin(x[i]) * TR_SETS, w[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[i] = next[i];
-    }
+            for (int i = 0; i < 4; ++i) l[i] = next[i];
+        }
+    };
+    if (mode == TR_COUNT) run(std::true_type{});
+    else run(std::false_type{});
     __syncthreads();
     for (int i = tid; i < TR_BINS; i += TR_SPLIT_THREADS) {
         u64 v = 0;
@@ -569,18 +660,21 @@ trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
 __global__ void __launch_bounds__(TR_SPLIT_THREADS)
 trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     constexpr int PER = TR_BINS / TR_SPLIT_THREADS;
-    __shared__ u64 of_wave[TR_SPLIT_THREADS / KVA_WAVE];
-    __shared__ int found[TR_LIST], cut_bin, asked, base;
+    __shared__ u64 of_wave[TR_SPLIT_WAVES];
+    // (a wavefront has a list of its own, and counts it itself)
+    __shared__ int found[TR_SPLIT_WAVES][TR_WAVE_LIST], cut_bin;
+    __shared__ u64 sums[TR_BUCKETS];
+    __shared__ unsigned short counts[TR_BUCKETS];
     __shared__ double table[TR_TABLE];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, bits = a.scale_bits;
     const float inv_t = a.inv_t[row];
-    const int mode = tr_mode(a, row);
+    const int mode = tr_mode(a, sp, row);
     if (!(inv_t > 0.f) || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
     int t0 = part * sp.part_tokens;
     float l[4];
-    tr_load4(rl, t0 + 4 * tid, a.vocab, l);
+    tr_load_step(rl, t0, a.vocab, l);
     u64 v[PER] = {};
     if (mode != TR_ALL) {
 #pragma unroll
@@ -591,7 +685,6 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     const float best = tr_logit(at);
     if (!(best < INFINITY)) return;
     int cut = TR_BINS;                      // the bin in which the cut lies; past the last: everything stays
-    if (tid == 0) asked = 0;
     tr_fill_table(table);
     if (mode != TR_ALL) {
         u64 mine = 0;
@@ -603,7 +696,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
         __syncthreads();
         u64 total = 0;
 #pragma unroll
-        for (int w = 0; w < TR_SPLIT_THREADS / KVA_WAVE; ++w) {
+        for (int w = 0; w < TR_SPLIT_WAVES; ++w) {
             if (w < wave) upto += of_wave[w];
             total += of_wave[w];
         }
@@ -622,82 +715,113 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     }
     __syncthreads();
     if (mode != TR_ALL) cut = cut_bin;
-    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    const TruncWeights weigh(best, inv_t, bits, table);
     const double least = tr_least(a, row);
-    const float scale = tr_bin_scale(weigh.rate, bits);
-    for (; t0 < end; t0 += TR_STEP) {
-        const int t = t0 + 4 * tid;
-        float next[4];
-        tr_load4(rl, t + TR_STEP, a.vocab, next);
-        unsigned asks = 0, sure = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int bin = l[i] > -INFINITY ? (mode == TR_ALL ? 0 : tr_bin(best, l[i], scale)) : TR_BINS + 1;
-            if (bin == cut || (mode == TR_COUNT && bin < cut)) asks |= 1u << i;
-            else if (bin < cut) sure |= 1u << i;
-        }
-        if (mode != TR_COUNT) {
-            // 256 ids of this wavefront
+    // (below this no logit is in the cut's bin: a bin and a bit more, rounded down)
+    const double reach = weigh.best - (4.0 * cut + 8.0) / weigh.rate;
+    const float nothing = mode == TR_ALL || cut >= weigh.last_bin() ? -INFINITY : (float)(reach - 1e-6 * fabs(reach));
+    int listed = 0;
+    auto run = [&](auto counting) {
+        for (; t0 < end; t0 += TR_STEP) {
+            float next[4];
+            tr_load_step(rl, t0 + TR_STEP, a.vocab, next);
             u64 sum = 0;
             unsigned count = 0;
-            if (__any(sure != 0)) {
+            bool asks[4] = {}, some = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) some |= l[i] >= nothing;
+            if (__any(some)) {
                 // (no branch around a weight: the four run side by side)
+                double x[4];
+                int bin[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const double x = weigh.scaled(l[i]);
-                    const u64 w = weigh.of(x);
-                    const bool stays = (sure >> i & 1) && x >= least;
-                    sum += stays ? w : 0;
-                    count += stays ? 1 : 0;
+                    x[i] = weigh.scaled(l[i]);
+                    bin[i] = l[i] > -INFINITY ? weigh.bin(x[i]) : TR_BINS + 1;
+                    asks[i] = counting ? bin[i] <= cut : bin[i] == cut;
                 }
-                sum = tr_wave_prefix(sum);
-                count = tr_wave_prefix(count);
-            }
-            const int bucket = t0 / TR_BUCKET + wave;
-            if (lane == KVA_WAVE - 1 && bucket < sp.buckets) {
-                sp.sums[(size_t)row * sp.buckets + bucket] = sum;
-                sp.counts[(size_t)row * sp.buckets + bucket] = count;
-            }
-        }
-        if (asks != 0) {
-            int to = atomicAdd(&asked, __popc(asks));
+                if (!counting) {
+                    u64 w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if ((asks >> i & 1) && to < TR_LIST) found[to++] = t + i;
-        }
+                    for (int i = 0; i < 4; ++i) w[i] = weigh.of(x[i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) l[i] = next[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const bool stays = bin[i] < cut && x[i] >= least;
+                        sum += stays ? w[i] : 0;
+                        count += stays ? 1 : 0;
+                    }
+                    sum = tr_wave_sum48(sum);
+                    count = tr_wave_prefix(count);
+                }
+                if (__any(asks[0] || asks[1] || asks[2] || asks[3])) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned long long votes = __ballot(asks[i]);
+                        const int to = listed + (int)__popcll(votes & ((1ull << lane) - 1));
+                        if (asks[i] && to < TR_WAVE_LIST) found[wave][to] = t0 + 4 * tid + i;
+                        listed += (int)__popcll(votes);
+                    }
+                }
+            }
+            if (!counting && lane == KVA_WAVE - 1) {
+                // 256 ids of this wavefront
+                sums[(t0 - part * sp.part_tokens) / TR_BUCKET + wave] = sum;
+                counts[(t0 - part * sp.part_tokens) / TR_BUCKET + wave] = (unsigned short)count;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[i] = next[i];
+        }
+    };
+    if (mode == TR_COUNT) run(std::true_type{});
+    else run(std::false_type{});
+    if (listed > 0) {
+        // (one list too long is as a row's too long)
+        const int n = min(listed, TR_WAVE_LIST);
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&sp.listed[row], listed > TR_WAVE_LIST ? TR_LIST + 1 : listed);
+        base = __builtin_amdgcn_readfirstlane(base);
+        for (int i = lane; i < min(n, TR_LIST - base); i += KVA_WAVE) sp.list[(size_t)row * TR_LIST + base + i] = found[wave][i];
     }
+    if (mode == TR_COUNT) return;
     __syncthreads();
-    const int n = asked;
-    if (n == 0) return;
-    if (tid == 0) base = atomicAdd(&sp.listed[row], n);
-    __syncthreads();
-    for (int i = tid; i < min(n, TR_LIST - base); i += TR_SPLIT_THREADS) sp.list[(size_t)row * TR_LIST + base + i] = found[i];
+    const int first = part * sp.part_tokens / TR_BUCKET, many = min(sp.buckets - first, sp.part_tokens / TR_BUCKET);
+    for (int i = tid; i < many; i += TR_SPLIT_THREADS) {
+        sp.sums[(size_t)row * sp.buckets + first + i] = sums[i];
+        sp.counts[(size_t)row * sp.buckets + first + i] = counts[i];
+    }
 }
 
-// grid (rows)
+// grid (rows).  Four wavefronts, one a SIMD: with sixteen the same steps took twice as long (64 rows 15 us), each waits for three others'
+// instructions.
 __global__ void __launch_bounds__(TR_THREADS)
 trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
+    constexpr int TOPS = TR_MAX_PARTS * TR_GROUPS / TR_THREADS;
     __shared__ TruncShared s;
     __shared__ u64 place[TR_LIST];
-    __shared__ double table[TR_TABLE];
-    __shared__ u64 bucket_sum[TR_THREADS];
-    __shared__ unsigned bucket_count[TR_THREADS];
-    __shared__ unsigned short bucket_of[TR_THREADS];
-    __shared__ int asked, buckets_in;
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid % KVA_WAVE, bits = a.scale_bits, vocab = a.vocab;
+    __shared__ unsigned short group_of[TR_MAX_PARTS * TR_GROUPS];
+    __shared__ int asked, groups_in;
+    const int row = blockIdx.x, tid = threadIdx.x, bits = a.scale_bits, vocab = a.vocab;
     const float *rl = a.logits + row * a.stride;
     const float inv_t = a.inv_t[row];
-    const int mode = tr_mode(a, row);
+    const int mode = tr_mode(a, sp, row), groups = sp.parts * TR_GROUPS;
     // everything that hangs on nothing else is asked for at once
-    const bool drawn = inv_t > 0.f, sums = tid < sp.buckets && drawn && (mode == TR_ALL || mode == TR_WEIGHT);
+    const bool drawn = inv_t > 0.f, sums = drawn && (mode == TR_ALL || mode == TR_WEIGHT);
     const u64 front = mode == TR_WEIGHT && drawn ? sp.sought[2 * row] : 0, sought = mode == TR_WEIGHT && drawn ? sp.sought[2 * row + 1] : 0;
     int n = drawn ? sp.listed[row] : 0;
     const int id0 = sp.list[(size_t)row * TR_LIST + tid];
-    bucket_sum[tid] = sums ? sp.sums[(size_t)row * sp.buckets + tid] : 0;
-    bucket_count[tid] = sums ? sp.counts[(size_t)row * sp.buckets + tid] : 0;
-    const u64 my_top = drawn && mode == TR_FEW && tid < sp.buckets ? sp.tops[(size_t)row * sp.buckets + tid] : ~0ull;
+    u64 tops[TOPS];
+    if (mode == TR_FEW) {
+#pragma unroll
+        for (int i = 0; i < TOPS; ++i)
+            tops[i] = tid + i * TR_THREADS < groups ? sp.tops[(size_t)row * groups + tid + i * TR_THREADS] : ~0ull;
+    }
+#pragma unroll
+    for (int i = 0; i < TR_BUCKETS / TR_THREADS; ++i) {
+        const int b = tid + i * TR_THREADS;
+        const bool on = sums && b < sp.buckets;
+        s.bucket_sum[b] = on ? sp.sums[(size_t)row * sp.buckets + b] : 0;
+        s.bucket_count[b] = on ? sp.counts[(size_t)row * sp.buckets + b] : 0;
+    }
     const u64 first = tr_best(sp, row);
     const float best = first == ~0ull ? 0.f : tr_logit(first);
     TruncResult r;
@@ -705,62 +829,74 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         if (tid == 0) r.store(a, row);
         return;
     }
-    tr_fill_table(table);
-    const TruncWeights weigh{(double)best, tr_rate(inv_t), bits, table};
+    tr_fill_table(s.table);
+    const TruncWeights weigh(best, inv_t, bits, s.table);
     const double least = tr_least(a, row);
     const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
     const unsigned k = mode == TR_FEW || mode == TR_COUNT ? (unsigned)a.top_k[row] : 0;
     u64 last = ~0ull, total = 0;            // the last place that stays
     auto weight = [&](u64 at) { return weigh.of(at); };
     if (mode == TR_FEW) {
-        // The k-th best of the best tokens of every 256 ids is no better than the k-th best token: what is sought lies among the
-        // tokens that are no worse than it, and those in the k times 256 ids it came from.
-        // (The end of one of 1,024 ranges between the best of them and the last: no better than the k-th, and soon found.)
-        u64 reach = ~0ull, from = my_top, to = my_top == ~0ull ? 0 : my_top;
-        s.count[tid] = 0;
-        if (tid == 0) asked = buckets_in = 0, s.lo = ~0ull;
+        // The k-th best of the groups' best tokens is no better than the k-th best token: what is sought lies among the tokens that are
+        // no worse than it, and those in the groups that have such a token.  "No worse" goes by 1,024 steps between the best of them
+        // and the last, or what weighs nothing: the k-th is soon found among them.
+        u64 from = ~0ull, to = 0;
+#pragma unroll
+        for (int i = 0; i < TOPS; ++i)
+            if (tops[i] != ~0ull) from = min(from, tops[i]), to = max(to, tops[i]);
+#pragma unroll
+        for (int i = 0; i < TR_PER; ++i) s.sum[tid + i * TR_THREADS] = 0, s.count[tid + i * TR_THREADS] = 0;
+        if (tid == 0) asked = groups_in = 0, s.found = TR_DIGITS;
         tr_block_range(s, from, to);
-        const u64 span = to - from;
-        const int shift = span < TR_DIGITS ? 0 : 64 - __clzll((long long)span) - 10;
-        if (my_top != ~0ull) atomicAdd(&s.count[(my_top - from) >> shift], 1u);
-        __syncthreads();
-        const unsigned mine = s.count[tid];
-        unsigned upto = mine;
-        u64 none = 0;
-        tr_block_prefix(s, none, upto);
-        if (upto - mine < k && k <= upto) s.lo = from + ((u64)(tid + 1) << shift) - 1;
-        __syncthreads();
-        reach = s.lo;                       // (fewer than k: all of them)
-        if (my_top != ~0ull && my_top <= reach) bucket_of[atomicAdd(&buckets_in, 1)] = (unsigned short)tid;
-        __syncthreads();
-        // (a wavefront a bucket, two of them on their way)
-        const int in = buckets_in;
-        float l[4], next[4];
-        int w = tid / KVA_WAVE, t = 0;
-        if (w < in) tr_load4(rl, t = bucket_of[w] * TR_BUCKET + 4 * lane, vocab, l);
-        for (; w < in; w += TR_WAVES) {
-            int after = 0;
-            if (w + TR_WAVES < in) tr_load4(rl, after = bucket_of[w + TR_WAVES] * TR_BUCKET + 4 * lane, vocab, next);
+        const float range = fminf(best - tr_logit(to), (float)fmin((double)TR_TABLE * (bits + 3) / weigh.rate, 3e38));
+        const float scale = range > 0.f ? (TR_DIGITS - 1) / range : 0.f;
+        auto step_of = [&](float l) { return (int)fminf((best - l) * scale, TR_DIGITS - 1.f); };
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (!(l[i] > -INFINITY)) continue;
-                const u64 at = tr_place(l[i], t + i);
-                if (at > reach) continue;
-                const int to = atomicAdd(&asked, 1);
-                if (to < TR_LIST) place[to] = at;
-                if (to < TR_PAIRS) s.place[to] = at;
+        for (int i = 0; i < TOPS; ++i)
+            if (tops[i] != ~0ull) atomicAdd(&s.count[step_of(tr_logit(tops[i]))], 1u);
+        __syncthreads();
+        const FourSums of = tr_four(s, s.sum, s.count);
+        unsigned seen = of.count;
+#pragma unroll
+        for (int i = TR_PER - 1; i >= 0; --i) {
+            if (seen - of.c[i] < k && k <= seen) s.found = tid * TR_PER + i;
+            seen -= of.c[i];
+        }
+        __syncthreads();
+        const int reach = s.found;          // (fewer than k: all of them)
+#pragma unroll
+        for (int i = 0; i < TOPS; ++i)
+            if (tops[i] != ~0ull && step_of(tr_logit(tops[i])) <= reach) group_of[atomicAdd(&groups_in, 1)] = (unsigned short)(tid + i * TR_THREADS);
+        __syncthreads();
+        // four threads a group and step: its 16 tokens
+        const int steps = sp.part_tokens / TR_STEP, in = groups_in * steps;
+        constexpr int AHEAD = 8;            // loads on their way
+        for (int j0 = tid / 4; j0 < in; j0 += AHEAD * TR_THREADS / 4) {
+            float l[AHEAD][4];
+            int t[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int j = j0 + u * TR_THREADS / 4, group = group_of[min(j, in - 1) / steps];
+                t[u] = j < in ? group / TR_GROUPS * sp.part_tokens + j % steps * TR_STEP + group % TR_GROUPS * 16 + tid % 4 * 4 : vocab;
+                tr_load4(rl, t[u], vocab, l[u]);
             }
-            t = after;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) l[i] = next[i];
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(l[u][i] > -INFINITY) || step_of(l[u][i]) > reach) continue;
+                    const u64 at = tr_place(l[u][i], t[u] + i);
+                    const int slot = atomicAdd(&asked, 1);
+                    if (slot < TR_LIST) place[slot] = at;
+                    if (slot < TR_PAIRS) s.place[slot] = at;
+                }
         }
         __syncthreads();
         n = asked;
     }
     if (n > TR_LIST) {
         __syncthreads();
-        r = trunc_whole_row(a, s, table, row);
-        if (tid == 0) r.store(a, row);
+        trunc_whole_row(a, s, rl, row);
         return;
     }
     if (mode != TR_FEW)
@@ -770,9 +906,9 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
             place[i] = at;
             if (i < TR_PAIRS) s.place[i] = at;
         }
+    __syncthreads();
     if (mode != TR_ALL) {
         const u64 need = mode == TR_WEIGHT ? sought : (u64)min(k, (unsigned)n);
-        __syncthreads();
         const bool by_count = mode != TR_WEIGHT;
         if (n <= TR_PAIRS) {
             const PairSums pairs = tr_pairs(s, n, front, weight);
@@ -793,48 +929,16 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
             if (by_count && p < 1.f) last = tr_cut(s, from, last, false, 0, tr_share(p, total), total, each, weight);
         }
     }
-    // what stays, by 256 ids: a thread each
-    if (mode == TR_ALL) __syncthreads();
+    // the list's tokens that stay, beside what lies in front of them
     for (int i = tid; i < n; i += TR_THREADS) {
         const u64 at = place[i];
         const double x = weigh.scaled(tr_logit(at));
         if (at > last || x < least) continue;
-        atomicAdd(&bucket_sum[(unsigned)at / TR_BUCKET], weigh.of(x));
-        atomicAdd(&bucket_count[(unsigned)at / TR_BUCKET], 1u);
+        atomicAdd(&s.bucket_sum[(unsigned)at / TR_BUCKET], weigh.of(x));
+        atomicAdd(&s.bucket_count[(unsigned)at / TR_BUCKET], 1u);
     }
     __syncthreads();
-    const u64 mine = bucket_sum[tid];
-    u64 sum = mine;
-    unsigned count = bucket_count[tid];
-    tr_block_prefix(s, sum, count);
-    if (tid == TR_THREADS - 1) s.hi = sum, s.inside_count = count;
-    __syncthreads();
-    const u64 all = s.hi, target = tr_target(a, row, all);
-    if (sum - mine <= target && target < sum) s.found = tid, s.above = sum - mine;
-    __syncthreads();
-    if (tid >= KVA_WAVE) return;
-    // the token: four neighbouring ones a lane
-    const int t = s.found * TR_BUCKET + 4 * lane;
-    float l[4];
-    u64 w[4];
-    tr_load4(rl, t, vocab, l);
-    sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = 0;
-        const double x = weigh.scaled(l[i]);
-        if (l[i] > -INFINITY && tr_place(l[i], t + i) <= last && x >= least) w[i] = weigh.of(x);
-        sum += w[i];
-    }
-    u64 run = s.above + tr_wave_prefix(sum) - sum;
-    if (run <= target && target < run + sum) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (run <= target && target < run + w[i])
-                TruncResult{t + i, (int)s.inside_count, tr_logprob(weigh.octaves(l[i]), all, bits)}.store(a, row);
-            run += w[i];
-        }
-    }
+    tr_draw(a, s, rl, row, TR_BUCKET, weigh, last, least);
 }
 
 // How many workgroups a row gets in the first three launches, and their tokens.
@@ -853,7 +957,7 @@ extern "C" long long kva_sample_truncated_workspace_bytes(int rows, int vocab) {
     if (rows <= 0 || !trunc_split(vocab)) return 0;
     int part_tokens;
     const long long parts = trunc_parts(rows, vocab, &part_tokens), buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
-    return rows * (8 * (parts + TR_BINS + 2 * buckets) + 4 * (buckets + TR_LIST + 1) + 16);
+    return rows * (8 * (parts + TR_BINS + parts * TR_GROUPS + buckets) + 4 * (buckets + TR_LIST + 1) + 16);
 }
 
 extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long stride, int rows, int vocab, const float *inv_t,
@@ -878,7 +982,8 @@ extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long 
     const int bits = log_vocab > 16 ? 62 - log_vocab : 46;
     const TruncArgs a{logits, stride, vocab, bits, inv_t, top_k, top_p, min_p, uniform, seed, key, step, tokens, host_mapped, kept, logprob};
     if (!trunc_split(vocab)) {
-        hipLaunchKernelGGL(sample_truncated_kernel, dim3(rows), dim3(TR_THREADS), 0, stream, a);
+        if (vocab <= TR_HELD_VOCAB) hipLaunchKernelGGL(sample_truncated_kernel<true>, dim3(rows), dim3(TR_THREADS), 0, stream, a);
+        else hipLaunchKernelGGL(sample_truncated_kernel<false>, dim3(rows), dim3(TR_THREADS), 0, stream, a);
         KVA_CHECK_LAUNCH("sample_truncated");
         return KVA_OK;
     }
@@ -889,7 +994,7 @@ extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long 
     sp.best = (u64 *)workspace;
     sp.bins = sp.best + (size_t)rows * sp.parts;
     sp.tops = sp.bins + (size_t)rows * TR_BINS;
-    sp.sought = sp.tops + (size_t)rows * sp.buckets;
+    sp.sought = sp.tops + (size_t)rows * sp.parts * TR_GROUPS;
     sp.sums = sp.sought + (size_t)rows * 2;
     sp.counts = (unsigned *)(sp.sums + (size_t)rows * sp.buckets);
     sp.list = (int *)(sp.counts + (size_t)rows * sp.buckets);

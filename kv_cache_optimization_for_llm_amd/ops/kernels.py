@@ -1330,7 +1330,8 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
        [0, 1)) or, without it, the number that :func:`sample` draws for (``seed``, ``rng_key``, ``rng_step``).
 
     Weights are held to 2^-45 of the best one's for vocabularies of up to 131,072 (half as finely for every doubling) and added up
-    exactly; tokens of less than half of that keep their place in the order and are never drawn.  Rows whose ``inv_temperature`` is
+    exactly; tokens of less than half of that keep their place in the order and are never drawn, and a ``min_p`` below an eighth of it is
+    none.  Rows whose ``inv_temperature`` is
     not above 0 take the best token.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability among
     them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
     tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
