@@ -9,10 +9,17 @@
 // One pass: the logits and a byte of marks a token come in 4 tokens a thread and load, a count is looked up only where the mark is
 // set, a grammar is a bit a token.  A row's biases are a list in no order: every workgroup picks out those of its own tokens,
 // 256 at a time, in the list's order, and the threads that hold the tokens add them.  What is computed is 32-bit throughout.
+//
+// What bounds it: memory.  A workgroup takes 1,024 tokens, which is as many loads on their way as there are (2,048 / 4,096 a workgroup:
+// one row of 128,256 5.1 / 7.4 us instead of 4.0, 256 rows with marks and counts 82 / 95 instead of 76).  Where the rows, what they
+// become and their marks are more than the memory-side cache's 256 MiB, all of it passes the caches by: 256 rows 59 to 63 us (4.7 TB/s) instead of
+// 76, and 109 instead of 110 with a draw behind it; 192 rows (210 MiB) 41 instead of 43, but 86 instead of 79 with the draw, which then finds nothing kept.
+// us in a graph: 1 row with everything 4.0, 64 rows with everything 18.1 (74 MB, 4.1 TB/s).
 #include "common.h"
 
 #define AL_THREADS 256
 #define AL_WAVES (AL_THREADS / KVA_WAVE)
+#define AL_UNITS 1
 
 typedef float al_f32x4 __attribute__((ext_vector_type(4), aligned(4)));         // (rows start at any multiple of their type)
 typedef uint16_t al_u16x4 __attribute__((ext_vector_type(4), aligned(2)));
@@ -37,7 +44,7 @@ struct AdjustArgs {
 };
 
 // grid (tiles, rows); a tile is UNITS x 1,024 tokens
-template <typename T, int UNITS>
+template <typename T, int UNITS, bool STREAMED>
 __global__ void __launch_bounds__(AL_THREADS)
 adjust_logits_kernel(AdjustArgs a) {
     __shared__ int hit_token[AL_THREADS];
@@ -52,10 +59,12 @@ adjust_logits_kernel(AdjustArgs a) {
         const int t = tile0 + 4 * (u * AL_THREADS + tid);
         if (t + 3 < vocab) {
             if constexpr (sizeof(T) == 4) {
-                const al_f32x4 v = *reinterpret_cast<const al_f32x4 *>(in + t);
+                const al_f32x4 *p = reinterpret_cast<const al_f32x4 *>(in + t);
+                const al_f32x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
                 l[u][0] = v.x, l[u][1] = v.y, l[u][2] = v.z, l[u][3] = v.w;
             } else {
-                const al_u16x4 v = *reinterpret_cast<const al_u16x4 *>(in + t);
+                const al_u16x4 *p = reinterpret_cast<const al_u16x4 *>(in + t);
+                const al_u16x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
                 l[u][0] = bf16_bits_to_float(v.x), l[u][1] = bf16_bits_to_float(v.y);
                 l[u][2] = bf16_bits_to_float(v.z), l[u][3] = bf16_bits_to_float(v.w);
             }
@@ -79,7 +88,8 @@ adjust_logits_kernel(AdjustArgs a) {
                 const int t = tile0 + 4 * (u * AL_THREADS + tid);
                 unsigned m = 0;
                 if (t + 3 < vocab) {
-                    const al_u8x4 v = *reinterpret_cast<const al_u8x4 *>(marks + t);
+                    const al_u8x4 *p = reinterpret_cast<const al_u8x4 *>(marks + t);
+                    const al_u8x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
                     m = (v.x != 0) | (v.y != 0) << 1 | (v.z != 0) << 2 | (v.w != 0) << 3;
                 } else {
 #pragma unroll
@@ -155,8 +165,11 @@ adjust_logits_kernel(AdjustArgs a) {
         v.y = bits & 2 ? l[u][1] : -INFINITY;
         v.z = bits & 4 ? l[u][2] : -INFINITY;
         v.w = bits & 8 ? l[u][3] : -INFINITY;
-        if (t + 3 < vocab) *reinterpret_cast<al_f32x4 *>(out + t) = v;
-        else
+        al_f32x4 *to = reinterpret_cast<al_f32x4 *>(out + t);
+        if (t + 3 < vocab) {
+            if (STREAMED) __builtin_nontemporal_store(v, to);
+            else *to = v;
+        } else
 #pragma unroll
             for (int i = 0; i < 3; ++i)
                 if (t + i < vocab) out[t + i] = v[i];
@@ -175,10 +188,13 @@ extern "C" int kva_adjust_logits(float *out, long long out_stride, const void *l
     if (rows == 0) return KVA_OK;
     const AdjustArgs a{logits, out, in_stride, out_stride, vocab, row_seat, seats, marks, counts, repetition, presence, frequency, bias_start,
                        bias_token, bias_value, biases, allowed_row, (const unsigned *)allowed, grammars, (vocab + 31) / 32};
-    const int tile = 4 * AL_THREADS;
+    const int tile = AL_UNITS * 4 * AL_THREADS;
+    const long long touched = (long long)rows * vocab * ((dtype == KVA_F32 ? 4 : 2) + 4 + (row_seat != nullptr ? 1 : 0));
+    const bool streamed = touched > 256ll << 20;
     const dim3 grid((vocab + tile - 1) / tile, rows), block(AL_THREADS);
-    if (dtype == KVA_F32) hipLaunchKernelGGL((adjust_logits_kernel<float, 1>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((adjust_logits_kernel<bf16_t, 1>), grid, block, 0, stream, a);
+    const auto kernel = dtype == KVA_F32 ? (streamed ? adjust_logits_kernel<float, AL_UNITS, true> : adjust_logits_kernel<float, AL_UNITS, false>)
+                                         : (streamed ? adjust_logits_kernel<bf16_t, AL_UNITS, true> : adjust_logits_kernel<bf16_t, AL_UNITS, false>);
+    hipLaunchKernelGGL(kernel, grid, block, 0, stream, a);
     KVA_CHECK_LAUNCH("adjust_logits");
     return KVA_OK;
 }

@@ -30,6 +30,7 @@
 // sought is the next turn's; the row is read again in every turn.
 #include "common.h"
 #include "counter_uniform.h"
+#include "wave_scan.h"
 
 #include <type_traits>
 
@@ -39,8 +40,6 @@
 #define TR_DIGITS 1024
 #define TR_PER (TR_DIGITS / TR_THREADS)
 #define TR_BUCKETS 1024                 // ranges of ids, in which what stays is added up
-
-typedef unsigned long long u64;
 
 struct TruncArgs {
     const float *logits;
@@ -126,42 +125,16 @@ __device__ inline void tr_fill_table(double *table) {
     if (threadIdx.x < TR_TABLE) table[threadIdx.x] = exp2((double)threadIdx.x / TR_TABLE);
 }
 
-// Numbers from lanes in front of this one, or `none` where there is no such lane.
-template <int CTRL, int ROWS>
-__device__ inline unsigned tr_from(unsigned v, unsigned none) {
-    return __builtin_amdgcn_update_dpp(none, v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS>
-__device__ inline u64 tr_from(u64 v, u64 none) {
-    return (u64)tr_from<CTRL, ROWS>((unsigned)(v >> 32), (unsigned)(none >> 32)) << 32 | tr_from<CTRL, ROWS>((unsigned)v, (unsigned)none);
-}
-// Inclusive prefix of the wavefront in the vector ALU: 1, 2, 4 and 8 lanes up inside rows of 16, then the last lane of a row to the
-// next one, then that of the first half to the second.
-template <typename T, typename OP>
-__device__ inline T tr_wave_scan(T v, T none, OP op) {
-    v = op(v, tr_from<0x111, 0xf>(v, none));
-    v = op(v, tr_from<0x112, 0xf>(v, none));
-    v = op(v, tr_from<0x114, 0xf>(v, none));
-    v = op(v, tr_from<0x118, 0xf>(v, none));
-    v = op(v, tr_from<0x142, 0xa>(v, none));
-    return op(v, tr_from<0x143, 0xc>(v, none));
-}
-template <typename T>
-__device__ inline T tr_wave_prefix(T v) {
-    return tr_wave_scan(v, (T)0, [](T a, T b) { return a + b; });
-}
-__device__ inline unsigned tr_last_lane(unsigned v) { return __builtin_amdgcn_readlane(v, KVA_WAVE - 1); }
-__device__ inline u64 tr_last_lane(u64 v) { return (u64)tr_last_lane((unsigned)(v >> 32)) << 32 | tr_last_lane((unsigned)v); }
 // Sum of numbers below 2^48 over the wavefront, in the last lane: 24 bits at a time, so that no step carries.
 __device__ inline u64 tr_wave_sum48(u64 v) {
-    const unsigned lo = tr_wave_prefix((unsigned)v & 0xffffffu), hi = tr_wave_prefix((unsigned)(v >> 24));
+    const unsigned lo = wave_prefix((unsigned)v & 0xffffffu), hi = wave_prefix((unsigned)(v >> 24));
     return ((u64)hi << 24) + lo;
 }
 __device__ inline u64 tr_wave_min(u64 v) {
-    return tr_last_lane(tr_wave_scan(v, ~0ull, [](u64 a, u64 b) { return a < b ? a : b; }));
+    return wave_last(wave_scan(v, ~0ull, [](u64 a, u64 b) { return a < b ? a : b; }));
 }
 __device__ inline u64 tr_wave_max(u64 v) {
-    return tr_last_lane(tr_wave_scan(v, 0ull, [](u64 a, u64 b) { return a > b ? a : b; }));
+    return wave_last(wave_scan(v, 0ull, [](u64 a, u64 b) { return a > b ? a : b; }));
 }
 
 #define TR_PAIRS 128                    // so many tokens are compared with one another
@@ -194,8 +167,8 @@ __device__ inline void tr_block_range(TruncShared &s, u64 &lo, u64 &hi) {
 // Inclusive prefix sums of a number and a count a thread over the workgroup.
 __device__ inline void tr_block_prefix(TruncShared &s, u64 &v, unsigned &c) {
     const int lane = threadIdx.x % KVA_WAVE, wave = threadIdx.x / KVA_WAVE;
-    v = tr_wave_prefix(v);
-    c = tr_wave_prefix(c);
+    v = wave_prefix(v);
+    c = wave_prefix(c);
     __syncthreads();
     if (lane == KVA_WAVE - 1) s.part[wave] = v, s.part_count[wave] = c;
     __syncthreads();
@@ -392,7 +365,7 @@ __device__ inline void tr_draw(const TruncArgs &a, TruncShared &s, const float *
         unsigned unused;
         tr_load4(rl, t, a.vocab, l);
         tr_stay4(l, t, weigh, last, least, w, unused);
-        const u64 mine = w[0] + w[1] + w[2] + w[3], upto = tr_wave_prefix(mine), whole = tr_last_lane(upto);
+        const u64 mine = w[0] + w[1] + w[2] + w[3], upto = wave_prefix(mine), whole = wave_last(upto);
         if (target >= run + whole) {            // (the same in all lanes; a range's sum is its tokens')
             run += whole;
             continue;
@@ -486,7 +459,7 @@ __device__ inline void trunc_whole_row(const TruncArgs &a, TruncShared &s, const
 #pragma unroll
             for (int i = 0; i < 4; ++i) l[i] = next[i];
         }
-        count = tr_wave_prefix(count);
+        count = wave_prefix(count);
         if (lane == KVA_WAVE - 1) s.bucket_sum[b] = sum, s.bucket_count[b] = count;
     }
     __syncthreads();
@@ -690,7 +663,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
         u64 mine = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) mine += v[i];
-        u64 upto = tr_wave_prefix(mine);
+        u64 upto = wave_prefix(mine);
         if (lane == KVA_WAVE - 1) of_wave[wave] = upto;
         if (tid == 0) cut_bin = TR_BINS - 1;            // (fewer tokens than k: all of them)
         __syncthreads();
@@ -751,7 +724,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
                         count += stays ? 1 : 0;
                     }
                     sum = tr_wave_sum48(sum);
-                    count = tr_wave_prefix(count);
+                    count = wave_prefix(count);
                 }
                 if (__any(asks[0] || asks[1] || asks[2] || asks[3])) {
 #pragma unroll
