@@ -10,7 +10,8 @@ Names and meanings follow the reference (``base/src/main.cu:42-105``,
 * ``IGNORE_EOS=1`` runs every request to its full budget; ``TEMPERATURE`` (unset or <= 0 is
   greedy) and ``SAMPLING_SEED`` choose the sampler; ``ORCA_POLICY=max|pow2|oracle`` is the
   contiguous mode's reservation policy; ``PREEMPTION_POLICY=recompute`` (``swap`` is refused:
-  this engine recomputes); ``REPETITION_PENALTY`` (the reference fixes 1.15);
+  this engine recomputes); ``REPETITION_PENALTY`` (the reference fixes 1.15); beyond the reference, for every request,
+  ``TOP_K``, ``TOP_P``, ``MIN_P``, ``PRESENCE_PENALTY`` and ``FREQUENCY_PENALTY`` (unset: none);
 * a request line is ``<request_id> <max_tokens> <n_seqs> <token> <token> ...``; a malformed
   line is reported on standard error and ignored;
 * output lines: ``{"type":"engine_config",...}`` once, ``{"id","slot","seq","tok"}`` per
@@ -137,6 +138,14 @@ def main(argv=None) -> int:
               file=sys.stderr)
         return 1
     penalty = float(env.get("REPETITION_PENALTY", "1.15") or 1.15)
+    asked = {name: kind(env[name.upper()]) for name, kind in (("top_k", int), ("top_p", float), ("min_p", float), ("presence_penalty", float),
+                                                              ("frequency_penalty", float)) if env.get(name.upper())}
+    from ..sampling.options import SampleOptions
+    try:
+        sampling = SampleOptions(**asked) if asked else None
+    except ValueError as e:
+        print(f"Unusable sampling options: {e}", file=sys.stderr)
+        return 1
     if temperature > 0:
         print(f"Sampling: temperature {temperature}, seed {seed} (greedy decoding is OFF)", file=sys.stderr)
 
@@ -149,12 +158,12 @@ def main(argv=None) -> int:
         gemm_tune_rows=serve_tune_rows(args.max_seqs, args.chunk_size, args.max_batch_tokens)
         if args.gemm_tune_rows == "auto" else [int(r) for r in args.gemm_tune_rows.split(",") if r.strip()]))
     runner = Runner(engine, ServeOptions(
-        temperature=temperature, sampling_seed=seed, ignore_eos=ignore_eos, repetition_penalty=penalty,
+        temperature=temperature, sampling_seed=seed, ignore_eos=ignore_eos, repetition_penalty=penalty, sampling=sampling,
         max_batch_tokens=args.max_batch_tokens, chunk_size=args.chunk_size, reserve_policy=policy))
     emit({"type": "engine_config", "mechanism": args.cache_mode, "batch_size": args.max_seqs,
           "max_batch_tokens": args.max_batch_tokens, "max_seq_len": engine.max_seq_len,
           "page_size": args.page_size, "temperature": temperature, "sampling_seed": seed,
-          "reserve_policy": policy, "preemption_policy": preemption, "repetition_penalty": penalty,
+          "reserve_policy": policy, "preemption_policy": preemption, "repetition_penalty": penalty, **asked,
           "dtype": args.dtype, "kv_pool_tokens": engine.cache.num_pages * args.page_size,
           "architecture": engine.spec.architecture})
 

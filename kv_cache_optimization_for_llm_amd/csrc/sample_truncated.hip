@@ -45,7 +45,7 @@ struct TruncArgs {
     const float *logits;
     long long stride;
     int vocab, scale_bits;
-    const float *inv_t;                 // <= 0: the best token
+    const float *inv_t;                 // <= 0: the best token; no number: the row is passed over
     const int *top_k;                   // absent: all of them
     const float *top_p, *min_p;
     const float *uniform;               // absent: the counter-based number of (seed, key, step)
@@ -473,6 +473,7 @@ __global__ void __launch_bounds__(TR_THREADS)
 sample_truncated_kernel(TruncArgs a) {
     __shared__ TruncShared s;
     __shared__ __attribute__((aligned(16))) float held[HELD ? TR_HELD_VOCAB : 4];
+    if (isnan(a.inv_t[blockIdx.x])) return;
     tr_fill_table(s.table);             // (the first barrier comes before its first use)
     const float *rl = a.logits + blockIdx.x * a.stride;
     if (HELD) {
@@ -543,6 +544,7 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ u64 of_wave[TR_SPLIT_WAVES];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     const float *rl = a.logits + row * a.stride;
+    if (isnan(a.inv_t[row])) return;
     // (the next launches add to these)
     const int per = (TR_BINS + sp.parts - 1) / sp.parts;
     for (int i = part * per + tid; i < min(TR_BINS, (part + 1) * per); i += TR_SPLIT_THREADS) sp.bins[(size_t)row * TR_BINS + i] = 0;
@@ -776,6 +778,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     const int row = blockIdx.x, tid = threadIdx.x, bits = a.scale_bits, vocab = a.vocab;
     const float *rl = a.logits + row * a.stride;
     const float inv_t = a.inv_t[row];
+    if (isnan(inv_t)) return;
     const int mode = tr_mode(a, sp, row), groups = sp.parts * TR_GROUPS;
     // everything that hangs on nothing else is asked for at once
     const bool drawn = inv_t > 0.f, sums = drawn && (mode == TR_ALL || mode == TR_WEIGHT);

@@ -19,6 +19,7 @@ from ..cache.manager import CacheManager
 from ..cache.manager import page_bytes as cache_page_bytes
 from ..config.model_config import read_config_json
 from ..models.builder import Model, spec_for_config
+from ..ops.kernels import MAX_STEP_ENTRIES, MAX_STEP_GROUPS
 from ..ops.library import KernelLibraryError, hip_lib
 from ..weights.loader import load_tensors
 from ..weights.random_init import random_tensors_on_device
@@ -171,7 +172,8 @@ class Engine:
         if options.use_graphs and self.dtype == torch.bfloat16 and self.model.graph_safe():
             from .graphs import DecodeGraphs, PortionGraphs
             self.graphs = DecodeGraphs(self.model, self.cache, self.device, self.feedback)
-            self.portion_graphs = PortionGraphs(self.model, self.cache, self.device, self.feedback)
+            if len(groups) <= MAX_STEP_GROUPS:
+                self.portion_graphs = PortionGraphs(self.model, self.cache, self.device, self.feedback)
 
     # ------------------------------------------------------------------ requests
     def has_request(self, request_id) -> bool:
@@ -250,8 +252,10 @@ class Engine:
                 return logits
             slot_maps = [[m[i:i + 1] for i in range(len(seats))] for m in slots]
         else:
-            slot_maps = [[self.cache.slot_mapping(seat, start, len(arr), g.index)
-                          for seat, start, arr in zip(seats, starts, toks)] for g in groups]
+            slot_maps = None        # the device makes them from the entries' lengths and its block tables
+            for g in groups:
+                for seat, start, arr in zip(seats, starts, toks):
+                    self.cache.check_mapped(seat, start, len(arr), g.index)
             self.cache.flush_tables()
             if self.portion_graphs is not None:
                 # a step shape that has been seen before runs from its graph
@@ -261,18 +265,23 @@ class Engine:
                 if key is not None:
                     logits = self.portion_graphs.run(
                         key, np.concatenate([np.asarray(t, dtype=np.int32) for t in toks]),
-                        np.asarray(seats, dtype=np.int32), np.asarray(starts, dtype=np.int32),
-                        [np.concatenate(m).astype(np.int32) for m in slot_maps])
+                        np.asarray(seats, dtype=np.int32), np.asarray(starts, dtype=np.int32))
                     if logits is not None:
                         return logits
-                    batch = build_batch(seats, starts, toks, wants, slot_maps, self.device)
-                    batch.feedback = self.feedback
+                    batch = self._batch(seats, starts, toks, wants, slot_maps)
                     logits = self.model.forward(batch, self.cache)
                     self.portion_graphs.note(key, batch)
                     return logits
-        batch = build_batch(seats, starts, toks, wants, slot_maps, self.device)
+        return self.model.forward(self._batch(seats, starts, toks, wants, slot_maps), self.cache)
+
+    def _batch(self, seats, starts, toks, wants, slot_maps) -> StepBatch:
+        groups = self.cache.groups
+        if slot_maps is None and (len(seats) > MAX_STEP_ENTRIES or len(groups) > MAX_STEP_GROUPS):
+            slot_maps = [[self.cache.slot_mapping(seat, start, len(arr), g.index)
+                          for seat, start, arr in zip(seats, starts, toks)] for g in groups]
+        batch = build_batch(seats, starts, toks, wants, slot_maps, self.device, [g.table_dev for g in groups], self.cache.page_size)
         batch.feedback = self.feedback
-        return self.model.forward(batch, self.cache)
+        return batch
 
     def _place(self, entries: Sequence[StepEntry]):
         """Seats, start positions and pages for every entry of the step."""

@@ -26,6 +26,7 @@ import torch
 
 from collections import OrderedDict
 
+from ..ops import kernels as K
 from .batch import StepBatch, attention_work_items
 
 
@@ -157,13 +158,12 @@ class _PortionSlot:
         self.T, self.E = T, E
         self.q_start = np.zeros(E + 1, dtype=np.int32)
         np.cumsum(lens, out=self.q_start[1:])
-        # the int32 staging buffer: token_ids, positions, tok_seat [T each], entry_seat,
-        # entry_start_pos [E each], one slot mapping [T] per cache group, then for every set of
-        # attention items the forward pass asks for: entry [n], row0 [n], meta [n, 8]
+        # the int32 staging buffer: token_ids [T], entry_seat, entry_start_pos [E each], then for every set of
+        # attention items the forward pass asks for: entry [n], row0 [n], meta [n, 8].  What a row holds beside its token -
+        # position, seat, and a slot per cache group [T each] - is made on the device in front of the graph
         self.at: Dict[str, Tuple[int, int]] = {}
         total = 0
-        for name, n in [("token_ids", T), ("positions", T), ("tok_seat", T), ("entry_seat", E),
-                        ("entry_start_pos", E)] + [(f"slots{g}", T) for g in range(num_groups)]:
+        for name, n in [("token_ids", T), ("entry_seat", E), ("entry_start_pos", E)]:
             self.at[name] = (total, n)
             total += (n + 3) // 4 * 4
         self.variants = list(variants)
@@ -177,11 +177,14 @@ class _PortionSlot:
         self.dev = torch.zeros(max(1, total), dtype=torch.int32, device=device)
         self.const = torch.cat([torch.from_numpy(self.q_start),
                                 torch.tensor(rows, dtype=torch.int32)]).to(device)
+        self.entry_len = torch.tensor(lens, dtype=torch.int32).to(device)
+        self.made_q_start = torch.zeros(E + 1, dtype=torch.int32, device=device)
+        made = torch.zeros((2 + num_groups, (T + 3) // 4 * 4), dtype=torch.int32, device=device)[:, :T]
         v = lambda name: self.dev[self.at[name][0]:self.at[name][0] + self.at[name][1]]
         self.batch = StepBatch(
             num_tokens=T, num_entries=E, num_logit_rows=R,
-            token_ids=v("token_ids"), positions=v("positions"), tok_seat=v("tok_seat"),
-            logit_rows=self.const[E + 1:], slot_mapping=[v(f"slots{g}") for g in range(num_groups)],
+            token_ids=v("token_ids"), positions=made[0], tok_seat=made[1],
+            logit_rows=self.const[E + 1:], slot_mapping=[made[2 + g] for g in range(num_groups)],
             entry_seat=v("entry_seat"), entry_q_start=self.const[:E + 1], entry_start_pos=v("entry_start_pos"),
             max_q_len=int(max(lens)), min_q_len=int(min(lens)), max_context=bucket,
             logits_for_all_rows=tuple(rows) == tuple(range(T)), feedback=feedback, static_items=True)
@@ -193,8 +196,7 @@ class _PortionSlot:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.logits: Optional[torch.Tensor] = None
 
-    def fill(self, tokens: np.ndarray, seats: np.ndarray, starts: np.ndarray,
-             slot_maps: Sequence[np.ndarray]) -> None:
+    def fill(self, tokens: np.ndarray, seats: np.ndarray, starts: np.ndarray, cache) -> None:
         self.copied.synchronize()        # the previous upload has left the staging buffer
         st = self.staging.numpy()
 
@@ -202,12 +204,8 @@ class _PortionSlot:
             o, n = self.at[name]
             st[o:o + n] = arr
         put("token_ids", tokens)
-        put("positions", np.repeat(starts - self.q_start[:-1], self.lens) + np.arange(self.T, dtype=np.int32))
-        put("tok_seat", np.repeat(seats, self.lens))
         put("entry_seat", seats)
         put("entry_start_pos", starts)
-        for g, sm in enumerate(slot_maps):
-            put(f"slots{g}", sm)
         for (group, tiles, which), (o, n) in zip(self.variants, self.items_at):
             ent, row0, meta = attention_work_items(self.q_start, starts, seats, group, tiles, which)
             st[o:o + n], st[o + n:o + 2 * n] = ent, row0
@@ -215,6 +213,9 @@ class _PortionSlot:
         self.batch.h_entry_start_pos, self.batch.h_entry_seat = starts, seats
         self.dev.copy_(self.staging, non_blocking=True)
         self.copied.record()
+        b = self.batch
+        K.step_rows(self.entry_len, b.entry_start_pos, b.entry_seat, [g.table_dev for g in cache.groups], cache.page_size,
+                    self.made_q_start, b.positions, b.tok_seat, b.slot_mapping)
 
 
 class PortionGraphs:
@@ -253,7 +254,7 @@ class PortionGraphs:
     def shape_key(self, lens: Sequence[int], starts: Sequence[int], rows: Sequence[int]) -> Optional[tuple]:
         from ..ops.attention import portion_choice
         T = int(sum(lens))
-        if T > PortionGraphs.MAX_TOKENS or len(rows) > PortionGraphs.MAX_LOGIT_ROWS:
+        if T > PortionGraphs.MAX_TOKENS or len(rows) > PortionGraphs.MAX_LOGIT_ROWS or len(lens) > K.MAX_STEP_ENTRIES:
             return None
         ln, st = np.asarray(lens, dtype=np.float64), np.asarray(starts, dtype=np.float64)
         long = ln > 1
@@ -287,8 +288,7 @@ class PortionGraphs:
             self.slots.popitem(last=False)
         return kept
 
-    def run(self, key: tuple, tokens: np.ndarray, seats: np.ndarray, starts: np.ndarray,
-            slot_maps: Sequence[np.ndarray]) -> Optional[torch.Tensor]:
+    def run(self, key: tuple, tokens: np.ndarray, seats: np.ndarray, starts: np.ndarray) -> Optional[torch.Tensor]:
         """Logits ``[wanted places, vocab]`` of the step, or ``None`` when the shape is new (the
         caller runs it eagerly and calls :meth:`note`)."""
         variants = self.seen.get(key)
@@ -308,7 +308,7 @@ class PortionGraphs:
             slot.kept = kept
         else:
             self.slots.move_to_end(key)
-        slot.fill(tokens, seats, starts, slot_maps)
+        slot.fill(tokens, seats, starts, self.cache)
         if slot.graph is None:
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()

@@ -2,9 +2,10 @@
 from __future__ import annotations
 
 from dataclasses import dataclass, replace
-from typing import Dict, Iterable, List, Optional, Sequence
+from typing import Dict, Iterable, List, Optional, Sequence, Union
 
-from ..sampling.sampler import SampleRow, Sampler
+from ..sampling.options import SampleOptions, pack_allowed
+from ..sampling.sampler import OptionRow, SampleRow, Sampler
 from .batch import StepEntry
 from .engine import Engine, EngineOptions
 from .scheduler import Event, Request, Scheduler, StepPlan, UnresolvedTokens
@@ -33,6 +34,7 @@ class ServeOptions:
     max_batch_tokens: int = 3072        # MAX_BATCH_TOKENS: a step's token budget
     chunk_size: Optional[int] = None    # most prompt tokens of one request per step
     reserve_policy: str = "max"         # ORCA_POLICY: max | pow2 | oracle (contiguous mode)
+    sampling: Optional[SampleOptions] = None    # of requests that bring no options of their own
     run_ahead: bool = True              # launch a step before the host has seen the previous step's tokens
 
 
@@ -53,40 +55,54 @@ class Runner:
         self.scheduler.on_admit = self._on_admit
         self.scheduler.on_release = self._on_release
         self._next_id = 0
+        self._grammars = 0            # seated sequences that have a grammar
+        self._kept: List[Event] = []  # events of a step that raised
         self._in_flight = None        # (ticket, pending tokens) of the step launched last
 
     # the scheduler owns seats; the engine only needs to know which request sits where
     def _on_admit(self, seq) -> None:
         self.engine.bind_request(engine_key(seq.request), seq.seat)
+        options = seq.request.options
         emitted = seq.prompt[len(seq.prompt) - seq.request.resumed_tokens:] if seq.request.resumed_tokens else ()
-        self.sampler.reset_seat(seq.seat, emitted)
+        if options is None:
+            self.sampler.reset_seat(seq.seat, emitted)
+        else:
+            self._grammars += options.grammar is not None
+            self.sampler.reset_seat(seq.seat, emitted, seq.prompt[:len(seq.prompt) - seq.request.resumed_tokens], options)
 
     def _on_release(self, seq) -> None:
+        if seq.request.options is not None:
+            self._grammars -= seq.request.options.grammar is not None
         self.engine.unbind_request(engine_key(seq.request))
 
     def submit(self, tokens: Sequence[int], max_new_tokens: int, *, request_id: Optional[int] = None,
-               n_seqs: int = 1, temperature: Optional[float] = None) -> int:
+               n_seqs: int = 1, temperature: Optional[float] = None, options: Optional[SampleOptions] = None) -> int:
         """Queues ``n_seqs`` copies of a request (reference wire format:
-        ``<id> <max_tokens> <n_seqs> <tok> ...``, ``base/src/request_queue.cpp:11-61``)."""
+        ``<id> <max_tokens> <n_seqs> <tok> ...``, ``base/src/request_queue.cpp:11-61``).  ``options``: what it asks of its
+        sampling beyond the temperature; without them the server's."""
         if not 1 <= n_seqs <= MAX_PARALLEL_SEQUENCES:
             raise ValueError(f"n_seqs {n_seqs} is not in 1..{MAX_PARALLEL_SEQUENCES}")
         if request_id is None:
             request_id = self._next_id
         self._next_id = max(self._next_id, request_id + 1)
         t = self.options.temperature if temperature is None else temperature
+        options = self.options.sampling if options is None else options
+        if options is not None and any(token >= self.engine.vocab_size for token in options.logit_bias or ()):
+            raise ValueError(f"logit_bias names a token outside the vocabulary of {self.engine.vocab_size}")
         for i in range(n_seqs):
             self.scheduler.add(Request(request_id, [int(x) for x in tokens], int(max_new_tokens),
-                                       seq_index=i, temperature=float(t)))
+                                       seq_index=i, temperature=float(t), options=options))
         return request_id
 
     def idle(self) -> bool:
-        return self.scheduler.idle() and self._in_flight is None
+        return self.scheduler.idle() and self._in_flight is None and not self._kept
 
     def cancel(self, request_id: int) -> List[Event]:
         """Ends a request now, whatever it was doing: the tokens of the step in flight are taken
         first (they are returned as events, before the ``done`` events with reason ``cancelled``),
         then its sequences leave the queue or give back their seats and pages."""
-        events = self._resolve_in_flight()
+        events, self._kept = self._kept, []
+        events.extend(self._resolve_in_flight())
         events.extend(self.scheduler.cancel(request_id))
         return events
 
@@ -105,12 +121,23 @@ class Runner:
             if e.sample:
                 req = e.seq.request
                 emitted_before = req.resumed_tokens + len(e.seq.generated)
-                rows.append(SampleRow(e.seq.seat, req.temperature, req.id * MAX_PARALLEL_SEQUENCES + req.seq_index,
-                                      e.start + len(e.tokens), apply_penalty=emitted_before > 0))
+                row = (e.seq.seat, req.temperature, req.id * MAX_PARALLEL_SEQUENCES + req.seq_index,
+                       e.start + len(e.tokens), emitted_before > 0)
+                if req.options is None:
+                    rows.append(SampleRow(*row))
+                else:
+                    rows.append(OptionRow(*row, options=req.options, allowed=self._allowed(e.seq)))
         logits = self.engine.step_planned(entries, [e.seq.seat for e in plan.entries],
                                           [e.start for e in plan.entries])
         # the tokens also stay on the device, where the next step's entries can name them
         return self.sampler.sample_async(logits, rows, out=self.engine.feedback)
+
+    def _allowed(self, seq):
+        """What a sequence's grammar leaves for its next token."""
+        req = seq.request
+        if req.options.grammar is None:
+            return None
+        return pack_allowed(req.options.grammar(req.tokens[len(req.tokens) - req.resumed_tokens:] + seq.generated), self.engine.vocab_size)
 
     def _resolve_in_flight(self) -> List[Event]:
         if self._in_flight is None:
@@ -123,24 +150,36 @@ class Runner:
         """Plans and launches one step.  With ``run_ahead`` the events of a step are returned by
         the call after the one that launched it (the device works on a step while the host
         prepares the next); without it every call waits for its own tokens."""
-        events: List[Event] = []
+        events, self._kept = self._kept, []
+        try:
+            self._step(events)
+        except BaseException:
+            self._kept = events         # what this call has seen is told by the next one
+            raise
+        return events
+
+    def _step(self, events: List[Event]) -> None:
+        if self._grammars and any(s.unresolved and s.request.options is not None and s.request.options.grammar is not None
+                                  for s in self.scheduler.running):
+            events.extend(self._resolve_in_flight())        # a grammar asks for the values of the tokens so far
         try:
             plan = self.scheduler.plan()
         except UnresolvedTokens:
             events.extend(self._resolve_in_flight())
             plan = self.scheduler.plan()
         launched = None
-        if plan.entries:
-            if len([e for e in plan.entries if e.sample]) > self.engine.feedback.shape[0]:
-                raise RuntimeError("more sampled rows than the engine's feedback buffer holds")
-            pending = self._launch(plan)
-            launched = (self.scheduler.book(plan), pending)
-        events.extend(self._resolve_in_flight())      # the step before the one just launched
-        events.extend(plan.events)
+        try:
+            if plan.entries:
+                if len([e for e in plan.entries if e.sample]) > self.engine.feedback.shape[0]:
+                    raise RuntimeError("more sampled rows than the engine's feedback buffer holds")
+                pending = self._launch(plan)
+                launched = (self.scheduler.book(plan), pending)
+            events.extend(self._resolve_in_flight())      # the step before the one just launched
+        finally:
+            events.extend(plan.events)
         self._in_flight = launched
         if launched is not None and not self.options.run_ahead:
             events.extend(self._resolve_in_flight())
-        return events
 
     def run_until_idle(self) -> Iterable[Event]:
         while not self.idle():
@@ -164,8 +203,9 @@ class LLM:
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 16, *,
                  temperature: Optional[float] = None, seed: Optional[int] = None,
                  ignore_eos: Optional[bool] = None, repetition_penalty: Optional[float] = None,
-                 return_reasons: bool = False):
-        """Generates for every prompt (token ids in, token ids out), batched continuously."""
+                 options: Union[None, SampleOptions, Sequence[Optional[SampleOptions]]] = None, return_reasons: bool = False):
+        """Generates for every prompt (token ids in, token ids out), batched continuously.  ``options``: what the requests ask of
+        their sampling, one for all of them or one each (None: the server's)."""
         opts = ServeOptions(**vars(self.serve_options))
         if temperature is not None:
             opts.temperature = temperature
@@ -176,7 +216,10 @@ class LLM:
         if repetition_penalty is not None:
             opts.repetition_penalty = repetition_penalty
         runner = Runner(self.engine, opts)
-        ids = [runner.submit(p, max_new_tokens) for p in prompts]
+        each = [options] * len(prompts) if options is None or isinstance(options, SampleOptions) else list(options)
+        if len(each) != len(prompts):
+            raise ValueError(f"{len(each)} options for {len(prompts)} prompts")
+        ids = [runner.submit(p, max_new_tokens, options=o) for p, o in zip(prompts, each)]
         out: Dict[int, List[int]] = {i: [] for i in ids}
         reasons: Dict[int, str] = {}
         for ev in runner.run_until_idle():

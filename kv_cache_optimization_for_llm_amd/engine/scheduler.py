@@ -57,6 +57,7 @@ class Request:
     resumed_tokens: int = 0           # how many of ``tokens`` (at the end) were generated before a preemption
     arrival: int = -1
     preempted: bool = False           # re-entered after a preemption (possibly with nothing generated yet)
+    options: object = None            # what the request asks of its sampling (sampling.options.SampleOptions)
 
 
 @dataclass
@@ -232,7 +233,7 @@ class Scheduler:
                             generated=done_before, reason="recompute"))
         resumed = Request(seq.request.id, tokens, seq.remaining, seq.request.seq_index,
                           seq.request.temperature, resumed_tokens=done_before,
-                          arrival=seq.request.arrival, preempted=True)
+                          arrival=seq.request.arrival, preempted=True, options=seq.request.options)
         if not seq.was_preempted:
             self._preempted_in_flight += 1
         self.preemption_pending = True

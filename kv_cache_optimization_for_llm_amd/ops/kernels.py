@@ -1332,7 +1332,7 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     Weights are held to 2^-45 of the best one's for vocabularies of up to 131,072 (half as finely for every doubling) and added up
     exactly; tokens of less than half of that keep their place in the order and are never drawn, and a ``min_p`` below an eighth of it is
     none.  Rows whose ``inv_temperature`` is
-    not above 0 take the best token.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability among
+    not above 0 take the best token, and rows where it is no number are passed over: what stands in the outputs stays.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability among
     them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
     tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
     what = "sample_truncated"
@@ -1363,6 +1363,10 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     space = torch.empty(size // 4, dtype=i32, device=logits.device) if size else None
     check(lib.kva_sample_truncated(tokens, logits.data_ptr(), stride, rows, vocab, *args, space.data_ptr() if size else None, _stream()), what)
     return out_tokens
+
+
+# what one launch of grow_tables or step_rows takes
+MAX_STEP_ENTRIES, MAX_STEP_GROUPS = 4096, 8
 
 
 def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, lengths: torch.Tensor, page_size: int,
@@ -2972,6 +2976,8 @@ KERNEL_CLASSES = {
     "gemv": "gemm (few rows)", "gemv_qkv_rope": "gemm (few rows)", "gemv_merged": "gemm (few rows)",
     "gemm_skinny_partials": "gemm (few rows)",
     "sample": "sampling", "sample_by_value": "sampling", "mark_tokens": "sampling",
+    "sample_truncated": "sampling", "adjust_logits": "sampling", "count_tokens": "sampling",
+    "grow_tables": "index arrays", "step_rows": "index arrays",
     "causal_conv_act": "recurrent mixers", "gated_delta_rule": "recurrent mixers",
     "gated_linear_attention": "recurrent mixers", "head_norm_gate": "elementwise",
     "moe_route": "routed experts", "moe_router": "routed experts", "moe_align": "routed experts", "moe_table_align": "routed experts", "moe_expert_rows": "routed experts", "moe_expert_tiles": "routed experts", "moe_few_rows": "routed experts",

@@ -13,9 +13,13 @@ Options and their meaning follow the reference (``base/src/main.cu:57-84``,
   request has already emitted are divided (if positive) or multiplied (if negative) by it, from
   the second generated token on.  The emitted-token mask lives in the request's seat, one byte
   per vocabulary entry.
+
+A row with options of its own (:class:`OptionRow`) has its logits adjusted first and, where it asks for a cut, is drawn from what the
+cuts leave; the rows beside it draw what they would draw without it.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
@@ -24,6 +28,7 @@ import torch
 
 from ..ops import kernels as K
 from ..ops.library import sample_rows
+from .options import SampleOptions, pack_allowed
 
 
 def counter_uniform(seed: int, key: int, step: int) -> float:
@@ -45,6 +50,14 @@ class SampleRow:
     rng_key: int = 0
     rng_step: int = 0
     apply_penalty: bool = False
+
+
+@dataclass
+class OptionRow(SampleRow):
+    """A row whose request has options; ``allowed``: what its grammar leaves (:func:`~.options.pack_allowed`'s words, or None)."""
+
+    options: SampleOptions = SampleOptions()
+    allowed: Optional[np.ndarray] = None
 
 
 class _Staging:
@@ -128,6 +141,11 @@ class Sampler:
         self.mask: Optional[torch.Tensor] = None
         if self.penalty != 1.0:
             self.mask = torch.zeros((max_seqs, vocab_size), dtype=torch.uint8, device=device)
+        # of requests with options: which tokens their seats have emitted (the mask where there is one), and how often; made when
+        # the first request asks for them
+        self.marks: Optional[torch.Tensor] = self.mask
+        self.counts: Optional[torch.Tensor] = None
+        self.max_seqs = max_seqs
         # pinned landing buffers for sample_async, used in turn (two samplings may be in flight)
         self._landing: List[torch.Tensor] = []
         self._events: list = []             # one a landing buffer, recorded behind the sampling that fills it
@@ -162,14 +180,32 @@ class Sampler:
             staging.sent.synchronize()      # its last copy has left it (three steps ago)
         return staging, views
 
-    def reset_seat(self, seat: int, emitted: Sequence[int] = ()) -> None:
+    def reset_seat(self, seat: int, emitted: Sequence[int] = (), prompt: Sequence[int] = (),
+                   options: Optional[SampleOptions] = None) -> None:
         """A request takes the seat: clear its mask and mark what it has emitted before (a
         recomputed request arrives with its earlier output)."""
+        counted = options is not None and (options.penalizes or (options.penalize_prompt and self.mask is not None))
+        if counted and self.counts is None:
+            if self.marks is None:
+                self.marks = torch.zeros((self.max_seqs, self.vocab_size), dtype=torch.uint8, device=self.device)
+            self.counts = torch.zeros((self.max_seqs, self.vocab_size), dtype=torch.int32, device=self.device)
+        if counted:
+            self.marks[seat].zero_()
+            self.counts[seat].zero_()
+            if len(emitted):
+                K.count_tokens(self.marks, self.counts, *self._pairs(seat, emitted))
+            if options.penalize_prompt and len(prompt):
+                K.count_tokens(self.marks, None, *self._pairs(seat, prompt))
+            return
         if self.mask is None:
             return
         self.mask[seat].zero_()
         if len(emitted):
             self.mark([seat] * len(emitted), emitted)
+
+    def _pairs(self, seat: int, tokens: Sequence[int]):
+        t = torch.from_numpy(np.asarray(tokens, dtype=np.int32)).to(self.device)
+        return torch.full_like(t, seat), t
 
     def mark(self, seats: Sequence[int], tokens: Sequence[int]) -> None:
         if self.mask is None or not len(seats):
@@ -208,6 +244,14 @@ class Sampler:
             event.record()
             return PendingTokens(host, event, 0)
         landing = host if self._kernel_writes_host else None
+        if OptionRow in set(map(type, rows)):
+            try:
+                self._sample_options(logits, rows, out, landing)
+                if landing is None:
+                    host[:n].copy_(out, non_blocking=True)
+            finally:
+                event.record()
+            return PendingTokens(host, event, n)
         if n <= K.sample_rows_by_value():
             args = self._args_few
             if args is None:
@@ -250,3 +294,85 @@ class Sampler:
         finally:
             event.record()
         return PendingTokens(host, event, n)
+
+    def _sample_options(self, logits: torch.Tensor, rows: Sequence[SampleRow], out: torch.Tensor, landing: Optional[torch.Tensor]) -> None:
+        """Rows some of which have options: adjusted logits, a draw of the rows without a cut as ever, a draw of the others."""
+        n, vocab = len(rows), self.vocab_size
+        opts = [r.options if isinstance(r, OptionRow) else None for r in rows]
+        cut = [o is not None and o.truncates and r.temperature > 0 for o, r in zip(opts, rows)]
+        # who is penalised by adjusting its logits (its own penalties, or the sampler's), and who in the draw (rows without options)
+        own = [o is not None and (o.penalizes or (self.mask is not None and (r.apply_penalty or o.penalize_prompt))) for o, r in zip(opts, rows)]
+        plain_penalty = [o is None and self.mask is not None and r.apply_penalty for o, r in zip(opts, rows)]
+        if self.counts is None and any(o is not None and o.penalizes for o in opts):
+            raise ValueError("a row asks for penalties of its own, but its seat was not reset with its options")
+        words = (vocab + 31) // 32
+        grammars, grammar_of = [], []
+        for r in rows:
+            packed = pack_allowed(r.allowed, vocab) if isinstance(r, OptionRow) else None
+            grammar_of.append(len(grammars) if packed is not None else -1)
+            if packed is not None:
+                grammars.append(packed)
+        biases = [sorted((o.logit_bias or {}).items()) if o is not None else [] for o in opts]
+        total_biases = sum(map(len, biases))
+        # one upload: ten numbers a row, the biases, the grammars
+        size = 11 * n + (n + 1) + 2 * total_biases + len(grammars) * words
+        # (a block of torch's pinned memory is not handed out again before the copy has left it)
+        staging = torch.empty(size, dtype=torch.int32, pin_memory=True)
+        i32 = staging.numpy()
+        u32, f32 = i32.view(np.uint32), i32.view(np.float32)
+        at = 0
+
+        def put(view, values):
+            nonlocal at
+            view[at:at + len(values)] = values
+            at += len(values)
+            return slice(at - len(values), at)
+
+        inverse = [1.0 / r.temperature if r.temperature > 0 else 0.0 for r in rows]
+        s_plain_t = put(f32, [0.0 if c else t for c, t in zip(cut, inverse)])
+        s_cut_t = put(f32, [t if c else math.nan for c, t in zip(cut, inverse)])
+        s_key = put(u32, [int(r.rng_key) & 0xFFFFFFFF for r in rows])
+        s_step = put(u32, [int(r.rng_step) & 0xFFFFFFFF for r in rows])
+        s_own = put(i32, [r.seat if w else -1 for r, w in zip(rows, own)])
+        s_plain = put(i32, [r.seat if w else -1 for r, w in zip(rows, plain_penalty)])
+        s_mark = put(i32, [r.seat for r in rows])
+        s_grammar = put(i32, grammar_of)
+        s_k = put(i32, [min(o.top_k, vocab) if o is not None else 0 for o in opts])
+        s_p = put(f32, [o.top_p if o is not None else 1.0 for o in opts])
+        s_m = put(f32, [o.min_p if o is not None else 0.0 for o in opts])
+        s_start = put(i32, np.cumsum([0] + [len(b) for b in biases]))
+        s_token = put(i32, [min(int(t), vocab) for b in biases for t, _ in b])
+        s_value = put(f32, [v for b in biases for _, v in b])
+        s_words = put(i32, np.concatenate(grammars) if grammars else [])
+        penalties = any(own)
+        if penalties:
+            extra = torch.empty((3, n), dtype=torch.float32, pin_memory=True)
+            extra.numpy()[0] = [(o.repetition_penalty if o.repetition_penalty is not None else self.penalty) if w else 1.0 for o, w in zip(opts, own)]
+            extra.numpy()[1] = [o.presence_penalty if w else 0.0 for o, w in zip(opts, own)]
+            extra.numpy()[2] = [o.frequency_penalty if w else 0.0 for o, w in zip(opts, own)]
+            extra = extra.to(self.device, non_blocking=True)
+        dev = staging.to(self.device, non_blocking=True)
+        real = dev.view(torch.float32)
+        if penalties or total_biases or grammars:
+            adjusted = torch.empty((n, vocab), dtype=torch.float32, device=self.device)
+            kw = {}
+            if penalties:
+                kw.update(row_seat=dev[s_own], marks=self.marks, repetition=extra[0])
+                if self.counts is not None:
+                    kw.update(counts=self.counts, presence=extra[1], frequency=extra[2])
+            if total_biases:
+                kw.update(bias=(dev[s_start], dev[s_token], real[s_value]))
+            if grammars:
+                kw.update(allowed=dev[s_words].view(len(grammars), words), allowed_row=dev[s_grammar])
+            logits = K.adjust_logits(logits, adjusted, **kw)
+        if not all(cut):
+            # (a row with a cut takes its best token here, and another below)
+            penalised = any(plain_penalty)
+            K.sample(logits, out, chunks=self.chunks, inv_temperature=real[s_plain_t], seed=self.seed, rng_key=dev[s_key], rng_step=dev[s_step],
+                     penalty_mask=self.mask if penalised else None, row_seat=dev[s_plain] if penalised else None, penalty=self.penalty,
+                     host_tokens=landing)
+        if any(cut):
+            K.sample_truncated(logits, out, inv_temperature=real[s_cut_t], top_k=dev[s_k], top_p=real[s_p], min_p=real[s_m], seed=self.seed,
+                               rng_key=dev[s_key], rng_step=dev[s_step], host_tokens=landing)
+        if self.marks is not None:
+            K.count_tokens(self.marks, self.counts, dev[s_mark], out)

@@ -1,0 +1,256 @@
+"""Options of requests through the sampler and the serving loop, against the plain model and the plain forms of what they ask for."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_llama as plain
+import plain_step_ends as ends
+from kv_cache_optimization_for_llm_amd.cache.manager import CacheManager
+from kv_cache_optimization_for_llm_amd.engine.batch import build_batch
+from kv_cache_optimization_for_llm_amd.engine.engine import EngineOptions
+from kv_cache_optimization_for_llm_amd.engine.runner import LLM, Runner, ServeOptions
+from kv_cache_optimization_for_llm_amd.parts.base import attention_cache_spec
+from kv_cache_optimization_for_llm_amd.sampling.options import SampleOptions, pack_allowed
+from kv_cache_optimization_for_llm_amd.sampling.sampler import OptionRow, Sampler, SampleRow, counter_uniform
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- the sampler
+@pytest.mark.parametrize("vocab, rows, penalty", [(301, 5, 1.0), (5003, 40, 1.3), (50021, 9, 1.0), (1000, 140, 1.15)])
+def test_rows_with_options_beside_rows_without(vocab, rows, penalty, gpu):
+    rng = np.random.default_rng(vocab)
+    pick = [None, SampleOptions(top_k=7), SampleOptions(top_p=0.8, min_p=0.01), SampleOptions(presence_penalty=0.7, frequency_penalty=0.3),
+            SampleOptions(top_k=40, top_p=0.95, repetition_penalty=1.4, penalize_prompt=True),
+            SampleOptions(logit_bias={int(t): float(b) for t, b in zip(rng.permutation(vocab)[:9], rng.standard_normal(9) * 4)}),
+            SampleOptions(top_p=0.9, frequency_penalty=-0.2), SampleOptions(penalize_prompt=True), SampleOptions(min_p=0.2)]
+    opts = [pick[i % len(pick)] for i in range(rows)]
+    ours, alone = (Sampler(vocab, rows + 1, gpu, seed=5, repetition_penalty=penalty) for _ in range(2))
+    prompts = [rng.integers(0, vocab, 20).tolist() for _ in range(rows)]
+    said = [rng.integers(0, vocab, rng.integers(0, 30)).tolist() for _ in range(rows)]
+    for i in range(rows):
+        ours.reset_seat(i, said[i], prompts[i], opts[i])
+        alone.reset_seat(i, said[i])
+    for step in range(4):
+        logits = torch.from_numpy((rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)).to(gpu)
+        t = [0.0 if i % 5 == 4 else 0.6 + 0.1 * (i % 7) for i in range(rows)]
+        free = [rng.random(vocab) < 0.3 if o is not None and i % 3 == 1 else None for i, o in enumerate(opts)]
+        made = []
+        for i, o in enumerate(opts):
+            args = (i, t[i], 8 * i, 100 + step, len(said[i]) > 0)
+            made.append(SampleRow(*args) if o is None else OptionRow(*args, options=o, allowed=free[i]))
+        before = logits.clone()
+        got = ours.sample(logits, made)
+        assert torch.equal(logits, before)
+        base = alone.sample(logits, [SampleRow(i, t[i], 8 * i, 100 + step, len(said[i]) > 0) for i in range(rows)])
+        for i, o in enumerate(opts):
+            if o is None:
+                assert got[i] == base[i]            # a neighbour's options change nothing
+                continue
+            marks, counts = np.zeros((1, vocab), np.uint8), np.zeros((1, vocab), np.int32)
+            own = o.penalizes or (penalty != 1.0 and (len(said[i]) > 0 or o.penalize_prompt))
+            for x in said[i]:
+                marks[0, x] = 1
+                counts[0, x] += 1
+            if o.penalize_prompt:
+                marks[0, prompts[i]] = 1
+            bias = None
+            if o.logit_bias:
+                ids = sorted(o.logit_bias)
+                bias = (np.asarray([0, len(ids)]), np.asarray(ids), np.asarray([o.logit_bias[x] for x in ids]))
+            kw = {}
+            if own:
+                kw.update(marks=marks, counts=counts, row_seat=[0], repetition=[o.repetition_penalty or penalty], presence=[o.presence_penalty],
+                          frequency=[o.frequency_penalty])
+            if free[i] is not None:
+                kw.update(allowed=pack_allowed(free[i], vocab)[None].astype(np.int64), allowed_row=[0])
+            x, _ = ends.adjust(logits[i:i + 1].cpu().numpy(), bias=bias, **kw)
+            u = counter_uniform(5, 8 * i, 100 + step)
+            if t[i] > 0 and o.truncates:
+                want = ends.truncated(x[0], np.float32(1 / t[i]), o.top_k, np.float32(o.top_p), np.float32(o.min_p), u)[0]
+            else:
+                want = ends.truncated(x[0], np.float32(1 / t[i]) if t[i] > 0 else 0.0, u=u)[0]
+            assert got[i] == want, (i, o)
+        for i in range(rows):
+            said[i].append(int(got[i]))
+        for i, o in enumerate(opts):        # the other sampler goes on from the same tokens
+            alone.reset_seat(i, said[i])
+
+
+def test_penalties_need_a_seat_that_knows_them(gpu):
+    s = Sampler(100, 2, gpu)
+    row = OptionRow(0, 0.0, 0, 1, False, options=SampleOptions(presence_penalty=1.0))
+    with pytest.raises(ValueError):
+        s.sample(torch.zeros(1, 100, device=gpu), [row])
+    s.reset_seat(0, [3, 3], [], row.options)
+    assert s.counts[0, 3].item() == 2 and s.sample(torch.zeros(1, 100, device=gpu), [row])[0] == 0
+    with pytest.raises(ValueError):
+        s.sample(torch.zeros(1, 100, device=gpu), [OptionRow(0, 0.0, 0, 1, False, allowed=[100])])
+    # nothing allowed: no token, told as such
+    assert s.sample(torch.zeros(1, 100, device=gpu), [OptionRow(0, 0.0, 0, 1, False, allowed=[])])[0] == -1
+
+
+# ---------------------------------------------------------------- generation
+def prompts_for(vocab, sizes, seed):
+    rng = np.random.default_rng(seed)
+    return [[int(t) for t in rng.integers(0, vocab - 4, n)] for n in sizes]
+
+
+def plain_generate(cfg, W, prompt, n, options, temperature, seed, key):
+    """One request by the plain model: logits of the whole sequence, adjusted and drawn in 64 bits."""
+    out = []
+    for _ in range(n):
+        x = plain.logits_all(cfg, W, prompt + out)[-1].numpy().astype(np.float32)
+        vocab = x.shape[0]
+        marks, counts = np.zeros((1, vocab), np.uint8), np.zeros((1, vocab), np.int32)
+        for t in out:
+            marks[0, t] = 1
+            counts[0, t] += 1
+        if options.penalize_prompt:
+            marks[0, prompt] = 1
+        kw = {}
+        if options.penalizes:
+            kw.update(marks=marks, counts=counts, row_seat=[0], repetition=[options.repetition_penalty or 1.0],
+                      presence=[options.presence_penalty], frequency=[options.frequency_penalty])
+        if options.logit_bias:
+            ids = sorted(options.logit_bias)
+            kw.update(bias=(np.asarray([0, len(ids)]), np.asarray(ids), np.asarray([options.logit_bias[i] for i in ids])))
+        if options.grammar is not None:
+            packed = pack_allowed(options.grammar(out), vocab)
+            if packed is not None:
+                kw.update(allowed=packed[None].astype(np.int64), allowed_row=[0])
+        x, _ = ends.adjust(x[None], **kw)
+        u = counter_uniform(seed, key, len(prompt) + len(out))
+        inv_t = np.float32(1 / temperature) if temperature > 0 else 0.0
+        out.append(ends.truncated(x[0], inv_t, options.top_k, np.float32(options.top_p), np.float32(options.min_p), u)[0])
+    return out
+
+
+def counting(out):
+    """A grammar: the n-th token is one of those with n % 5 as the rest by 5."""
+    return np.arange(301) % 5 == len(out) % 5
+
+
+def test_generation_with_options_is_the_plain_models(sharp_model_dirs, gpu):
+    folder = sharp_model_dirs["D"]              # a vocabulary of 301
+    cfg, W = plain.load_model_dir(folder)
+    prompts = prompts_for(301, [9, 23, 40, 5, 17, 12], 3)
+    options = [SampleOptions(top_k=5), SampleOptions(top_p=0.7, presence_penalty=1.5, frequency_penalty=0.4),
+               SampleOptions(grammar=counting, top_k=20), SampleOptions(repetition_penalty=1.5, penalize_prompt=True, min_p=0.05),
+               SampleOptions(logit_bias={3: 4.0, 7: -math.inf, 11: 5.0}, top_p=0.9), SampleOptions(grammar=lambda out: [2, 3, 5, 7, 11])]
+    for temperature in (0.0, 0.9):
+        want = [plain_generate(cfg, W, p, 8, o, temperature, 21, 8 * i) for i, (p, o) in enumerate(zip(prompts, options))]
+        for ahead in (False, True):
+            llm = LLM(folder, EngineOptions(dtype="float32", max_seqs=4, max_seq_len=96), ServeOptions(run_ahead=ahead))
+            got = llm.generate(prompts, max_new_tokens=8, ignore_eos=True, temperature=temperature, seed=21, options=options)
+            assert got == want
+            llm.engine.cache.check()
+
+
+def test_neighbours_without_options_and_the_servers_own(model_dirs, gpu):
+    """Requests without options generate what they generate alone; the server's options are those of requests that bring none."""
+    folder = model_dirs["A"]
+    prompts = prompts_for(256, [8, 30, 14, 21], 5)
+    llm = LLM(folder, EngineOptions(dtype="bfloat16", max_seqs=4, max_seq_len=128), ServeOptions(repetition_penalty=1.2))
+    base = llm.generate(prompts, 20, ignore_eos=True, temperature=0.8, seed=3)
+    some = SampleOptions(top_k=4, presence_penalty=0.5)
+    mixed = llm.generate(prompts, 20, ignore_eos=True, temperature=0.8, seed=3, options=[None, some, None, SampleOptions(grammar=lambda out: [5, 6])])
+    assert mixed[0] == base[0] and mixed[2] == base[2] and set(mixed[3]) <= {5, 6}
+    llm.serve_options.sampling = some
+    own = llm.generate(prompts, 20, ignore_eos=True, temperature=0.8, seed=3)
+    assert own[1] == mixed[1]
+    # top_k = 1 is the best token whatever the temperature
+    llm.serve_options.sampling, llm.serve_options.repetition_penalty = None, 1.0
+    assert llm.generate(prompts, 12, ignore_eos=True, temperature=1.3, options=SampleOptions(top_k=1)) == llm.generate(prompts, 12, ignore_eos=True)
+    with pytest.raises(ValueError):
+        llm.generate(prompts, 4, options=[some])
+    with pytest.raises(ValueError):
+        llm.generate(prompts, 4, options=SampleOptions(logit_bias={256: 1.0}))
+
+
+def test_a_grammar_that_leaves_nothing_ends_the_request(model_dirs, gpu):
+    llm = LLM(model_dirs["A"], EngineOptions(dtype="bfloat16", max_seqs=2, max_seq_len=64))
+    out, reasons = llm.generate(prompts_for(256, [5, 6], 1), 10, ignore_eos=True, return_reasons=True,
+                                options=[SampleOptions(grammar=lambda out: [1, 2] if len(out) < 3 else []), None])
+    assert len(out[0]) == 3 and reasons[0] == "invalid_logits" and len(out[1]) == 10 and reasons[1] == "length"
+    llm.engine.cache.check()
+
+
+def test_preempted_requests_with_options(model_dirs, gpu):
+    prompts = prompts_for(256, [30, 30, 30], 6)
+    options = [SampleOptions(presence_penalty=1.0, frequency_penalty=0.5), SampleOptions(top_p=0.8, repetition_penalty=1.3, penalize_prompt=True),
+               SampleOptions(grammar=lambda out: np.arange(256) % 3 != len(out) % 3, frequency_penalty=0.2)]
+    big = LLM(model_dirs["A"], EngineOptions(dtype="float32", max_seqs=4, max_seq_len=128, cache_tokens=1024))
+    small = LLM(model_dirs["A"], EngineOptions(dtype="float32", max_seqs=4, max_seq_len=128, cache_tokens=11 * 16))
+    for t in (0.0, 0.8):
+        want = big.generate(prompts, 50, ignore_eos=True, temperature=t, seed=5, options=options)
+        got = small.generate(prompts, 50, ignore_eos=True, temperature=t, seed=5, options=options)
+        assert big.last_runner.scheduler.preemptions == 0 and small.last_runner.scheduler.preemptions > 0
+        assert got == want
+
+
+def test_a_grammar_that_raises_is_heard_and_the_request_can_be_cancelled(model_dirs, gpu):
+    llm = LLM(model_dirs["A"], EngineOptions(dtype="bfloat16", max_seqs=2, max_seq_len=64))
+    runner = Runner(llm.engine, ServeOptions(ignore_eos=True))
+
+    def grammar(out):
+        if len(out) == 2:
+            raise RuntimeError("no such state")
+        return None
+    bad = runner.submit([1, 2, 3], 6, options=SampleOptions(grammar=grammar))
+    good = runner.submit([4, 5], 6)
+    events = []
+    with pytest.raises(RuntimeError, match="no such state"):
+        while not runner.idle():
+            events += runner.step()
+    events += runner.cancel(bad)
+    while not runner.idle():
+        events += runner.step()
+    tokens = [e.token for e in events if e.kind == "token" and e.request_id == good]
+    assert tokens == llm.generate([[4, 5]], 6, ignore_eos=True)[0]
+    llm.engine.cache.check()
+
+
+# ---------------------------------------------------------------- the step's arrays
+def test_batches_made_on_the_device_are_the_hosts(gpu):
+    rng = np.random.default_rng(4)
+    specs = [(attention_cache_spec(1, 16), [0]), (attention_cache_spec(1, 16, "window", 40), [1])]
+    m = CacheManager(specs, {}, page_size=16, num_pages=400, max_seqs=70, max_seq_len=512, device=gpu, dtype=torch.bfloat16)
+    live, state = {}, None
+    for turn in range(12):
+        for seat in list(live):
+            if rng.random() < 0.3:
+                m.free(seat)
+                del live[seat]
+        while m.free_seats and (len(live) < 3 or rng.random() < 0.8):
+            seat = m.admit(object())
+            live[seat] = 0
+        seats = [int(s) for s in rng.permutation(sorted(live))[:rng.integers(1, len(live) + 1)]]
+        lens = [int(rng.integers(1, 40)) if rng.random() < 0.5 else 1 for _ in seats]
+        lens = [min(n, 512 - live[s]) for n, s in zip(lens, seats)]
+        keep = [i for i, (n, s) in enumerate(zip(lens, seats)) if n > 0 and m.grow(s, live[s] + n)]
+        seats, lens = [seats[i] for i in keep], [lens[i] for i in keep]
+        starts = [live[s] for s in seats]
+        if not seats:
+            continue
+        toks = [rng.integers(0, 99, n).tolist() for n in lens]
+        wants = [[n - 1] for n in lens]
+        for g in (0, 1):
+            for s, a, n in zip(seats, starts, lens):
+                m.check_mapped(s, a, n, g)
+        maps = [[m.slot_mapping(s, a, n, g) for s, a, n in zip(seats, starts, lens)] for g in (0, 1)]
+        m.flush_tables()
+        for g in m.groups:              # spans of many seats at once, of one, and freed ones
+            assert np.array_equal(g.table_dev.cpu().numpy(), g.table_host)
+        host = build_batch(seats, starts, toks, wants, maps, gpu)
+        made = build_batch(seats, starts, toks, wants, None, gpu, [g.table_dev for g in m.groups], 16)
+        for name in ("token_ids", "positions", "tok_seat", "logit_rows", "entry_seat", "entry_q_start", "entry_start_pos"):
+            assert torch.equal(getattr(host, name), getattr(made, name)), name
+        assert all(torch.equal(a, b) for a, b in zip(host.slot_mapping, made.slot_mapping))
+        assert (host.num_tokens, host.max_context, host.logits_for_all_rows) == (made.num_tokens, made.max_context, made.logits_for_all_rows)
+        for s, a, n in zip(seats, starts, lens):
+            live[s] = a + n
+            m.commit(s, a + n)
+        m.check()
