@@ -17,7 +17,7 @@
 //
 // Vocabularies of up to 262,144 take four launches, the first three of them with many workgroups a row, each of some steps of
 // 1,024 tokens:
-//   1. trunc_best_kernel     the best place of every workgroup's tokens; for a small k also of groups of some 32 to 512
+//   1. trunc_best_kernel     the best place of every workgroup's tokens; for a small k also of groups of 32 to 512
 //   2. trunc_bins_kernel     bins by the distance from the best, 1/32 of a factor of two wide: how many tokens a bin has where
 //                            the row asks for k, their weight where it asks for p alone
 //   3. trunc_collect_kernel  finds the bin in which the cut lies and leaves a list of tokens: where k is asked for those of all bins up to
@@ -25,9 +25,14 @@
 //   4. trunc_pick_kernel     a workgroup a row: for a small k its list from the groups that can hold the k best (such rows pass 2 and 3 by);
 //                            the cuts among the list's tokens, what stays by 256 ids, then the token among 256
 // A list has room for 4,096 tokens.  A row with more in the bin of its cut (nearly equal logits), or with a larger k among
-// them, is taken by the last kernel alone, as rows of larger vocabularies are by sample_truncated_kernel: a cut is found by counting, the places still in
-// question are cut into 1,024 ranges, their numbers and weights added up in LDS, and the range in which the sum passes what is
-// sought is the next turn's; the row is read again in every turn.
+// them, is taken by the last kernel alone, as rows of larger vocabularies are by sample_truncated_kernel: a cut is found by counting,
+// the places still in question are cut into 1,024 ranges, their numbers and weights added up in LDS, and the range in which the sum passes what is
+// sought is the next turn's; the row is read again in every turn (out of LDS up to 16,384 tokens).
+//
+// us in a graph.  Vocabulary 128,256: 1 row of a p 21, of a k 17; 64 rows of p 0.9 49 (7.2 + 18 + 17 + 9.2 for the four kernels), of a k up to 50 25 (7.7 + 2.0 + 2.0 +
+// 14.8: 33 MB are 6.4 us at a copy's rate); 256 rows of p 0.98 at a temperature of 2, which keep most of the vocabulary, 117 (21 + 33 + 59 + 11: the
+// first reads 131 MB at 6.2 TB/s, the next two weigh every token); rows of nearly equal logits 410 to 480.  One launch, against four: 1,024 tokens 10 / 16
+// to 25, 2,048 13 to 15 / 17 to 22, 4,096 16 to 21 / 17 to 29, 8,192 28 to 31 / 18 to 25.
 #include "common.h"
 #include "counter_uniform.h"
 #include "wave_scan.h"
@@ -84,9 +89,9 @@ __device__ inline void tr_load4(const float *rl, int t, int vocab, float (&l)[4]
 // How a row weighs its logits.  With x = 128 (s - (best - l) / (T ln 2)) and m its nearest whole number, W = 2^(m / 128) 2^((x - m) / 128):
 // the first from a table of 2^(j / 128) and an exponent, the second, 1 + q with |q| < 0.0028, by three terms of its series (2e-12 off).
 // A number below 2^51 and 1.5 2^52 (2^52) add up to one whose last bits are the number's whole part, rounded.  A logit that weighs
-// less than 1/8, and one that is none, has the x of 1/8 and the weight 0.  What bounds the kernels that weigh a whole row is the number of
-// instructions: 64-bit ones take as long as others, and these are eleven; a polynomial of ten terms without a table took 58 us where
-// this takes 30 (256 rows' bins).
+// less than 1/8, and one that is none, has the x of 1/8 and the weight 0.  What bounds the kernels that weigh a whole row is the
+// number of instructions, 64-bit ones above all (some ten cycles each): a polynomial of eleven terms and an exponent instead of the table, 256 rows of
+// 128,256: bins 38 us instead of 33, sums 63 instead of 59.
 #define TR_TABLE 128
 struct TruncWeights {
     double best, rate;                  // 128 / (T ln 2)
@@ -137,7 +142,7 @@ __device__ inline u64 tr_wave_max(u64 v) {
     return wave_last(wave_scan(v, 0ull, [](u64 a, u64 b) { return a > b ? a : b; }));
 }
 
-#define TR_PAIRS 128                    // so many tokens are compared with one another
+#define TR_PAIRS 64                     // so many tokens are compared with one another
 
 struct TruncShared {
     u64 sum[TR_DIGITS];
@@ -194,8 +199,8 @@ __device__ inline FourSums tr_four(TruncShared &s, const u64 *sum, const unsigne
     return r;
 }
 
-// Up to 128 tokens, their places in s.place: how many of them and what weight (beside `front`) lies up to each of them, itself
-// included.  Four threads a token, or two of more than 64, which all get it.
+// Up to 64 tokens, their places in s.place: how many of them and what weight (beside `front`) lies up to each of them, itself
+// included.  Four threads a token, which all get it.
 struct PairSums {
     bool on;
     u64 place, own, upto;
@@ -203,17 +208,18 @@ struct PairSums {
 };
 template <typename WEIGHT>
 __device__ inline PairSums tr_pairs(TruncShared &s, int n, u64 front, WEIGHT weight) {
-    const int tid = threadIdx.x, share = n <= TR_THREADS / 4 ? 4 : 2, j = tid / share;
+    const int tid = threadIdx.x, j = tid / 4;
     if (tid < n) s.weight[tid] = weight(s.place[tid]);
     __syncthreads();
     PairSums r{j < n, j < n ? s.place[j] : 0, j < n ? s.weight[j] : 0, 0, 0};
 #pragma unroll 4
-    for (int i = tid % share; i < n; i += share) {
+    for (int i = tid % 4; i < n; i += 4) {
         const bool in = s.place[i] <= r.place;
         r.upto += in ? s.weight[i] : 0;
         r.rank += in ? 1 : 0;
     }
-    for (int off = 1; off < share; off <<= 1) {
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
         r.upto += __shfl_xor(r.upto, off, KVA_WAVE);
         r.rank += __shfl_xor(r.rank, off, KVA_WAVE);
     }
@@ -495,7 +501,8 @@ sample_truncated_kernel(TruncArgs a) {
 #define TR_SPLIT_WAVES (TR_SPLIT_THREADS / KVA_WAVE)
 #define TR_WAVE_LIST 1024
 #define TR_MAX_PARTS 64
-#define TR_FEW_MOST 256
+#define TR_FEW_MOST 512
+#define TR_FEW_STEPS 2048
 #define TR_GROUPS 64                    // groups a part
 #define TR_MAX_VOCAB (TR_BUCKET * TR_BUCKETS)
 
@@ -506,17 +513,22 @@ struct TruncSpace {                     // of all rows
     u64 *sought;                        // [2]: the weight in front of the cut's bin, and the one the cut has to reach
     u64 *sums;                          // [buckets]: what stays for certain, by ids
     unsigned *counts;                   // [buckets]
-    int *list;                          // [TR_LIST]
+    u64 *list;                          // [TR_LIST]: places
     int *listed;                        // [1]: tokens that asked for a place in the list
     int parts, part_tokens, buckets;
 };
 
-// What a row's cut is found by: nothing, the number of tokens up to a bin, their weight, or the best tokens of the groups (a k of up to
-// half as many as there are of those: 64 rows of 128,256 and k up to 50, us: 22 instead of 37).
+// What a row's cut is found by: nothing, the number of tokens up to a bin, their weight, or the best tokens of the groups.  The last is for a
+// small k, as long as one workgroup reads the k groups it leaves sooner than many read the row twice more: by the steps a group
+// has, up to 4,096 of all of them, or 2,048 from k = 257 on (and k at most half of the groups).  us by groups / by bins, all rows of a launch: 64 rows of
+// 128,256 and k up to 100 (8 steps a group) 29 / 44, up to 250 40 / 60, 256 rows and k up to 100 (32 steps) 59 / 84; 64 rows and k up to 2,000, those
+// up to 512 by groups 93, up to 256 80, up to 64 71 (a launch with both kinds pays for both); 37 rows of 50,021 and k up to 400 (2 steps) 31 / 41.
 enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2, TR_FEW = 3 };
 __device__ inline int tr_mode(const TruncArgs &a, const TruncSpace &sp, int row) {
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    if (k > 0 && k < a.vocab) return k <= min(TR_FEW_MOST, sp.parts * TR_GROUPS / 2) ? TR_FEW : TR_COUNT;
+    if (k > 0 && k < a.vocab) return k <= min(TR_FEW_MOST, sp.parts * TR_GROUPS / 2) &&
+                                               k * (sp.part_tokens / TR_STEP) <= (k <= TR_FEW_MOST / 2 ? 2 * TR_FEW_STEPS : TR_FEW_STEPS)
+                                           ? TR_FEW : TR_COUNT;
     return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
 }
 
@@ -755,7 +767,10 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
         int base = 0;
         if (lane == 0) base = atomicAdd(&sp.listed[row], listed > TR_WAVE_LIST ? TR_LIST + 1 : listed);
         base = __builtin_amdgcn_readfirstlane(base);
-        for (int i = lane; i < min(n, TR_LIST - base); i += KVA_WAVE) sp.list[(size_t)row * TR_LIST + base + i] = found[wave][i];
+        for (int i = lane; i < min(n, TR_LIST - base); i += KVA_WAVE) {
+            const int id = found[wave][i];
+            sp.list[(size_t)row * TR_LIST + base + i] = tr_place(rl[id], id);
+        }
     }
     if (mode == TR_COUNT) return;
     __syncthreads();
@@ -766,8 +781,8 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     }
 }
 
-// grid (rows).  Four wavefronts, one a SIMD: with sixteen the same steps took twice as long (64 rows 15 us), each waits for three others'
-// instructions.
+// grid (rows).  A chain of short steps with a barrier between them; four wavefronts, one a SIMD, so that a step of all lanes (a prefix
+// sum over 1,024 numbers, say) costs its instructions once.
 __global__ void __launch_bounds__(TR_THREADS)
 trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     constexpr int TOPS = TR_MAX_PARTS * TR_GROUPS / TR_THREADS;
@@ -784,7 +799,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     const bool drawn = inv_t > 0.f, sums = drawn && (mode == TR_ALL || mode == TR_WEIGHT);
     const u64 front = mode == TR_WEIGHT && drawn ? sp.sought[2 * row] : 0, sought = mode == TR_WEIGHT && drawn ? sp.sought[2 * row + 1] : 0;
     int n = drawn ? sp.listed[row] : 0;
-    const int id0 = sp.list[(size_t)row * TR_LIST + tid];
+    const u64 *list = sp.list + (size_t)row * TR_LIST, place0 = list[tid];
     u64 tops[TOPS];
     if (mode == TR_FEW) {
 #pragma unroll
@@ -846,7 +861,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         __syncthreads();
         // four threads a group and step: its 16 tokens
         const int steps = sp.part_tokens / TR_STEP, in = groups_in * steps;
-        constexpr int AHEAD = 8;            // loads on their way
+        constexpr int AHEAD = 4;            // loads on their way
         for (int j0 = tid / 4; j0 < in; j0 += AHEAD * TR_THREADS / 4) {
             float l[AHEAD][4];
             int t[AHEAD];
@@ -875,13 +890,12 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         trunc_whole_row(a, s, rl, row);
         return;
     }
-    if (mode != TR_FEW)
-        for (int i = tid; i < n; i += TR_THREADS) {
-            const int id = i == tid ? id0 : sp.list[(size_t)row * TR_LIST + i];
-            const u64 at = tr_place(rl[id], id);
-            place[i] = at;
-            if (i < TR_PAIRS) s.place[i] = at;
-        }
+    if (mode != TR_FEW) {
+        if (tid < n) place[tid] = place0;
+        if (tid < min(n, TR_PAIRS)) s.place[tid] = place0;
+#pragma unroll 4
+        for (int i = tid + TR_THREADS; i < n; i += TR_THREADS) place[i] = list[i];
+    }
     __syncthreads();
     if (mode != TR_ALL) {
         const u64 need = mode == TR_WEIGHT ? sought : (u64)min(k, (unsigned)n);
@@ -933,7 +947,7 @@ extern "C" long long kva_sample_truncated_workspace_bytes(int rows, int vocab) {
     if (rows <= 0 || !trunc_split(vocab)) return 0;
     int part_tokens;
     const long long parts = trunc_parts(rows, vocab, &part_tokens), buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
-    return rows * (8 * (parts + TR_BINS + parts * TR_GROUPS + buckets) + 4 * (buckets + TR_LIST + 1) + 16);
+    return rows * (8 * (parts + TR_BINS + parts * TR_GROUPS + 2 + TR_LIST + buckets) + 4 * (buckets + 1));
 }
 
 extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long stride, int rows, int vocab, const float *inv_t,
@@ -972,9 +986,9 @@ extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long 
     sp.tops = sp.bins + (size_t)rows * TR_BINS;
     sp.sought = sp.tops + (size_t)rows * sp.parts * TR_GROUPS;
     sp.sums = sp.sought + (size_t)rows * 2;
-    sp.counts = (unsigned *)(sp.sums + (size_t)rows * sp.buckets);
-    sp.list = (int *)(sp.counts + (size_t)rows * sp.buckets);
-    sp.listed = sp.list + (size_t)rows * TR_LIST;
+    sp.list = sp.sums + (size_t)rows * sp.buckets;
+    sp.counts = (unsigned *)(sp.list + (size_t)rows * TR_LIST);
+    sp.listed = (int *)(sp.counts + (size_t)rows * sp.buckets);
     const dim3 grid(sp.parts, rows), block(TR_SPLIT_THREADS);
     hipLaunchKernelGGL(trunc_best_kernel, grid, block, 0, stream, a, sp);
     hipLaunchKernelGGL(trunc_bins_kernel, grid, block, 0, stream, a, sp);

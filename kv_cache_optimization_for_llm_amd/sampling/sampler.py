@@ -244,7 +244,7 @@ class Sampler:
             event.record()
             return PendingTokens(host, event, 0)
         landing = host if self._kernel_writes_host else None
-        if OptionRow in set(map(type, rows)):
+        if any(issubclass(kind, OptionRow) for kind in set(map(type, rows))):
             try:
                 self._sample_options(logits, rows, out, landing)
                 if landing is None:
