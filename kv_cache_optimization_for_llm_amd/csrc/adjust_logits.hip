@@ -176,18 +176,27 @@ adjust_logits_kernel(AdjustArgs a) {
     }
 }
 
-extern "C" int kva_adjust_logits(float *out, long long out_stride, const void *logits, int dtype, long long in_stride, int rows, int vocab,
-                                 const int *row_seat, int seats, const unsigned char *marks, const int *counts, const float *repetition,
-                                 const float *presence, const float *frequency, const int *bias_start, const int *bias_token,
-                                 const float *bias_value, int biases, const int *allowed_row, const int *allowed, int grammars,
-                                 hipStream_t stream) {
+// address [11], the host's: of row_seat, marks, counts, repetition, presence, frequency, the biases' starts, tokens and values, allowed_row
+// and allowed (0: absent)
+extern "C" int kva_adjust_logits(const long long *address, float *out, long long out_stride, const void *logits, int dtype, long long in_stride,
+                                 int rows, int vocab, int seats, int biases, int grammars, hipStream_t stream) {
+    const int *row_seat = (const int *)address[0], *counts = (const int *)address[2], *bias_start = (const int *)address[6],
+              *bias_token = (const int *)address[7], *allowed_row = (const int *)address[9];
+    const unsigned char *marks = (const unsigned char *)address[1];
+    const float *repetition = (const float *)address[3], *presence = (const float *)address[4], *frequency = (const float *)address[5],
+                *bias_value = (const float *)address[8];
+    const unsigned *allowed = (const unsigned *)address[10];
     KVA_REQUIRE(dtype == KVA_F32 || dtype == KVA_BF16, "adjust_logits: dtype %d", dtype);
     KVA_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab < 1 << 30, "adjust_logits: bad sizes rows=%d vocab=%d", rows, vocab);
     KVA_REQUIRE(row_seat == nullptr || (marks != nullptr && seats > 0), "adjust_logits: seats without marks");
     KVA_REQUIRE(allowed_row == nullptr || (allowed != nullptr && grammars > 0), "adjust_logits: grammars are missing");
+    KVA_REQUIRE(marks != nullptr || (counts == nullptr && repetition == nullptr), "adjust_logits: counts and repetition need marks");
     if (rows == 0) return KVA_OK;
+    KVA_REQUIRE((marks == nullptr) == (row_seat == nullptr) && (allowed == nullptr) == (allowed_row == nullptr),
+                "adjust_logits: marks and seats, grammars and the rows' numbers of them go together");
+    KVA_REQUIRE(biases == 0 || (bias_start != nullptr && bias_token != nullptr && bias_value != nullptr), "adjust_logits: a part of the biases is missing");
     const AdjustArgs a{logits, out, in_stride, out_stride, vocab, row_seat, seats, marks, counts, repetition, presence, frequency, bias_start,
-                       bias_token, bias_value, biases, allowed_row, (const unsigned *)allowed, grammars, (vocab + 31) / 32};
+                       bias_token, bias_value, biases, allowed_row, allowed, grammars, (vocab + 31) / 32};
     const int tile = AL_UNITS * 4 * AL_THREADS;
     const long long touched = (long long)rows * vocab * ((dtype == KVA_F32 ? 4 : 2) + 4 + (row_seat != nullptr ? 1 : 0));
     const bool streamed = touched > 256ll << 20;
@@ -216,6 +225,7 @@ extern "C" int kva_count_tokens(unsigned char *marks, int *counts, int seats, in
                                 hipStream_t stream) {
     KVA_REQUIRE(n >= 0 && seats > 0 && vocab > 0, "count_tokens: bad sizes");
     if (n == 0) return KVA_OK;
+    KVA_REQUIRE(marks != nullptr && of != nullptr && tokens != nullptr, "count_tokens: marks, seats and tokens are needed");
     hipLaunchKernelGGL(count_tokens_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, marks, counts, seats, vocab, of, tokens, n);
     KVA_CHECK_LAUNCH("count_tokens");
     return KVA_OK;

@@ -950,10 +950,15 @@ extern "C" long long kva_sample_truncated_workspace_bytes(int rows, int vocab) {
     return rows * (8 * (parts + TR_BINS + parts * TR_GROUPS + 2 + TR_LIST + buckets) + 4 * (buckets + 1));
 }
 
-extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long stride, int rows, int vocab, const float *inv_t,
-                                    const int *top_k, const float *top_p, const float *min_p, const float *uniform, unsigned seed,
-                                    const unsigned *key, const unsigned *step, int *kept, float *logprob, int *host_tokens,
-                                    void *workspace, hipStream_t stream) {
+// address [10], the host's: of the tokens, inverse temperatures, top_k, top_p, min_p, uniform numbers, keys, steps, kept and logprob (0: absent)
+extern "C" int kva_sample_truncated(const long long *address, const float *logits, long long stride, int rows, int vocab, unsigned seed,
+                                    int *host_tokens, void *workspace, hipStream_t stream) {
+    int *tokens = (int *)address[0], *kept = (int *)address[8];
+    const int *top_k = (const int *)address[2];
+    const unsigned *key = (const unsigned *)address[6], *step = (const unsigned *)address[7];
+    const float *inv_t = (const float *)address[1], *top_p = (const float *)address[3], *min_p = (const float *)address[4],
+                *uniform = (const float *)address[5];
+    float *logprob = (float *)address[9];
     int *host_mapped = nullptr;
     if (host_tokens != nullptr) {
         void *dev = nullptr;
@@ -964,7 +969,7 @@ extern "C" int kva_sample_truncated(int *tokens, const float *logits, long long 
         host_mapped = (int *)dev;
     }
     KVA_REQUIRE(rows >= 0 && rows <= 65535 && vocab > 0 && vocab <= 1 << 24, "sample_truncated: bad sizes rows=%d vocab=%d", rows, vocab);
-    KVA_REQUIRE(inv_t != nullptr || rows == 0, "sample_truncated: a temperature per row is needed");
+    KVA_REQUIRE((inv_t != nullptr && tokens != nullptr) || rows == 0, "sample_truncated: a temperature and a place for a token per row are needed");
     KVA_REQUIRE(uniform != nullptr || (key != nullptr && step != nullptr) || rows == 0, "sample_truncated: random numbers or keys and steps are needed");
     if (rows == 0) return KVA_OK;
     int log_vocab = 0;

@@ -68,12 +68,16 @@ grow_tables_kernel(GrowArgs a) {
     }
 }
 
-extern "C" int kva_grow_tables(int *table, int rows, int blocks, const int *seats, const int *held, const int *lengths, int entries,
-                               int page_size, const int *pages, int num_pages, int *offsets, hipStream_t stream) {
+// address [6], the host's: of the table, seats, held, lengths, pages and offsets
+extern "C" int kva_grow_tables(const long long *address, int rows, int blocks, int entries, int page_size, int num_pages, hipStream_t stream) {
+    int *table = (int *)address[0], *offsets = (int *)address[5];
+    const int *seats = (const int *)address[1], *held = (const int *)address[2], *lengths = (const int *)address[3], *pages = (const int *)address[4];
     KVA_REQUIRE(entries >= 0 && entries <= ST_MAX_ENTRIES, "grow_tables: %d requests are not in 0..%d", entries, ST_MAX_ENTRIES);
     KVA_REQUIRE(rows > 0 && blocks > 0 && page_size > 0 && num_pages >= 0, "grow_tables: bad sizes rows=%d blocks=%d page_size=%d pages=%d", rows,
                 blocks, page_size, num_pages);
     if (entries == 0) return KVA_OK;
+    KVA_REQUIRE(table != nullptr && seats != nullptr && held != nullptr && lengths != nullptr && offsets != nullptr && (pages != nullptr || num_pages == 0),
+                "grow_tables: a seat, held blocks and a length per request, and a row of pages are needed");
     hipLaunchKernelGGL(grow_tables_kernel, dim3(entries), dim3(ST_THREADS), 0, stream,
                        GrowArgs{table, seats, held, lengths, pages, offsets, entries, rows, blocks, page_size, num_pages});
     KVA_CHECK_LAUNCH("grow_tables");
@@ -201,20 +205,26 @@ step_rows_kernel(RowsArgs a) {
     }
 }
 
-// group [groups][4], the host's: a table's address, its rows and blocks, and the address of the group's slots
-extern "C" int kva_step_rows(const int *lengths, const int *starts, const int *seats, int entries, const long long *group, int groups,
-                             int page_size, int tokens, int *q_start, int *positions, int *tok_seat, hipStream_t stream) {
+// address [6 + 2 groups], the host's: of lengths, starts, seats, q_start, positions and tok_seat, then of a group's table and slots each; size
+// [groups][2], the host's: a table's rows and blocks
+extern "C" int kva_step_rows(const long long *address, const long long *size, int entries, int groups, int page_size, int tokens, hipStream_t stream) {
     KVA_REQUIRE(entries >= 0 && entries <= ST_MAX_ENTRIES, "step_rows: %d entries are not in 0..%d", entries, ST_MAX_ENTRIES);
     KVA_REQUIRE(groups >= 0 && groups <= ST_MAX_GROUPS, "step_rows: %d groups are not in 0..%d", groups, ST_MAX_GROUPS);
     KVA_REQUIRE(tokens >= 0 && page_size > 0, "step_rows: bad sizes tokens=%d page_size=%d", tokens, page_size);
     const int shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
-    RowsArgs a{lengths, starts, seats, q_start, positions, tok_seat, entries, tokens, page_size, shift, groups, {}, {}, {}, {}};
-    for (int g = 0; g < groups; ++g, group += 4) {
-        KVA_REQUIRE(group[1] > 0 && group[2] > 0 && group[1] <= INT_MAX && group[2] <= INT_MAX, "step_rows: table %d is %lld x %lld", g, group[1], group[2]);
-        a.table[g] = (const int *)group[0];
-        a.rows[g] = (int)group[1];
-        a.blocks[g] = (int)group[2];
-        a.slots[g] = (int *)group[3];
+    RowsArgs a{(const int *)address[0], (const int *)address[1], (const int *)address[2], (int *)address[3], (int *)address[4], (int *)address[5],
+               entries, tokens, page_size, shift, groups, {}, {}, {}, {}};
+    KVA_REQUIRE(a.q_start != nullptr && (entries == 0 || (a.lengths != nullptr && a.starts != nullptr && a.seats != nullptr)) &&
+                    (tokens == 0 || (a.positions != nullptr && a.tok_seat != nullptr)),
+                "step_rows: a length, a start and a seat per entry, and places for what is made of them are needed");
+    for (int g = 0; g < groups; ++g) {
+        const long long rows = size[2 * g], blocks = size[2 * g + 1];
+        KVA_REQUIRE(rows > 0 && blocks > 0 && rows <= INT_MAX && blocks <= INT_MAX, "step_rows: table %d is %lld x %lld", g, rows, blocks);
+        a.table[g] = (const int *)address[6 + 2 * g];
+        a.slots[g] = (int *)address[7 + 2 * g];
+        KVA_REQUIRE(a.table[g] != nullptr && (tokens == 0 || a.slots[g] != nullptr), "step_rows: table %d or its slots are missing", g);
+        a.rows[g] = (int)rows;
+        a.blocks[g] = (int)blocks;
     }
     const int grid = max(1, (int)(((long long)tokens + 4 * ST_THREADS - 1) / (4 * ST_THREADS)));
     const bool staged = entries <= ST_STAGED, few = groups <= 2;

@@ -3,6 +3,8 @@
 ``libkva_hip.so``  - every ``csrc/*.hip`` file, compiled with hipcc for gfx950.
 ``libkva_host.<interpreter>.so`` - ``csrc/host/*.cpp``, C++ without a GPU runtime; one function takes Python objects,
 laid out as the interpreter that compiled it lays them out: every interpreter has a library of its own.
+``libkva_tensors.<interpreter>.so`` - ``csrc/host/torch/*.cpp``, against torch's headers, of that interpreter and torch alone; where it
+cannot be built, what it does is done in Python.
 
 Libraries are kept in ``<package>/_lib`` when that folder can be written, otherwise in a
 per-user folder under the system's temporary directory.  A stamp file holds a hash of the
@@ -20,7 +22,7 @@ import tempfile
 import time
 from concurrent.futures import ThreadPoolExecutor
 from concurrent.futures import TimeoutError as FutureTimeout
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(PKG_DIR, "csrc")
@@ -203,7 +205,46 @@ def build_host(force: bool = False) -> str:
     return lib
 
 
+def tensors_name() -> str:
+    return f"libkva_tensors.{sysconfig.get_config_var('SOABI') or sys.implementation.cache_tag}.so"
+
+
+def build_tensors(force: bool = False) -> Optional[str]:
+    """Path of an up-to-date library of ``csrc/host/torch`` for this interpreter and torch, or ``None`` where it cannot be
+    built (no headers, no compiler, no folder to write to)."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
+    d = os.path.join(CSRC, "host", "torch")
+    sources = sorted(os.path.join(d, f) for f in os.listdir(d) if f.endswith(".cpp"))
+    flags = [*HOST_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    name, digest = tensors_name(), _digest(sources, flags + [tensors_name(), sys.version, torch.__version__, root])
+    if not force:
+        cur = _find_current(name, digest)
+        if cur:
+            return cur
+    cxx = shutil.which("g++") or shutil.which("c++") or shutil.which("clang++")
+    if cxx is None or not all(os.path.isdir(i) for i in include) or not os.path.isfile(os.path.join(include[-1], "Python.h")):
+        return None
+    try:
+        out_dir = _writable_dir()
+        lib = os.path.join(out_dir, name)
+        tmp = lib + f".tmp{os.getpid()}"
+        libs = os.path.join(root, "lib")
+        _say(f"compiling the reader of tensors into {out_dir}")
+        _run([cxx, *flags, *[x for i in include for x in ("-isystem", i)], *sources, "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
+              f"-Wl,-rpath,{libs}", "-o", tmp], "compiling " + name)
+        os.replace(tmp, lib)
+        with open(lib + ".stamp", "w") as f:
+            f.write(digest + "\n")
+    except (BuildError, OSError) as e:
+        _say(f"{name} was not built, its checks run in Python: {str(e).splitlines()[0]}")
+        return None
+    return lib
+
+
 def build_all(force: bool = False) -> Tuple[str, str]:
+    build_tensors(force)
     return build_host(force), build_hip(force)
 
 

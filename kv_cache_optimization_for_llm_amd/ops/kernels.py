@@ -13,7 +13,7 @@ from typing import Optional
 
 import torch
 
-from .library import KernelError, check, hip_lib
+from .library import KernelError, check, hip_lib, tensor_reader
 
 F32, BF16 = 0, 1
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -1196,42 +1196,71 @@ def mark_tokens(mask: torch.Tensor, seats: torch.Tensor, tokens: torch.Tensor) -
           "mark_tokens")
 
 
-def _at(what: str, name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: tuple, device: int) -> Optional[int]:
-    """The address of a contiguous tensor of this type and shape on the device that the launch goes to; ``None`` for no tensor.  (What
-    it looks at first takes a fifth of the time of the reasons it gives: these launches are a few microseconds long.)"""
+def _at(what: str, name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: tuple, device: int) -> int:
+    """The address of a contiguous tensor of this type and shape on the device that the launch goes to; 0 for no tensor."""
     if t is None:
-        return None
-    try:
-        if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():
-            return t.data_ptr()
-    except AttributeError:
-        raise KernelError(f"{what}: {name}: expected a tensor, got {type(t).__name__}") from None
+        return 0
+    if not isinstance(t, torch.Tensor):
+        raise KernelError(f"{what}: {name}: expected a tensor, got {type(t).__name__}")
     if t.shape != shape:
         raise KernelError(f"{what}: {name} is {tuple(t.shape)}, expected {tuple(shape)}")
-    _dev(t, f"{what}: {name}", dtype)
-    raise KernelError(f"{what}: {name} is on {t.device}, the launch goes to cuda:{device}")
-
-
-def _launch_device(what: str, t: torch.Tensor) -> int:
-    """The current device, which has to be the tensor's: the launch goes to its stream."""
-    if not t.is_cuda:
-        raise KernelError(f"{what}: tensor is on {t.device}; the kernels run on the GPU only")
-    device = _RAW_DEVICE()
+    if t.dtype != dtype:
+        raise KernelError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+    if t.layout is not torch.strided or not t.is_contiguous():
+        raise KernelError(f"{what}: {name} must be contiguous")
     if t.get_device() != device:
-        raise KernelError(f"{what}: a tensor is on {t.device}, the current device is cuda:{device}")
-    return device
+        raise KernelError(f"{what}: {name} is on {t.device}, the launch goes to " + (f"cuda:{device}" if device >= 0 else "no GPU"))
+    return t.data_ptr()
 
 
-def _rows_of(what: str, name: str, t: torch.Tensor) -> int:
-    """Elements from a row of ``[rows, columns]`` to the next; the elements of a row lie next to each other."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+_READER = None
+
+
+def _reader():
+    global _READER
+    if _READER is None:
+        _READER = tensor_reader() or False
+    return _READER
+
+
+def _addresses(what: str, names: str, spec: tuple) -> array:
+    """The addresses of ``spec``'s tensors, ``(device, tensor, dtype, shape, tensor, dtype, shape, ...)``, each as :func:`_at` has
+    it, all of them before :func:`_here` looks at the device; in one native call where the reader of tensors is there and nothing is wrong."""
+    out = _NO_ADDRESS * (len(spec) // 3)
+    reader = _reader()
+    if not reader or reader[0](spec, out.buffer_info()[0]) != 0:
+        for i, name in enumerate(names.split()):
+            out[i] = _at(what, name, *spec[3 * i + 1:3 * i + 4], spec[0])
+    return out
+
+
+_NO_ADDRESS = array("q", (0,))
+
+
+def _rows_of(what: str, name: str, t: torch.Tensor) -> tuple:
+    """(address, rows, columns, elements from a row to the next, type, device) of a matrix on the GPU; the elements of a row lie next to
+    each other."""
+    reader = _reader()
+    if reader:
+        out = _NO_ADDRESS * 6
+        if reader[1](t, out.buffer_info()[0]) == 0:
+            return out.tolist()
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.layout is not torch.strided:
         raise KernelError(f"{what}: {name} must be [rows, vocabulary]")
     (rows, cols), (stride, one) = t.shape, t.stride()
     if cols > 1 and one != 1:
         raise KernelError(f"{what}: the elements of a row of {name} must lie next to each other")
     if rows > 1 and stride < cols:
         raise KernelError(f"{what}: rows of {name} overlap")
-    return stride if rows > 1 else cols
+    return t.data_ptr(), rows, cols, stride if rows > 1 else cols, dtype_code(t.dtype), t.get_device()
+
+
+def _here(what: str, device: int) -> None:
+    """The tensors' device has to be the current one: the launch goes to its stream."""
+    if device < 0:
+        raise KernelError(f"{what}: the tensors are not on a GPU; the kernels run there only")
+    if device != _RAW_DEVICE():
+        raise KernelError(f"{what}: the tensors are on cuda:{device}, the current device is cuda:{_RAW_DEVICE()}")
 
 
 def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional[torch.Tensor] = None,
@@ -1253,10 +1282,6 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional
 
     A row that names a seat or a grammar that is not there gets -inf everywhere: no token can be taken from it."""
     what = "adjust_logits"
-    in_stride, out_stride = _rows_of(what, "logits", logits), _rows_of(what, "out", out)
-    rows, vocab = logits.shape
-    if out.shape != logits.shape:
-        raise KernelError(f"{what}: out {tuple(out.shape)} does not fit logits {tuple(logits.shape)}")
     if (marks is None) != (row_seat is None):
         raise KernelError(f"{what}: marks and the seats of the rows go together")
     if marks is None and (counts is not None or repetition is not None):
@@ -1265,40 +1290,38 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional
         raise KernelError(f"{what}: presence and frequency need counts")
     if (allowed is None) != (allowed_row is None):
         raise KernelError(f"{what}: grammars and the rows' numbers of them go together")
+    if bias is not None and (len(bias) != 3 or any(t is None for t in bias)):
+        raise KernelError(f"{what}: bias is (start, token, value)")
+    p_in, rows, vocab, in_stride, code, device = _rows_of(what, "logits", logits)
+    p_out, rows_out, vocab_out, out_stride, out_code, out_device = _rows_of(what, "out", out)
+    if rows_out != rows or vocab_out != vocab or out_code != F32 or out_device != device:
+        raise KernelError(f"{what}: out {tuple(out.shape)} {out.dtype} on {out.device} is not float32 of the shape and on the device of the logits")
     seats = grammars = biases = 0
     start = token = value = None
     if marks is not None:
         seats = marks.shape[0] if marks.dim() == 2 else 0
         if seats < 1:
             raise KernelError(f"{what}: marks must be [seats, {vocab}]")
+    words = (vocab + 31) // 32
     if allowed is not None:
         grammars = allowed.shape[0] if allowed.dim() == 2 else 0
         if grammars < 1:
-            raise KernelError(f"{what}: allowed must be [grammars, {(vocab + 31) // 32}] words of 32 tokens")
+            raise KernelError(f"{what}: allowed must be [grammars, {words}] words of 32 tokens")
     if bias is not None:
-        if len(bias) != 3:
-            raise KernelError(f"{what}: bias is (start, token, value)")
         start, token, value = bias
-        biases = token.shape[0] if token.dim() == 1 else -1
-    per_row = (rows,)
-    f32, i32 = torch.float32, torch.int32
-    # (shapes first: they are refused without a device, too)
-    device = logits.get_device() if logits.is_cuda else -1
-    args = (_at(what, "row_seat", row_seat, i32, per_row, device), seats, _at(what, "marks", marks, torch.uint8, (seats, vocab), device),
-            _at(what, "counts", counts, i32, (seats, vocab), device), _at(what, "repetition", repetition, f32, per_row, device),
-            _at(what, "presence", presence, f32, per_row, device), _at(what, "frequency", frequency, f32, per_row, device),
-            _at(what, "bias start", start, i32, (rows + 1,), device), _at(what, "bias token", token, i32, (biases,), device),
-            _at(what, "bias value", value, f32, (biases,), device), biases, _at(what, "allowed_row", allowed_row, i32, per_row, device),
-            _at(what, "allowed", allowed, i32, (grammars, (vocab + 31) // 32), device), grammars)
-    _launch_device(what, logits)
-    if out.dtype is not f32 or out.get_device() != device:
-        raise KernelError(f"{what}: out must be float32 on the logits' device")
-    p_in, p_out, code = logits.data_ptr(), out.data_ptr(), dtype_code(logits.dtype)
+        biases = token.numel()
     if rows and vocab and not (p_in == p_out and code == F32 and in_stride == out_stride):
         size = 4 if code == F32 else 2
         if p_in < p_out + 4 * ((rows - 1) * out_stride + vocab) and p_out < p_in + size * ((rows - 1) * in_stride + vocab):
             raise KernelError(f"{what}: out overlaps the logits without being them")
-    check(hip_lib().kva_adjust_logits(p_out, out_stride, p_in, code, in_stride, rows, vocab, *args, _stream()), what)
+    n, table, f32, i32 = (rows,), (seats, vocab), torch.float32, torch.int32
+    address = _addresses(what, "row_seat marks counts repetition presence frequency bias_start bias_token bias_value allowed_row allowed",
+                         (device, row_seat, i32, n, marks, torch.uint8, table, counts, i32, table, repetition, f32, n, presence, f32, n,
+                          frequency, f32, n, start, i32, (rows + 1,), token, i32, (biases,), value, f32, (biases,), allowed_row, i32, n,
+                          allowed, i32, (grammars, words)))
+    _here(what, device)
+    check(hip_lib().kva_adjust_logits(address.buffer_info()[0], p_out, out_stride, p_in, code, in_stride, rows, vocab, seats, biases, grammars,
+                                      _stream()), what)
     return out
 
 
@@ -1308,11 +1331,11 @@ def count_tokens(marks: torch.Tensor, counts: Optional[torch.Tensor], seats: tor
     what = "count_tokens"
     if marks.dim() != 2 or tokens.dim() != 1:
         raise KernelError(f"{what}: one seat per token, marks and counts [seats, vocab]")
-    rows, n, i32, device = marks.shape, tokens.shape, torch.int32, marks.get_device() if marks.is_cuda else -1
-    args = (_at(what, "marks", marks, torch.uint8, rows, device), _at(what, "counts", counts, i32, rows, device), rows[0], rows[1],
-            _at(what, "seats", seats, i32, n, device), _at(what, "tokens", tokens, i32, n, device), n[0])
-    _launch_device(what, marks)
-    check(hip_lib().kva_count_tokens(*args, _stream()), what)
+    rows, n, i32 = marks.shape, tokens.shape, torch.int32
+    address = _addresses(what, "marks counts seats tokens", (marks.get_device(), marks, torch.uint8, rows, counts, i32, rows, seats, i32, n,
+                                                             tokens, i32, n))
+    _here(what, marks.get_device())
+    check(hip_lib().kva_count_tokens(address[0], address[1], rows[0], rows[1], address[2], address[3], n[0], _stream()), what)
 
 
 def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temperature: torch.Tensor, top_k: Optional[torch.Tensor] = None,
@@ -1336,32 +1359,28 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
     tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
     what = "sample_truncated"
-    stride = _rows_of(what, "logits", logits)
-    rows, vocab = logits.shape
     if inv_temperature is None:
         raise KernelError(f"{what}: inv_temperature is needed")
     if uniform is None and (rng_key is None or rng_step is None):
         raise KernelError(f"{what}: random numbers, or a key and a step per row, are needed")
     if uniform is not None and (rng_key is not None or rng_step is not None):
         raise KernelError(f"{what}: random numbers are given twice")
+    p_in, rows, vocab, stride, code, device = _rows_of(what, "logits", logits)
+    if code != F32:
+        raise KernelError(f"{what}: logits are {logits.dtype}, expected torch.float32")
     if host_tokens is not None and (host_tokens.is_cuda or not host_tokens.is_pinned() or host_tokens.dtype != torch.int32
                                     or host_tokens.dim() != 1 or host_tokens.shape[0] < rows or not host_tokens.is_contiguous()):
         raise KernelError(f"{what}: host_tokens must be a pinned host int32 vector with a place per row")
-    device = logits.get_device() if logits.is_cuda else -1
     n, f32, i32 = (rows,), torch.float32, torch.int32
-    args = (_at(what, "inv_temperature", inv_temperature, f32, n, device), _at(what, "top_k", top_k, i32, n, device),
-            _at(what, "top_p", top_p, f32, n, device), _at(what, "min_p", min_p, f32, n, device), _at(what, "uniform", uniform, f32, n, device),
-            int(seed) & 0xFFFFFFFF, _at(what, "rng_key", rng_key, i32, n, device), _at(what, "rng_step", rng_step, i32, n, device),
-            _at(what, "kept", kept, i32, n, device), _at(what, "logprob", logprob, f32, n, device),
-            host_tokens.data_ptr() if host_tokens is not None else None)
-    tokens = _at(what, "out_tokens", out_tokens, i32, n, device)
-    _launch_device(what, logits)
-    if logits.dtype is not f32:
-        raise KernelError(f"{what}: logits are {logits.dtype}, expected torch.float32")
+    address = _addresses(what, "out_tokens inv_temperature top_k top_p min_p uniform rng_key rng_step kept logprob",
+                         (device, out_tokens, i32, n, inv_temperature, f32, n, top_k, i32, n, top_p, f32, n, min_p, f32, n, uniform, f32, n,
+                          rng_key, i32, n, rng_step, i32, n, kept, i32, n, logprob, f32, n))
+    _here(what, device)
     lib = hip_lib()
     size = lib.kva_sample_truncated_workspace_bytes(rows, vocab)
     space = torch.empty(size // 4, dtype=i32, device=logits.device) if size else None
-    check(lib.kva_sample_truncated(tokens, logits.data_ptr(), stride, rows, vocab, *args, space.data_ptr() if size else None, _stream()), what)
+    check(lib.kva_sample_truncated(address.buffer_info()[0], p_in, stride, rows, vocab, int(seed) & 0xFFFFFFFF,
+                                   host_tokens.data_ptr() if host_tokens is not None else None, space.data_ptr() if size else None, _stream()), what)
     return out_tokens
 
 
@@ -1380,18 +1399,16 @@ def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, le
     what = "grow_tables"
     if seats.dim() != 1 or pages.dim() != 1 or table.dim() != 2:
         raise KernelError(f"{what}: a table [rows, blocks], a seat, held blocks and a length per request, and a row of pages")
-    n, i32, device = seats.shape, torch.int32, table.get_device() if table.is_cuda else -1
-    entries = n[0]
+    n, size, i32, entries = seats.shape, table.shape, torch.int32, seats.shape[0]
     if offsets is None:
         offsets = torch.empty(entries + 1, dtype=i32, device=table.device)
-    size = table.shape
-    args = (_at(what, "table", table, i32, size, device), size[0], size[1], _at(what, "seats", seats, i32, n, device),
-            _at(what, "held", held, i32, n, device), _at(what, "lengths", lengths, i32, n, device), entries, int(page_size),
-            _at(what, "pages", pages, i32, pages.shape, device), pages.shape[0], _at(what, "offsets", offsets, i32, (entries + 1,), device))
-    _launch_device(what, table)
+    address = _addresses(what, "table seats held lengths pages offsets",
+                         (table.get_device(), table, i32, size, seats, i32, n, held, i32, n, lengths, i32, n, pages, i32, pages.shape,
+                          offsets, i32, (entries + 1,)))
+    _here(what, table.get_device())
     if entries == 0:
         return offsets.zero_()
-    check(hip_lib().kva_grow_tables(*args, _stream()), what)
+    check(hip_lib().kva_grow_tables(address.buffer_info()[0], size[0], size[1], entries, int(page_size), pages.shape[0], _stream()), what)
     return offsets
 
 
@@ -1406,16 +1423,16 @@ def step_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, 
     what = "step_rows"
     if lengths.dim() != 1 or positions.dim() != 1 or len(slots) != len(tables) or any(t.dim() != 2 for t in tables):
         raise KernelError(f"{what}: a length per entry, a position per token, tables [rows, blocks] and as many arrays of slots")
-    n, tokens, i32, device = lengths.shape, positions.shape, torch.int32, lengths.get_device() if lengths.is_cuda else -1
-    groups = []
+    n, tokens, i32 = lengths.shape, positions.shape, torch.int32
+    spec = (lengths.get_device(), lengths, i32, n, starts, i32, n, seats, i32, n, q_start, i32, (n[0] + 1,), positions, i32, tokens,
+            tok_seat, i32, tokens)
+    sizes = array("q")
     for t, s in zip(tables, slots):
-        groups += (_at(what, "table", t, i32, t.shape, device), *t.shape, _at(what, "slots", s, i32, tokens, device))
-    args = (_at(what, "q_start", q_start, i32, (n[0] + 1,), device), _at(what, "positions", positions, i32, tokens, device),
-            _at(what, "tok_seat", tok_seat, i32, tokens, device))
-    first = (_at(what, "lengths", lengths, i32, n, device), _at(what, "starts", starts, i32, n, device), _at(what, "seats", seats, i32, n, device))
-    _launch_device(what, lengths)
-    groups = array("q", groups)
-    check(hip_lib().kva_step_rows(*first, n[0], groups.buffer_info()[0], len(tables), int(page_size), tokens[0], *args, _stream()), what)
+        spec += (t, i32, t.shape, s, i32, tokens)
+        sizes.extend(t.shape)
+    address = _addresses(what, "lengths starts seats q_start positions tok_seat" + " table slots" * len(tables), spec)
+    _here(what, spec[0])
+    check(hip_lib().kva_step_rows(address.buffer_info()[0], sizes.buffer_info()[0], n[0], len(tables), int(page_size), tokens[0], _stream()), what)
 
 
 _MAX_SPLITS = None

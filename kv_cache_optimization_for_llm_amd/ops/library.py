@@ -102,11 +102,11 @@ _HIP_SIGNATURES = {
     "kva_event_synchronize": [P],
     "kva_event_destroy": [P],
     "kva_mark_tokens": [P, P, P, I, I, P],
-    "kva_sample_truncated": [P, P, LL, I, I, P, P, P, P, P, U, P, P, P, P, P, P, P],
-    "kva_adjust_logits": [P, LL, P, I, LL, I, I, P, I, P, P, P, P, P, P, P, P, I, P, P, I, P],
+    "kva_sample_truncated": [P, P, LL, I, I, U, P, P, P],
+    "kva_adjust_logits": [P, P, LL, P, I, LL, I, I, I, I, I, P],
     "kva_count_tokens": [P, P, I, I, P, P, I, P],
-    "kva_grow_tables": [P, I, I, P, P, P, I, I, P, I, P, P],
-    "kva_step_rows": [P, P, P, I, P, I, I, I, P, P, P, P],
+    "kva_grow_tables": [P, I, I, I, I, I, P],
+    "kva_step_rows": [P, P, I, I, I, I, P],
     "kva_delta_token": [I, P, I, I, I, P, I, P, LL, I, I, I, I, P, P, P, I, F, P, F, P, I, I, I, I, P, I, I, I, F, P, P, I, I, I, I, I, P],
     "kva_linear_token": [I, P, I, I, I, I, I, I, I, P, I, P, F, F, P, LL, I, P, F, P, I, I, I, I, P, I, I, I, F, P, P, I, I, I, I, P],
     "kva_space_token": [I, P, I, I, I, P, P, I, P, LL, I, I, I, P, P, P, P, F, I, P, I, I, I, F, P, P, I, I, I, I, I, I, P],
@@ -258,3 +258,25 @@ def sample_rows():
             fn.argtypes, fn.restype = [ctypes.py_object, LL, P, LL, I], I
         _sample_rows = fn
     return _sample_rows or None
+
+
+_tensor_reader = None
+
+
+def tensor_reader():
+    """``(kva_tensor_args, kva_tensor_rows)`` of the reader of tensors (they take Python objects and are called with the
+    interpreter's lock held), or None where it was not built."""
+    global _tensor_reader
+    if _tensor_reader is None:
+        path = build.build_tensors()
+        try:
+            lib = ctypes.PyDLL(path) if path else None
+        except OSError:
+            lib = None
+        if lib is None:
+            _tensor_reader = False
+        else:
+            lib.kva_tensor_args.argtypes, lib.kva_tensor_args.restype = [ctypes.py_object, LL], LL
+            lib.kva_tensor_rows.argtypes, lib.kva_tensor_rows.restype = [ctypes.py_object, LL], LL
+            _tensor_reader = (lib.kva_tensor_args, lib.kva_tensor_rows)
+    return _tensor_reader or None

@@ -254,3 +254,18 @@ def test_batches_made_on_the_device_are_the_hosts(gpu):
             live[s] = a + n
             m.commit(s, a + n)
         m.check()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_steps_of_more_entries_than_a_launch_takes(model_dirs, gpu, dtype, monkeypatch):
+    """Beyond what one launch makes rows for, the host makes them: the same tokens."""
+    prompts = prompts_for(256, [30, 9, 21, 3], 8)
+    llm = LLM(model_dirs["A"], EngineOptions(dtype=dtype, max_seqs=4, max_seq_len=64))
+    want = llm.generate(prompts, 10, ignore_eos=True)
+    from kv_cache_optimization_for_llm_amd.engine import engine as module
+    from kv_cache_optimization_for_llm_amd.ops import kernels
+    monkeypatch.setattr(module, "MAX_STEP_ENTRIES", 1)
+    monkeypatch.setattr(kernels, "MAX_STEP_ENTRIES", 1)
+    few = LLM(model_dirs["A"], EngineOptions(dtype=dtype, max_seqs=4, max_seq_len=64))
+    assert few.generate(prompts, 10, ignore_eos=True) == want
+    few.engine.cache.check()

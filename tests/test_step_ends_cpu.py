@@ -1,5 +1,6 @@
 """Refusals of the operators around a model's layers, and their plain forms, without a GPU."""
 import math
+from array import array
 
 import numpy as np
 import pytest
@@ -7,7 +8,7 @@ import torch
 
 import plain_step_ends as plain
 from kv_cache_optimization_for_llm_amd.ops import kernels as K
-from kv_cache_optimization_for_llm_amd.ops.library import KernelError
+from kv_cache_optimization_for_llm_amd.ops.library import KernelError, check, hip_lib, tensor_reader
 
 
 def i32(*shape):
@@ -120,3 +121,65 @@ def test_plain_tables_by_hand():
     assert table.tolist() == [[9, -1, -1, -1], [-1] * 4, [-1, 7, 8, -1]]
     q, pos, seat, slots = plain.step_rows([2, 0, 1], [15, 3, 0], [2, 1, 0], [table], 16)
     assert q == [0, 2, 2, 3] and pos == [15, 16, 0] and seat == [2, 2, 0] and slots == [[-1, 112, 144]]
+
+
+@pytest.mark.parametrize("message, call", [
+    (r"row_seat is \(3,\), expected \(2,\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), row_seat=i32(3), marks=marks(4, 40))),
+    (r"marks is \(4, 41\), expected \(4, 40\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), row_seat=i32(2), marks=marks(4, 41))),
+    (r"marks is torch.int32", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), row_seat=i32(2), marks=i32(4, 40))),
+    (r"counts must be contiguous", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), row_seat=i32(2), marks=marks(4, 40), counts=i32(40, 4).t())),
+    (r"allowed is \(1, 1\), expected \(1, 2\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), allowed=i32(1, 1), allowed_row=i32(2))),
+    (r"bias_start is \(2,\), expected \(3,\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), bias=(i32(2), i32(5), f32(5)))),
+    (r"bias_value is \(4,\), expected \(5,\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), bias=(i32(3), i32(5), f32(4)))),
+    (r"bias is \(start, token, value\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), bias=(None, i32(5), f32(5)))),
+    (r"bias is \(start, token, value\)", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), bias=(i32(3), i32(5), None))),
+    (r"out .* is not float32", lambda: K.adjust_logits(f32(2, 40), f32(2, 40).bfloat16())),
+    (r"repetition: expected a tensor", lambda: K.adjust_logits(f32(2, 40), f32(2, 40), row_seat=i32(2), marks=marks(4, 40), repetition=1.5)),
+    (r"not on a GPU", lambda: K.adjust_logits(f32(2, 40), f32(2, 40))),
+    (r"inv_temperature is \(3,\)", lambda: K.sample_truncated(f32(2, 40), i32(2), inv_temperature=f32(3), uniform=f32(2))),
+    (r"out_tokens is \(3,\)", lambda: K.sample_truncated(f32(2, 40), i32(3), inv_temperature=f32(2), uniform=f32(2))),
+    (r"logits are torch.bfloat16", lambda: K.sample_truncated(f32(2, 40).bfloat16(), i32(2), inv_temperature=f32(2), uniform=f32(2))),
+    (r"top_k is torch.float32", lambda: K.sample_truncated(f32(2, 40), i32(2), inv_temperature=f32(2), uniform=f32(2), top_k=f32(2))),
+    (r"not on a GPU", lambda: K.sample_truncated(f32(2, 40), i32(2), inv_temperature=f32(2), uniform=f32(2))),
+    (r"held is \(2,\)", lambda: K.grow_tables(i32(4, 8), i32(3), i32(2), i32(3), 16, i32(9))),
+    (r"offsets is \(3,\)", lambda: K.grow_tables(i32(4, 8), i32(3), i32(3), i32(3), 16, i32(9), i32(3))),
+    (r"table must be contiguous", lambda: K.grow_tables(i32(8, 4).t(), i32(3), i32(3), i32(3), 16, i32(9))),
+    (r"not on a GPU", lambda: K.grow_tables(i32(4, 8), i32(3), i32(3), i32(3), 16, i32(9))),
+    (r"q_start is \(3,\)", lambda: K.step_rows(i32(3), i32(3), i32(3), [i32(4, 8)], 16, i32(3), i32(5), i32(5), [i32(5)])),
+    (r"slots is \(6,\)", lambda: K.step_rows(i32(3), i32(3), i32(3), [i32(4, 8)], 16, i32(4), i32(5), i32(5), [i32(6)])),
+    (r"not on a GPU", lambda: K.step_rows(i32(3), i32(3), i32(3), [i32(4, 8)], 16, i32(4), i32(5), i32(5), [i32(5)])),
+    (r"counts is \(2, 8\)", lambda: K.count_tokens(marks(2, 9), i32(2, 8), i32(3), i32(3))),
+    (r"not on a GPU", lambda: K.count_tokens(marks(2, 9), i32(2, 9), i32(3), i32(3)))])
+def test_refusals_say_why(message, call):
+    with pytest.raises(KernelError, match=message):
+        call()
+
+
+def test_the_reader_of_tensors_takes_gpu_tensors_only():
+    """Whatever it does not know goes to the checks in Python: wrong objects, tensors of the host, odd lists."""
+    reader = tensor_reader()
+    assert reader is not None, "torch's headers are here: it has to build"
+    args, rows = reader
+    out = array("q", [7] * 6)
+    at = out.buffer_info()[0]
+    assert args((0,), at) == 0
+    assert args((0, None, torch.int32, (3,)), at) == 0 and out[0] == 0
+    assert args((-1, i32(3), torch.int32, (3,)), at) != 0
+    assert args((0, None, torch.int32, (3,), i32(3), torch.int32, (3,)), at) == 2
+    for bad in ((0, 5, torch.int32, (3,)), (0, i32(3), "int32", (3,)), (0, i32(3), torch.int32, 3), (0, i32(3), torch.int32, ("a",)),
+                ("a",), (0, i32(3)), [0], None, (1 << 80,)):
+        assert args(bad, at) != 0
+    for bad in (f32(3, 4), None, 5, f32(3)):
+        assert rows(bad, at) != 0
+
+
+def test_a_launch_needs_its_tensors():
+    """What the C entries refuse before any launch: addresses that are not there."""
+    lib = hip_lib()
+    none, one = array("q", [0] * 16), array("q", [4, 4])
+    at, size = none.buffer_info()[0], one.buffer_info()[0]
+    for call in (lambda: lib.kva_grow_tables(at, 4, 4, 2, 16, 3, 0), lambda: lib.kva_step_rows(at, size, 2, 1, 16, 2, 0),
+                 lambda: lib.kva_count_tokens(0, 0, 2, 9, 0, 0, 3, 0), lambda: lib.kva_adjust_logits(at, 64, 40, 64, 0, 40, 2, 40, 0, 3, 0, 0),
+                 lambda: lib.kva_sample_truncated(at, 64, 40, 2, 40, 0, 0, 0, 0)):
+        with pytest.raises(KernelError):
+            check(call(), "a launch")

@@ -444,3 +444,121 @@ def test_a_step_in_a_graph(gpu):
             before[2][seat_of[r], drawn[r]] += 1
             before[1][seat_of[r], drawn[r]] = 1
         assert np.array_equal(counts.cpu().numpy(), before[2]) and np.array_equal(marks.cpu().numpy(), before[1])
+
+
+# ---------------------------------------------------------------- calls that a user may make
+@pytest.mark.parametrize("native", [True, False])
+def test_refusals_on_the_gpu(gpu, native, monkeypatch):
+    """The native check of the tensors and the one in Python refuse the same calls for the same reasons, and pass the same."""
+    if not native:
+        monkeypatch.setattr(K, "_READER", False)
+    i = lambda *s: torch.zeros(s, dtype=torch.int32, device=gpu)
+    f = lambda *s: torch.zeros(s, device=gpu)
+    m = lambda *s: torch.zeros(s, dtype=torch.uint8, device=gpu)
+    for message, call in (
+            (r"row_seat is \(3,\)", lambda: K.adjust_logits(f(2, 40), f(2, 40), row_seat=i(3), marks=m(4, 40))),
+            (r"row_seat is on cpu", lambda: K.adjust_logits(f(2, 40), f(2, 40), row_seat=i(2).cpu(), marks=m(4, 40))),
+            (r"marks is torch.int32", lambda: K.adjust_logits(f(2, 40), f(2, 40), row_seat=i(2), marks=i(4, 40))),
+            (r"counts must be contiguous", lambda: K.adjust_logits(f(2, 40), f(2, 40), row_seat=i(2), marks=m(4, 40), counts=i(40, 4).t())),
+            (r"out .* is not float32", lambda: K.adjust_logits(f(2, 40), f(2, 40).cpu())),
+            (r"rows of logits overlap", lambda: K.adjust_logits(f(1, 40).expand(2, 40), f(2, 40))),
+            (r"next to each other", lambda: K.adjust_logits(f(2, 80)[:, ::2], f(2, 40))),
+            (r"dtype", lambda: K.adjust_logits(f(2, 40).half(), f(2, 40))),
+            (r"a place for a token per row", lambda: K.sample_truncated(f(2, 40), None, inv_temperature=f(2), uniform=f(2))),
+            (r"logits are torch.bfloat16", lambda: K.sample_truncated(f(2, 40).bfloat16(), i(2), inv_temperature=f(2), uniform=f(2))),
+            (r"top_p: expected a tensor", lambda: K.sample_truncated(f(2, 40), i(2), inv_temperature=f(2), uniform=f(2), top_p=0.9)),
+            (r"are needed", lambda: K.grow_tables(i(4, 8), i(3), None, i(3), 16, i(9))),
+            (r"lengths is \(2,\)", lambda: K.grow_tables(i(4, 8), i(3), i(3), i(2), 16, i(9))),
+            (r"are needed", lambda: K.step_rows(i(3), i(3), None, [i(4, 8)], 16, i(4), i(5), i(5), [i(5)])),
+            (r"slots are missing", lambda: K.step_rows(i(3), i(3), i(3), [i(4, 8)], 16, i(4), i(5), i(5), [None])),
+            (r"slots is \(6,\)", lambda: K.step_rows(i(3), i(3), i(3), [i(4, 8)], 16, i(4), i(5), i(5), [i(6)])),
+            (r"are needed", lambda: K.count_tokens(m(2, 9), i(2, 9), None, i(3)))):
+        with pytest.raises(KernelError, match=message):
+            call()
+    rng = np.random.default_rng(6)
+    a = adjust_case(rng, 5, 333, 6, 50, 20, 2, torch.float32)
+    check_adjusted(adjust_on(gpu, a, torch.float32), a)
+    table = i(3, 4)
+    assert K.grow_tables(table, dev([2]), dev([1]), dev([40]), 16, dev([8, 9])).tolist() == [0, 2] and table[2].tolist() == [0, 8, 9, 0]
+
+
+def test_adjust_logits_larger_than_the_caches(gpu):
+    """300 rows of 100,003 tokens: more than 256 MiB, which pass the caches by; apart and in place."""
+    rng = np.random.default_rng(12)
+    a = adjust_case(rng, 300, 100003, 40, 30, 5, 0, torch.float32)
+    a["bias"] = tuple(a["bias"])
+    check_adjusted(adjust_on(gpu, a, torch.float32), a)
+    x = dev(a["logits"], torch.float32)
+    check_adjusted(adjust_on(gpu, a, torch.float32, out=x, logits=x), a)
+
+
+@pytest.mark.parametrize("vocab", [300, 20000, 262147])
+def test_sample_truncated_passes_rows_over(gpu, vocab):
+    """A row whose inverse temperature is no number: what is in its places stays, the rows beside it draw what they draw alone."""
+    rng = np.random.default_rng(vocab)
+    x = rows_of("model", rng, 9, vocab).astype(np.float32)
+    inv_t, u = np.full(9, 0.7, np.float32), rng.random(9).astype(np.float32)
+    inv_t[[0, 4, 8]] = np.nan
+    k, p, m = np.full(9, 50), np.full(9, 0.9, np.float32), np.zeros(9, np.float32)
+    got = draw_on(gpu, x, inv_t, k, p, m, u)
+    over = np.isnan(inv_t)
+    assert (got[0][over] == -9).all() and (got[1][over] == -9).all() and (got[2][over] == 9).all()
+    stay = ~over
+    check_drawn(x[stay], inv_t[stay], k[stay], p[stay], m[stay], u[stay], *(t[stay] for t in got))
+    host = torch.full((9,), -5, dtype=torch.int32, pin_memory=True)
+    out = torch.full((9,), -9, dtype=torch.int32, device=gpu)
+    K.sample_truncated(dev(x, torch.float32), out, inv_temperature=dev(inv_t, torch.float32), uniform=dev(u, torch.float32), host_tokens=host)
+    torch.cuda.synchronize()
+    assert (host[over] == -5).all() and torch.equal(host[stay], out.cpu()[stay])
+
+
+def test_two_draws_at_once(gpu):
+    """Draws on two streams beside each other, over and over: no workspace is another's."""
+    rng = np.random.default_rng(2)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    cases = []
+    for rows, vocab in ((30, 50021), (3, 128256)):
+        x = dev(rows_of("model", rng, rows, vocab), torch.float32)
+        kw = dict(inv_temperature=torch.full((rows,), 0.8, device=gpu), top_p=torch.full((rows,), 0.95, device=gpu),
+                  uniform=dev(rng.random(rows), torch.float32))
+        outs = [torch.empty(rows, dtype=torch.int32, device=gpu) for _ in range(20)]
+        want = torch.empty(rows, dtype=torch.int32, device=gpu)
+        K.sample_truncated(x, want, **kw)
+        cases.append((x, kw, outs, want))
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, (x, kw, outs, _) in zip(streams, cases):
+            with torch.cuda.stream(s):
+                K.sample_truncated(x, outs[i], **kw)
+    torch.cuda.synchronize()
+    for _, _, outs, want in cases:
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_two_graphs_of_draws(gpu):
+    """Two captured draws, replayed in turn and over new logits, with eager draws between."""
+    rng = np.random.default_rng(14)
+    rows, vocab = 7, 50021
+    x = torch.zeros(rows, vocab, device=gpu)
+    kw = dict(inv_temperature=torch.full((rows,), 0.9, device=gpu), top_p=torch.full((rows,), 0.9, device=gpu),
+              uniform=dev(rng.random(rows), torch.float32))
+    outs = [torch.zeros(rows, dtype=torch.int32, device=gpu) for _ in range(2)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        K.sample_truncated(x, outs[0], **kw)
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            K.sample_truncated(x, outs[i], top_k=torch.full((rows,), 5 + 60 * i, dtype=torch.int32, device=gpu), **kw)
+        graphs.append(g)
+    for turn in range(6):
+        x.copy_(dev(rows_of("model", rng, rows, vocab), torch.float32))
+        for i in ((0, 1), (1, 0))[turn % 2]:
+            outs[i].fill_(-3)
+            graphs[i].replay()
+            eager = torch.empty_like(outs[0])
+            K.sample_truncated(x, eager, top_k=torch.full((rows,), 5 + 60 * i, dtype=torch.int32, device=gpu), **kw)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], eager)
