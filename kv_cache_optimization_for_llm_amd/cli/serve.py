@@ -138,10 +138,10 @@ def main(argv=None) -> int:
               file=sys.stderr)
         return 1
     penalty = float(env.get("REPETITION_PENALTY", "1.15") or 1.15)
-    asked = {name: kind(env[name.upper()]) for name, kind in (("top_k", int), ("top_p", float), ("min_p", float), ("presence_penalty", float),
-                                                              ("frequency_penalty", float)) if env.get(name.upper())}
     from ..sampling.options import SampleOptions
     try:
+        asked = {name: kind(env[name.upper()]) for name, kind in (("top_k", int), ("top_p", float), ("min_p", float), ("presence_penalty", float),
+                                                                  ("frequency_penalty", float)) if env.get(name.upper())}
         sampling = SampleOptions(**asked) if asked else None
     except ValueError as e:
         print(f"Unusable sampling options: {e}", file=sys.stderr)

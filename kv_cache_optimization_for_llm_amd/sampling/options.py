@@ -14,6 +14,9 @@ from typing import Callable, Mapping, Optional, Sequence
 import numpy as np
 
 
+_MOST = float(np.finfo(np.float32).max)         # what the kernels compute in
+
+
 @dataclass(frozen=True)
 class SampleOptions:
     """``repetition_penalty``: None is the server's.  ``penalize_prompt``: the repetition penalty takes the prompt's tokens as emitted
@@ -40,13 +43,13 @@ class SampleOptions:
             if not lo <= v <= hi or (name == "top_p" and v == 0):
                 raise ValueError(f"{name} {v!r} is not between 0 and 1")
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite")
-        if self.repetition_penalty is not None and not (self.repetition_penalty > 0 and math.isfinite(self.repetition_penalty)):
-            raise ValueError("repetition_penalty must be positive")
+            if not abs(getattr(self, name)) <= _MOST:
+                raise ValueError(f"{name} must be finite in 32 bits")
+        if self.repetition_penalty is not None and not 1 / _MOST <= self.repetition_penalty <= _MOST:
+            raise ValueError("repetition_penalty must be positive and finite in 32 bits, as its inverse")
         for token, value in (self.logit_bias or {}).items():
-            if int(token) != token or token < 0 or math.isnan(value) or value == math.inf:
-                raise ValueError(f"logit_bias {token!r}: {value!r} is not a token id and a number below infinity")
+            if int(token) != token or token < 0 or not value <= _MOST:
+                raise ValueError(f"logit_bias {token!r}: {value!r} is not a token id and a number below the infinity of 32 bits")
         if self.grammar is not None and not callable(self.grammar):
             raise ValueError("grammar must be callable")
 

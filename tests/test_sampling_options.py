@@ -77,3 +77,14 @@ def test_positions_without_a_page_are_refused():
         m.check_mapped(seat, 12, 1, 0)
     m.flush_tables()                    # (no device: nothing to bring up to date)
     assert not m.groups[0].dirty
+
+
+@pytest.mark.parametrize("bad", [dict(logit_bias={3: 1e39}), dict(presence_penalty=1e39), dict(frequency_penalty=-1e39), dict(repetition_penalty=1e-50),
+                                 dict(repetition_penalty=1e39), dict(logit_bias={3: float("nan")})])
+def test_numbers_that_32_bits_do_not_hold_are_refused(bad):
+    with pytest.raises(ValueError):
+        SampleOptions(**bad)
+
+
+def test_a_ban_may_be_as_low_as_it_likes():
+    assert SampleOptions(logit_bias={3: -1e300, 4: -float("inf")}).logit_bias[4] == -float("inf")
