@@ -29,14 +29,15 @@
 // the places still in question are cut into 1,024 ranges, their numbers and weights added up in LDS, and the range in which the sum passes what is
 // sought is the next turn's; the row is read again in every turn (out of LDS up to 16,384 tokens).
 //
-// us in a graph.  Vocabulary 128,256: 1 row of a p 21, of a k 17; 64 rows of p 0.9 49 (7.2 + 18 + 17 + 9.2 for the four kernels), of a k up to 50 25 (7.7 + 2.0 + 2.0 +
-// 14.8: 33 MB are 6.4 us at a copy's rate); 256 rows of p 0.98 at a temperature of 2, which keep most of the vocabulary, 117 (21 + 33 + 59 + 11: the
+// us in a graph.  Vocabulary 128,256: 1 row of a p 21, of a k 17; 64 rows of p 0.9 49 (7.2 + 18 + 17 + 9.2 for the four kernels), of a k up to 50 24 (7.4 + 1.8 + 1.8 +
+// 14.2: 33 MB are 6.4 us at a copy's rate); 256 rows of p 0.98 at a temperature of 2, which keep most of the vocabulary, 117 (21 + 33 + 59 + 11: the
 // first reads 131 MB at 6.2 TB/s, the next two weigh every token); rows of nearly equal logits 410 to 480.  One launch, against four: 1,024 tokens 10 / 16
 // to 25, 2,048 13 to 15 / 17 to 22, 4,096 16 to 21 / 17 to 29, 8,192 28 to 31 / 18 to 25.
 #include "common.h"
 #include "counter_uniform.h"
 #include "wave_scan.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #define TR_THREADS 256
@@ -501,8 +502,10 @@ sample_truncated_kernel(TruncArgs a) {
 #define TR_SPLIT_WAVES (TR_SPLIT_THREADS / KVA_WAVE)
 #define TR_WAVE_LIST 1024
 #define TR_MAX_PARTS 64
-#define TR_FEW_MOST 512
-#define TR_FEW_STEPS 2048
+#define TR_FEW_MOST 1024
+#define TR_FEW_MOST_OF_FEW_ROWS 256
+#define TR_FEW_ROWS 3
+#define TR_FEW_STEPS 4096
 #define TR_GROUPS 64                    // groups a part
 #define TR_MAX_VOCAB (TR_BUCKET * TR_BUCKETS)
 
@@ -516,19 +519,19 @@ struct TruncSpace {                     // of all rows
     u64 *list;                          // [TR_LIST]: places
     int *listed;                        // [1]: tokens that asked for a place in the list
     int parts, part_tokens, buckets;
+    int few;                            // the largest k that is found by the groups' best tokens
 };
 
 // What a row's cut is found by: nothing, the number of tokens up to a bin, their weight, or the best tokens of the groups.  The last is for a
-// small k, as long as one workgroup reads the k groups it leaves sooner than many read the row twice more: by the steps a group
-// has, up to 4,096 of all of them, or 2,048 from k = 257 on (and k at most half of the groups).  us by groups / by bins, all rows of a launch: 64 rows of
-// 128,256 and k up to 100 (8 steps a group) 29 / 44, up to 250 40 / 60, 256 rows and k up to 100 (32 steps) 59 / 84; 64 rows and k up to 2,000, those
-// up to 512 by groups 93, up to 256 80, up to 64 71 (a launch with both kinds pays for both); 37 rows of 50,021 and k up to 400 (2 steps) 31 / 41.
+// small k, as long as one workgroup reads the k groups it leaves sooner than many read the row twice more: up to 1,024, half of the groups, and
+// 4,096 steps of theirs; of three rows, which have the chip to themselves, up to 256.  us in a graph by groups / by bins, k of all of a launch's rows up
+// to ...: 1 row of 128,256 (2 steps a group), 600 28 / 24; 4 rows, 600 29 / 31, 1,000 35 / 31; 16 rows, 1,000 36 / 67; 37 rows of 50,021 (2 steps), 400
+// 26 / 52, 1,000 44 / 57; 64 rows of 128,256 (8 steps), 100 28 / 51, 400 45 / 62; 256 rows of 128,256 (32 steps), 100 56 / 84.  A launch with both
+// kinds pays for both: these with k up to 250 100 / 85.
 enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2, TR_FEW = 3 };
 __device__ inline int tr_mode(const TruncArgs &a, const TruncSpace &sp, int row) {
     const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    if (k > 0 && k < a.vocab) return k <= min(TR_FEW_MOST, sp.parts * TR_GROUPS / 2) &&
-                                               k * (sp.part_tokens / TR_STEP) <= (k <= TR_FEW_MOST / 2 ? 2 * TR_FEW_STEPS : TR_FEW_STEPS)
-                                           ? TR_FEW : TR_COUNT;
+    if (k > 0 && k < a.vocab) return k <= sp.few ? TR_FEW : TR_COUNT;
     return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
 }
 
@@ -859,27 +862,48 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         for (int i = 0; i < TOPS; ++i)
             if (tops[i] != ~0ull && step_of(tr_logit(tops[i])) <= reach) group_of[atomicAdd(&groups_in, 1)] = (unsigned short)(tid + i * TR_THREADS);
         __syncthreads();
-        // four threads a group and step: its 16 tokens
-        const int steps = sp.part_tokens / TR_STEP, in = groups_in * steps;
+        // Four threads a group and step: its 16 tokens.  A wavefront is alone on its SIMD, so what counts is the length of the chain: all of a
+        // round's hits are places taken by one addition, and none of it branches but the taking (37 rows of 50,021 and k up to 400: 27 us,
+        // 31 with an addition a token).
+        const int steps = sp.part_tokens / TR_STEP, in = groups_in * steps, lane = tid % KVA_WAVE;
+        // (j / steps is the high half of j (2^32 / steps, rounded up): j is below 2^15)
+        const unsigned inverse = steps > 1 ? (unsigned)((0x100000000ull + steps - 1) / steps) : 0;
+        const float limit = reach < TR_DIGITS - 1 ? reach + 1.f : NAN;          // (of the last step on: all of them)
         constexpr int AHEAD = 4;            // loads on their way
-        for (int j0 = tid / 4; j0 < in; j0 += AHEAD * TR_THREADS / 4) {
-            float l[AHEAD][4];
-            int t[AHEAD];
+        for (int base = 0; base < in; base += AHEAD * TR_THREADS / 4) {
+            tr_f32x4 l[AHEAD];
+            int from_id[AHEAD];
+            unsigned hit[AHEAD], hits = 0;
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const int j = j0 + u * TR_THREADS / 4, group = group_of[min(j, in - 1) / steps];
-                t[u] = j < in ? group / TR_GROUPS * sp.part_tokens + j % steps * TR_STEP + group % TR_GROUPS * 16 + tid % 4 * 4 : vocab;
-                tr_load4(rl, t[u], vocab, l[u]);
+                const int j = base + tid / 4 + u * TR_THREADS / 4, at = min(j, in - 1), which = steps > 1 ? (int)__umulhi((unsigned)at, inverse) : at;
+                const int group = group_of[which];
+                const int t = j < in ? group / TR_GROUPS * sp.part_tokens + (at - which * steps) * TR_STEP + group % TR_GROUPS * 16 + tid % 4 * 4 : vocab;
+                from_id[u] = min(t, vocab - 4);
+                hit[u] = 15u << min(t - from_id[u], 4);         // (a load that would end behind the row begins in front of its tokens)
+                l[u] = *reinterpret_cast<const tr_f32x4 *>(rl + from_id[u]);
             }
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
+            for (int u = 0; u < AHEAD; ++u) {
+                unsigned in_reach = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!(l[u][i] > -INFINITY) || step_of(l[u][i]) > reach) continue;
-                    const u64 at = tr_place(l[u][i], t[u] + i);
-                    const int slot = atomicAdd(&asked, 1);
+                for (int i = 0; i < 4; ++i) in_reach |= l[u][i] > -INFINITY && !((best - l[u][i]) * scale >= limit) ? 1u << i : 0;
+                hit[u] &= in_reach;
+                hits += __popc(hit[u]);
+            }
+            const unsigned upto = wave_prefix(hits);
+            int slot = 0;
+            if (lane == KVA_WAVE - 1 && upto > 0) slot = atomicAdd(&asked, (int)upto);
+            slot = __builtin_amdgcn_readlane(slot, KVA_WAVE - 1) + (int)(upto - hits);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                while (hit[u] != 0) {
+                    const int i = __ffs(hit[u]) - 1;
+                    hit[u] &= hit[u] - 1;
+                    const u64 at = tr_place(i < 2 ? (i == 0 ? l[u][0] : l[u][1]) : (i == 2 ? l[u][2] : l[u][3]), from_id[u] + i);
                     if (slot < TR_LIST) place[slot] = at;
                     if (slot < TR_PAIRS) s.place[slot] = at;
+                    ++slot;
                 }
         }
         __syncthreads();
@@ -986,6 +1010,7 @@ extern "C" int kva_sample_truncated(const long long *address, const float *logit
     TruncSpace sp;
     sp.parts = trunc_parts(rows, vocab, &sp.part_tokens);
     sp.buckets = (vocab + TR_BUCKET - 1) / TR_BUCKET;
+    sp.few = std::min({rows <= TR_FEW_ROWS ? TR_FEW_MOST_OF_FEW_ROWS : TR_FEW_MOST, sp.parts * TR_GROUPS / 2, TR_FEW_STEPS / (sp.part_tokens / TR_STEP)});
     sp.best = (u64 *)workspace;
     sp.bins = sp.best + (size_t)rows * sp.parts;
     sp.tops = sp.bins + (size_t)rows * TR_BINS;
