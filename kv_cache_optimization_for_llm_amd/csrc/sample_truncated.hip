@@ -61,6 +61,27 @@ struct TruncArgs {
     float *logprob;
 };
 
+// What a row asks for.  Where a row's draw ends (`drawn`) all of it is loaded at once, one trip to memory in front of everything else; an
+// absent array's place is taken by one that is there.  (us in a graph, loaded where used / at once: 1 row 21.4 / 20.8, 64 rows without cuts 28.6 / 27.3.
+// The kernels that weigh whole rows gain nothing: 256 rows 117 / 120.)
+struct TruncRow {
+    float inv_t, p, min_p, u;
+    int k;
+    __device__ inline TruncRow(const TruncArgs &a, int row, bool drawn) {
+        const float *ps = a.top_p != nullptr ? a.top_p : a.inv_t, *ms = a.min_p != nullptr ? a.min_p : a.inv_t;
+        const int *ks = a.top_k != nullptr ? a.top_k : reinterpret_cast<const int *>(a.inv_t);
+        inv_t = a.inv_t[row], p = ps[row], min_p = ms[row], k = ks[row], u = 0.f;
+        if (drawn) {
+            if (a.uniform != nullptr) u = a.uniform[row];
+            else u = counter_uniform(a.seed, a.key[row], a.step[row]);
+        }
+        if (drawn) asm volatile("" : "+s"(inv_t), "+s"(p), "+s"(min_p), "+s"(k), "+v"(u));         // (else each is loaded where it is used first)
+        p = a.top_p != nullptr ? p : 1.f;
+        min_p = a.min_p != nullptr ? min_p : 0.f;
+        k = a.top_k != nullptr ? k : 0;
+    }
+};
+
 // descending logits as ascending 32-bit numbers; the two zeros are one (l + 0: -0 becomes 0)
 __device__ inline unsigned tr_falling(float l) {
     const unsigned b = __float_as_uint(l + 0.f);
@@ -269,13 +290,11 @@ __device__ inline u64 tr_share(float p, u64 total) {
 }
 
 // The x of TruncWeights that a token needs to stay (the best ones stay in any case).
-__device__ inline double tr_least(const TruncArgs &a, int row) {
-    const float least = a.min_p != nullptr ? a.min_p[row] : 0.f;
-    return least > 0.f ? TR_TABLE * (a.scale_bits + fmin(log2((double)least), 0.0)) : -INFINITY;
+__device__ inline double tr_least(const TruncRow &row, int bits) {
+    return row.min_p > 0.f ? TR_TABLE * (bits + fmin(log2((double)row.min_p), 0.0)) : -INFINITY;
 }
 
-__device__ inline u64 tr_target(const TruncArgs &a, int row, u64 all) {
-    const float u = a.uniform != nullptr ? a.uniform[row] : counter_uniform(a.seed, a.key[row], a.step[row]);
+__device__ inline u64 tr_target(float u, u64 all) {
     const u64 target = u > 0.f ? (u64)(fmin((double)u, 1.0) * (double)all) : 0ull;
     return min(target, all - 1);
 }
@@ -350,12 +369,12 @@ __device__ inline void tr_stay4(const float (&l)[4], int t, const TruncWeights &
 }
 
 // The token of a row, from what stays by ranges of `per` ids (a multiple of 256), in s.bucket_sum and s.bucket_count.
-__device__ inline void tr_draw(const TruncArgs &a, TruncShared &s, const float *rl, int row, int per, const TruncWeights &weigh, u64 last, double least) {
+__device__ inline void tr_draw(const TruncArgs &a, TruncShared &s, const float *rl, int row, float u, int per, const TruncWeights &weigh, u64 last, double least) {
     const int tid = threadIdx.x, lane = tid % KVA_WAVE;
     const FourSums sums = tr_four(s, s.bucket_sum, s.bucket_count);
     if (tid == TR_THREADS - 1) s.hi = sums.upto, s.inside_count = sums.count;
     __syncthreads();
-    const u64 all = s.hi, target = tr_target(a, row, all);
+    const u64 all = s.hi, target = tr_target(u, all);
     u64 run = sums.upto;
 #pragma unroll
     for (int i = TR_PER - 1; i >= 0; --i) {
@@ -389,9 +408,10 @@ __device__ inline void tr_draw(const TruncArgs &a, TruncShared &s, const float *
 }
 
 // A row (`rl`: its logits) by one workgroup that reads it in every turn; s.table is filled, or will be with the next barrier.
-__device__ inline void trunc_whole_row(const TruncArgs &a, TruncShared &s, const float *rl, int row) {
+__device__ inline void trunc_whole_row(const TruncArgs &a, TruncShared &s, const float *rl, int row, const TruncRow &of) {
     const int tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, vocab = a.vocab, bits = a.scale_bits;
-    const float inv_t = a.inv_t[row];
+    const float inv_t = of.inv_t, p = of.p;
+    const int k = of.k;
     auto each = [&](auto f) {
         float l[4];
         tr_load4(rl, 4 * tid, vocab, l);
@@ -425,11 +445,9 @@ __device__ inline void trunc_whole_row(const TruncArgs &a, TruncShared &s, const
         return;
     }
     const TruncWeights weigh(best, inv_t, bits, s.table);
-    const double least = tr_least(a, row);
+    const double least = tr_least(of, bits);
     auto weight = [&](u64 at) { return weigh.of(at); };
     u64 last = hi, total = 0;               // the last place that stays, the weight up to it
-    const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
     __syncthreads();
     if (k > 0 && (unsigned)k < valid) last = tr_cut(s, lo, hi, true, 0, (u64)k, total, each, weight);
     if (p < 1.f) {
@@ -470,7 +488,7 @@ __device__ inline void trunc_whole_row(const TruncArgs &a, TruncShared &s, const
         if (lane == KVA_WAVE - 1) s.bucket_sum[b] = sum, s.bucket_count[b] = count;
     }
     __syncthreads();
-    tr_draw(a, s, rl, row, per, weigh, last, least);
+    tr_draw(a, s, rl, row, of.u, per, weigh, last, least);
 }
 
 // grid (rows).  HELD: the row stands in LDS.
@@ -480,7 +498,8 @@ __global__ void __launch_bounds__(TR_THREADS)
 sample_truncated_kernel(TruncArgs a) {
     __shared__ TruncShared s;
     __shared__ __attribute__((aligned(16))) float held[HELD ? TR_HELD_VOCAB : 4];
-    if (isnan(a.inv_t[blockIdx.x])) return;
+    const TruncRow of(a, blockIdx.x, true);
+    if (isnan(of.inv_t)) return;
     tr_fill_table(s.table);             // (the first barrier comes before its first use)
     const float *rl = a.logits + blockIdx.x * a.stride;
     if (HELD) {
@@ -490,7 +509,7 @@ sample_truncated_kernel(TruncArgs a) {
             *reinterpret_cast<float4 *>(held + t) = make_float4(l[0], l[1], l[2], l[3]);       // (each thread its own: no barrier yet)
         }
     }
-    trunc_whole_row(a, s, HELD ? held : rl, blockIdx.x);
+    trunc_whole_row(a, s, HELD ? held : rl, blockIdx.x, of);
 }
 
 // ---------------------------------------------------------------- many workgroups a row
@@ -529,10 +548,9 @@ struct TruncSpace {                     // of all rows
 // 26 / 52, 1,000 44 / 57; 64 rows of 128,256 (8 steps), 100 28 / 51, 400 45 / 62; 256 rows of 128,256 (32 steps), 100 56 / 84.  A launch with both
 // kinds pays for both: these with k up to 250 100 / 85.
 enum { TR_ALL = 0, TR_COUNT = 1, TR_WEIGHT = 2, TR_FEW = 3 };
-__device__ inline int tr_mode(const TruncArgs &a, const TruncSpace &sp, int row) {
-    const int k = a.top_k != nullptr ? a.top_k[row] : 0;
-    if (k > 0 && k < a.vocab) return k <= sp.few ? TR_FEW : TR_COUNT;
-    return a.top_p != nullptr && a.top_p[row] < 1.f ? TR_WEIGHT : TR_ALL;
+__device__ inline int tr_mode(const TruncArgs &a, const TruncSpace &sp, const TruncRow &row) {
+    if (row.k > 0 && row.k < a.vocab) return row.k <= sp.few ? TR_FEW : TR_COUNT;
+    return row.p < 1.f ? TR_WEIGHT : TR_ALL;
 }
 
 // The four tokens of a thread in the step that begins at t0 (the same in all threads: a whole step needs no test a token).
@@ -559,14 +577,15 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ u64 of_wave[TR_SPLIT_WAVES];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     const float *rl = a.logits + row * a.stride;
-    if (isnan(a.inv_t[row])) return;
+    float l[4], top = -INFINITY;
+    tr_load_step(rl, part * sp.part_tokens, a.vocab, l);
+    const TruncRow of(a, row, false);
+    if (isnan(of.inv_t)) return;
     // (the next launches add to these)
     const int per = (TR_BINS + sp.parts - 1) / sp.parts;
     for (int i = part * per + tid; i < min(TR_BINS, (part + 1) * per); i += TR_SPLIT_THREADS) sp.bins[(size_t)row * TR_BINS + i] = 0;
     if (part == 0 && tid == 0) sp.listed[row] = 0;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens), lane = tid % KVA_WAVE, wave = tid / KVA_WAVE;
-    float l[4], top = -INFINITY;
-    tr_load_step(rl, part * sp.part_tokens, a.vocab, l);
     int id = 0;
     for (int t0 = part * sp.part_tokens; t0 < end; t0 += TR_STEP) {
         const int t = t0 + 4 * tid;
@@ -579,7 +598,7 @@ trunc_best_kernel(TruncArgs a, TruncSpace sp) {
         for (int i = 0; i < 4; ++i) l[i] = next[i];
     }
     u64 at = top > -INFINITY ? tr_place(top, id) : ~0ull;
-    if (tr_mode(a, sp, row) == TR_FEW) {
+    if (tr_mode(a, sp, of) == TR_FEW) {
         u64 of = min(at, (u64)__shfl_xor(at, 1, KVA_WAVE));
         of = min(of, (u64)__shfl_xor(of, 2, KVA_WAVE));
         if (tid % 4 == 0) sp.tops[((size_t)row * sp.parts + part) * TR_GROUPS + tid / 4] = of;
@@ -601,8 +620,9 @@ trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ u64 bins[TR_BINS * TR_SETS];
     __shared__ double table[TR_TABLE];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, bits = a.scale_bits;
-    const float inv_t = a.inv_t[row];
-    const int mode = tr_mode(a, sp, row);
+    const TruncRow of(a, row, false);
+    const float inv_t = of.inv_t;
+    const int mode = tr_mode(a, sp, of);
     if (!(inv_t > 0.f) || mode == TR_ALL || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
@@ -657,8 +677,9 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ unsigned short counts[TR_BUCKETS];
     __shared__ double table[TR_TABLE];
     const int part = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, bits = a.scale_bits;
-    const float inv_t = a.inv_t[row];
-    const int mode = tr_mode(a, sp, row);
+    const TruncRow of(a, row, false);
+    const float inv_t = of.inv_t;
+    const int mode = tr_mode(a, sp, of);
     if (!(inv_t > 0.f) || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
@@ -690,7 +711,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
             if (w < wave) upto += of_wave[w];
             total += of_wave[w];
         }
-        const u64 need = mode == TR_COUNT ? (u64)a.top_k[row] : tr_share(a.top_p[row], total);
+        const u64 need = mode == TR_COUNT ? (u64)of.k : tr_share(of.p, total);
         u64 run = upto - mine;
         if (run < need && need <= upto) {
 #pragma unroll
@@ -706,7 +727,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     __syncthreads();
     if (mode != TR_ALL) cut = cut_bin;
     const TruncWeights weigh(best, inv_t, bits, table);
-    const double least = tr_least(a, row);
+    const double least = tr_least(of, bits);
     // (below this no logit is in the cut's bin: a bin and a bit more, rounded down)
     const double reach = weigh.best - (4.0 * cut + 8.0) / weigh.rate;
     const float nothing = mode == TR_ALL || cut >= weigh.last_bin() ? -INFINITY : (float)(reach - 1e-6 * fabs(reach));
@@ -738,10 +759,9 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
                     for (int i = 0; i < 4; ++i) {
                         const bool stays = bin[i] < cut && x[i] >= least;
                         sum += stays ? w[i] : 0;
-                        count += stays ? 1 : 0;
+                        count += (unsigned)__popcll(__ballot(stays));
                     }
                     sum = tr_wave_sum48(sum);
-                    count = wave_prefix(count);
                 }
                 if (__any(asks[0] || asks[1] || asks[2] || asks[3])) {
 #pragma unroll
@@ -795,9 +815,10 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     __shared__ int asked, groups_in;
     const int row = blockIdx.x, tid = threadIdx.x, bits = a.scale_bits, vocab = a.vocab;
     const float *rl = a.logits + row * a.stride;
-    const float inv_t = a.inv_t[row];
+    const TruncRow of(a, row, true);
+    const float inv_t = of.inv_t, p = of.p;
     if (isnan(inv_t)) return;
-    const int mode = tr_mode(a, sp, row), groups = sp.parts * TR_GROUPS;
+    const int mode = tr_mode(a, sp, of), groups = sp.parts * TR_GROUPS;
     // everything that hangs on nothing else is asked for at once
     const bool drawn = inv_t > 0.f, sums = drawn && (mode == TR_ALL || mode == TR_WEIGHT);
     const u64 front = mode == TR_WEIGHT && drawn ? sp.sought[2 * row] : 0, sought = mode == TR_WEIGHT && drawn ? sp.sought[2 * row + 1] : 0;
@@ -825,9 +846,8 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     }
     tr_fill_table(s.table);
     const TruncWeights weigh(best, inv_t, bits, s.table);
-    const double least = tr_least(a, row);
-    const float p = a.top_p != nullptr ? a.top_p[row] : 1.f;
-    const unsigned k = mode == TR_FEW || mode == TR_COUNT ? (unsigned)a.top_k[row] : 0;
+    const double least = tr_least(of, bits);
+    const unsigned k = mode == TR_FEW || mode == TR_COUNT ? (unsigned)of.k : 0;
     u64 last = ~0ull, total = 0;            // the last place that stays
     auto weight = [&](u64 at) { return weigh.of(at); };
     if (mode == TR_FEW) {
@@ -849,12 +869,12 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         for (int i = 0; i < TOPS; ++i)
             if (tops[i] != ~0ull) atomicAdd(&s.count[step_of(tr_logit(tops[i]))], 1u);
         __syncthreads();
-        const FourSums of = tr_four(s, s.sum, s.count);
-        unsigned seen = of.count;
+        const FourSums by = tr_four(s, s.sum, s.count);
+        unsigned seen = by.count;
 #pragma unroll
         for (int i = TR_PER - 1; i >= 0; --i) {
-            if (seen - of.c[i] < k && k <= seen) s.found = tid * TR_PER + i;
-            seen -= of.c[i];
+            if (seen - by.c[i] < k && k <= seen) s.found = tid * TR_PER + i;
+            seen -= by.c[i];
         }
         __syncthreads();
         const int reach = s.found;          // (fewer than k: all of them)
@@ -911,7 +931,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     }
     if (n > TR_LIST) {
         __syncthreads();
-        trunc_whole_row(a, s, rl, row);
+        trunc_whole_row(a, s, rl, row, of);
         return;
     }
     if (mode != TR_FEW) {
@@ -952,7 +972,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         atomicAdd(&s.bucket_count[(unsigned)at / TR_BUCKET], 1u);
     }
     __syncthreads();
-    tr_draw(a, s, rl, row, TR_BUCKET, weigh, last, least);
+    tr_draw(a, s, rl, row, of.u, TR_BUCKET, weigh, last, least);
 }
 
 // How many workgroups a row gets in the first three launches, and their tokens.
