@@ -3,7 +3,7 @@
 ``libkva_hip.so``  - every ``csrc/*.hip`` file, compiled with hipcc for gfx950.
 ``libkva_host.<interpreter>.so`` - ``csrc/host/*.cpp``, C++ without a GPU runtime; one function takes Python objects,
 laid out as the interpreter that compiled it lays them out: every interpreter has a library of its own.
-``libkva_tensors.<interpreter>.so`` - ``csrc/host/torch/*.cpp``, against torch's headers, of that interpreter and torch alone; where it
+``libkva_launches.<interpreter>.so`` - ``csrc/host/torch/*.cpp``, against torch's headers, of that interpreter and torch alone; where it
 cannot be built, what it does is done in Python.
 
 Libraries are kept in ``<package>/_lib`` when that folder can be written, otherwise in a
@@ -205,11 +205,11 @@ def build_host(force: bool = False) -> str:
     return lib
 
 
-def tensors_name() -> str:
-    return f"libkva_tensors.{sysconfig.get_config_var('SOABI') or sys.implementation.cache_tag}.so"
+def launches_name() -> str:
+    return f"libkva_launches.{sysconfig.get_config_var('SOABI') or sys.implementation.cache_tag}.so"
 
 
-def build_tensors(force: bool = False) -> Optional[str]:
+def build_launches(force: bool = False) -> Optional[str]:
     """Path of an up-to-date library of ``csrc/host/torch`` for this interpreter and torch, or ``None`` where it cannot be
     built (no headers, no compiler, no folder to write to)."""
     import torch
@@ -218,7 +218,7 @@ def build_tensors(force: bool = False) -> Optional[str]:
     d = os.path.join(CSRC, "host", "torch")
     sources = sorted(os.path.join(d, f) for f in os.listdir(d) if f.endswith(".cpp"))
     flags = [*HOST_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    name, digest = tensors_name(), _digest(sources, flags + [tensors_name(), sys.version, torch.__version__, root])
+    name, digest = launches_name(), _digest(sources, flags + [launches_name(), sys.version, torch.__version__, root])
     if not force:
         cur = _find_current(name, digest)
         if cur:
@@ -231,7 +231,7 @@ def build_tensors(force: bool = False) -> Optional[str]:
         lib = os.path.join(out_dir, name)
         tmp = lib + f".tmp{os.getpid()}"
         libs = os.path.join(root, "lib")
-        _say(f"compiling the reader of tensors into {out_dir}")
+        _say(f"compiling the launches' checks into {out_dir}")
         _run([cxx, *flags, *[x for i in include for x in ("-isystem", i)], *sources, "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10",
               f"-Wl,-rpath,{libs}", "-o", tmp], "compiling " + name)
         os.replace(tmp, lib)
@@ -244,7 +244,7 @@ def build_tensors(force: bool = False) -> Optional[str]:
 
 
 def build_all(force: bool = False) -> Tuple[str, str]:
-    build_tensors(force)
+    build_launches(force)
     return build_host(force), build_hip(force)
 
 

@@ -13,7 +13,7 @@ from typing import Optional
 
 import torch
 
-from .library import KernelError, check, hip_lib, tensor_reader
+from .library import KernelError, check, hip_lib, launches
 
 F32, BF16 = 0, 1
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -1213,38 +1213,26 @@ def _at(what: str, name: str, t: Optional[torch.Tensor], dtype: torch.dtype, sha
     return t.data_ptr()
 
 
-_READER = None
+_LAUNCHES = None
 
 
-def _reader():
-    global _READER
-    if _READER is None:
-        _READER = tensor_reader() or False
-    return _READER
+def _launches(t: torch.Tensor):
+    """The native launches, which check what the functions below check and return None where they do not take a call (or False:
+    there are none, or ``t`` is not on a GPU)."""
+    global _LAUNCHES
+    if _LAUNCHES is None:
+        _LAUNCHES = launches() or False
+    return _LAUNCHES and getattr(t, "is_cuda", False) and _LAUNCHES
 
 
 def _addresses(what: str, names: str, spec: tuple) -> array:
-    """The addresses of ``spec``'s tensors, ``(device, tensor, dtype, shape, tensor, dtype, shape, ...)``, each as :func:`_at` has
-    it, all of them before :func:`_here` looks at the device; in one native call where the reader of tensors is there and nothing is wrong."""
-    out = _NO_ADDRESS * (len(spec) // 3)
-    reader = _reader()
-    if not reader or reader[0](spec, out.buffer_info()[0]) != 0:
-        for i, name in enumerate(names.split()):
-            out[i] = _at(what, name, *spec[3 * i + 1:3 * i + 4], spec[0])
-    return out
-
-
-_NO_ADDRESS = array("q", (0,))
+    """The addresses of ``spec``'s tensors, ``(device, tensor, dtype, shape, tensor, dtype, shape, ...)``, each as :func:`_at` has it."""
+    return array("q", [_at(what, name, *spec[3 * i + 1:3 * i + 4], spec[0]) for i, name in enumerate(names.split())])
 
 
 def _rows_of(what: str, name: str, t: torch.Tensor) -> tuple:
     """(address, rows, columns, elements from a row to the next, type, device) of a matrix on the GPU; the elements of a row lie next to
     each other."""
-    reader = _reader()
-    if reader:
-        out = _NO_ADDRESS * 6
-        if reader[1](t, out.buffer_info()[0]) == 0:
-            return out.tolist()
     if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.layout is not torch.strided:
         raise KernelError(f"{what}: {name} must be [rows, vocabulary]")
     (rows, cols), (stride, one) = t.shape, t.stride()
@@ -1282,6 +1270,12 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional
 
     A row that names a seat or a grammar that is not there gets -inf everywhere: no token can be taken from it."""
     what = "adjust_logits"
+    native = _launches(logits)
+    code = native.adjust_logits(logits, out, row_seat, marks, counts, repetition, presence, frequency, bias, allowed_row, allowed,
+                                _RAW_DEVICE(), _stream()) if native else None
+    if code is not None:
+        check(code, what)
+        return out
     if (marks is None) != (row_seat is None):
         raise KernelError(f"{what}: marks and the seats of the rows go together")
     if marks is None and (counts is not None or repetition is not None):
@@ -1329,6 +1323,11 @@ def count_tokens(marks: torch.Tensor, counts: Optional[torch.Tensor], seats: tor
     """``marks[seat, token] = 1`` and, with counts, ``counts[seat, token] += 1`` for every pair of ``seats`` and ``tokens`` (int32,
     as often as it is there); pairs outside the arrays are passed over."""
     what = "count_tokens"
+    native = _launches(marks)
+    code = native.count_tokens(marks, counts, seats, tokens, _RAW_DEVICE(), _stream()) if native else None
+    if code is not None:
+        check(code, what)
+        return
     if marks.dim() != 2 or tokens.dim() != 1:
         raise KernelError(f"{what}: one seat per token, marks and counts [seats, vocab]")
     rows, n, i32 = marks.shape, tokens.shape, torch.int32
@@ -1359,6 +1358,12 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
     tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
     what = "sample_truncated"
+    native = _launches(logits)
+    code = native.sample_truncated(logits, out_tokens, inv_temperature, top_k, top_p, min_p, uniform, rng_key, rng_step, kept, logprob,
+                                   host_tokens, seed, _RAW_DEVICE(), _stream()) if native else None
+    if code is not None:
+        check(code, what)
+        return out_tokens
     if inv_temperature is None:
         raise KernelError(f"{what}: inv_temperature is needed")
     if uniform is None and (rng_key is None or rng_step is None):
@@ -1397,6 +1402,11 @@ def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, le
     takes none of them and its row stays as it is; one whose seat or blocks are outside the table needs none.  No row may be
     named by two requests whose blocks overlap.  Up to 4,096 requests."""
     what = "grow_tables"
+    native = _launches(table)
+    code = native.grow_tables(table, seats, held, lengths, pages, offsets, page_size, _RAW_DEVICE(), _stream()) if native and offsets is not None else None
+    if code is not None:
+        check(code, what)
+        return offsets
     if seats.dim() != 1 or pages.dim() != 1 or table.dim() != 2:
         raise KernelError(f"{what}: a table [rows, blocks], a seat, held blocks and a length per request, and a row of pages")
     n, size, i32, entries = seats.shape, table.shape, torch.int32, seats.shape[0]
@@ -1421,6 +1431,11 @@ def step_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, 
     to 8 groups), -1 where no page is mapped, or the position or the seat is outside the table.  Rows behind the last entry's are left
     as they were, and rows that the arrays have no room for are not made.  Everything is int32; up to 4,096 entries."""
     what = "step_rows"
+    native = _launches(lengths)
+    code = native.step_rows(lengths, starts, seats, tables, page_size, q_start, positions, tok_seat, slots, _RAW_DEVICE(), _stream()) if native else None
+    if code is not None:
+        check(code, what)
+        return
     if lengths.dim() != 1 or positions.dim() != 1 or len(slots) != len(tables) or any(t.dim() != 2 for t in tables):
         raise KernelError(f"{what}: a length per entry, a position per token, tables [rows, blocks] and as many arrays of slots")
     n, tokens, i32 = lengths.shape, positions.shape, torch.int32

@@ -7,6 +7,8 @@ allocator library, which needs no GPU.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_uint, c_void_p, POINTER
 
@@ -260,23 +262,24 @@ def sample_rows():
     return _sample_rows or None
 
 
-_tensor_reader = None
+_launches = None
 
 
-def tensor_reader():
-    """``(kva_tensor_args, kva_tensor_rows)`` of the reader of tensors (they take Python objects and are called with the
-    interpreter's lock held), or None where it was not built."""
-    global _tensor_reader
-    if _tensor_reader is None:
-        path = build.build_tensors()
-        try:
-            lib = ctypes.PyDLL(path) if path else None
-        except OSError:
-            lib = None
-        if lib is None:
-            _tensor_reader = False
-        else:
-            lib.kva_tensor_args.argtypes, lib.kva_tensor_args.restype = [ctypes.py_object, LL], LL
-            lib.kva_tensor_rows.argtypes, lib.kva_tensor_rows.restype = [ctypes.py_object, LL], LL
-            _tensor_reader = (lib.kva_tensor_args, lib.kva_tensor_rows)
-    return _tensor_reader or None
+def launches():
+    """The module of native launches (``csrc/host/torch/launches.cpp``), bound to the kernel library's entries, or None where it
+    was not built."""
+    global _launches
+    if _launches is None:
+        lib, module = hip_lib(), False
+        path = build.build_launches()
+        if path:
+            try:
+                loader = importlib.machinery.ExtensionFileLoader("kva_launches", path)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("kva_launches", path, loader=loader))
+                module.bind(*[ctypes.cast(getattr(lib, name), c_void_p).value for name in (
+                    "kva_adjust_logits", "kva_count_tokens", "kva_sample_truncated", "kva_sample_truncated_workspace_bytes", "kva_grow_tables",
+                    "kva_step_rows")])
+            except ImportError:
+                module = False
+        _launches = module
+    return _launches or None

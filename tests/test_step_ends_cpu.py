@@ -8,7 +8,7 @@ import torch
 
 import plain_step_ends as plain
 from kv_cache_optimization_for_llm_amd.ops import kernels as K
-from kv_cache_optimization_for_llm_amd.ops.library import KernelError, check, hip_lib, tensor_reader
+from kv_cache_optimization_for_llm_amd.ops.library import KernelError, check, hip_lib, launches
 
 
 def i32(*shape):
@@ -155,22 +155,23 @@ def test_refusals_say_why(message, call):
         call()
 
 
-def test_the_reader_of_tensors_takes_gpu_tensors_only():
-    """Whatever it does not know goes to the checks in Python: wrong objects, tensors of the host, odd lists."""
-    reader = tensor_reader()
-    assert reader is not None, "torch's headers are here: it has to build"
-    args, rows = reader
-    out = array("q", [7] * 6)
-    at = out.buffer_info()[0]
-    assert args((0,), at) == 0
-    assert args((0, None, torch.int32, (3,)), at) == 0 and out[0] == 0
-    assert args((-1, i32(3), torch.int32, (3,)), at) != 0
-    assert args((0, None, torch.int32, (3,), i32(3), torch.int32, (3,)), at) == 2
-    for bad in ((0, 5, torch.int32, (3,)), (0, i32(3), "int32", (3,)), (0, i32(3), torch.int32, 3), (0, i32(3), torch.int32, ("a",)),
-                ("a",), (0, i32(3)), [0], None, (1 << 80,)):
-        assert args(bad, at) != 0
-    for bad in (f32(3, 4), None, 5, f32(3)):
-        assert rows(bad, at) != 0
+def test_native_launches_take_gpu_tensors_only():
+    """Whatever they do not take goes to the checks in Python: too few arguments, wrong objects, tensors of the host."""
+    native = launches()
+    assert native is not None, "torch's headers are here: it has to build"
+    calls = dict(adjust_logits=[f32(2, 40), f32(2, 40), i32(2), marks(3, 40), i32(3, 40), f32(2), f32(2), f32(2), (i32(3), i32(5), f32(5)), i32(2), i32(1, 2)],
+                 count_tokens=[marks(3, 40), i32(3, 40), i32(5), i32(5)],
+                 sample_truncated=[f32(2, 40), i32(2), f32(2), i32(2), f32(2), f32(2), f32(2), None, None, i32(2), f32(2), None, 0],
+                 grow_tables=[i32(3, 4), i32(2), i32(2), i32(2), i32(9), i32(3), 16],
+                 step_rows=[i32(2), i32(2), i32(2), [i32(3, 4)], 16, i32(3), i32(5), i32(5), [i32(5)]])
+    for name, args in calls.items():
+        call = getattr(native, name)
+        assert call(*args, 0, 0) is None and call(*args, -1, 0) is None and call(*args) is None and call() is None
+        for i in range(len(args)):
+            for other in (None, 5, "a", 1 << 80, [], (1, 2), object()):
+                assert call(*args[:i], other, *args[i + 1:], 0, 0) is None, (name, i)
+    with pytest.raises(TypeError):
+        native.bind(1, 2)
 
 
 def test_a_launch_needs_its_tensors():

@@ -449,9 +449,11 @@ def test_a_step_in_a_graph(gpu):
 # ---------------------------------------------------------------- calls that a user may make
 @pytest.mark.parametrize("native", [True, False])
 def test_refusals_on_the_gpu(gpu, native, monkeypatch):
-    """The native check of the tensors and the one in Python refuse the same calls for the same reasons, and pass the same."""
+    """The native checks and those in Python refuse the same calls for the same reasons, and pass the same."""
     if not native:
-        monkeypatch.setattr(K, "_READER", False)
+        monkeypatch.setattr(K, "_LAUNCHES", False)
+    else:
+        assert K._launches(torch.zeros(1, device=gpu))
     i = lambda *s: torch.zeros(s, dtype=torch.int32, device=gpu)
     f = lambda *s: torch.zeros(s, device=gpu)
     m = lambda *s: torch.zeros(s, dtype=torch.uint8, device=gpu)
