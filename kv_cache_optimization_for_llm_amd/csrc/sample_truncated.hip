@@ -564,11 +564,11 @@ __device__ inline void tr_load_step(const float *rl, int t0, int vocab, float (&
     }
 }
 
-// The best place of a row, from its parts' (every wavefront for itself).
-__device__ inline u64 tr_best(const TruncSpace &sp, int row) {
-    u64 at = ~0ull;
-    for (int c = threadIdx.x % KVA_WAVE; c < sp.parts; c += KVA_WAVE) at = min(at, sp.best[(size_t)row * sp.parts + c]);
-    return tr_wave_min(at);
+// The best place of a row, from its parts' (every wavefront for itself): asked for first, found later.
+static_assert(TR_MAX_PARTS <= KVA_WAVE, "a lane a part");
+__device__ inline u64 tr_part_best(const TruncSpace &sp, int row) {
+    const int part = threadIdx.x % KVA_WAVE;
+    return part < sp.parts ? sp.best[(size_t)row * sp.parts + part] : ~0ull;
 }
 
 // grid (parts, rows)
@@ -626,11 +626,12 @@ trunc_bins_kernel(TruncArgs a, TruncSpace sp) {
     if (!(inv_t > 0.f) || mode == TR_ALL || mode == TR_FEW) return;
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
+    const u64 part_best = tr_part_best(sp, row);
     float l[4];
     tr_load_step(rl, part * sp.part_tokens, a.vocab, l);
     for (int i = tid; i < TR_BINS * TR_SETS; i += TR_SPLIT_THREADS) bins[i] = 0;
     tr_fill_table(table);
-    const u64 at = tr_best(sp, row);
+    const u64 at = tr_wave_min(part_best);
     if (at == ~0ull) return;
     const float best = tr_logit(at);
     const TruncWeights weigh(best, inv_t, bits, table);
@@ -684,6 +685,7 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
     const float *rl = a.logits + row * a.stride;
     const int end = min(a.vocab, (part + 1) * sp.part_tokens);
     int t0 = part * sp.part_tokens;
+    const u64 part_best = tr_part_best(sp, row);
     float l[4];
     tr_load_step(rl, t0, a.vocab, l);
     u64 v[PER] = {};
@@ -691,12 +693,12 @@ trunc_collect_kernel(TruncArgs a, TruncSpace sp) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) v[i] = sp.bins[(size_t)row * TR_BINS + tid * PER + i];
     }
-    const u64 at = tr_best(sp, row);
+    tr_fill_table(table);
+    const u64 at = tr_wave_min(part_best);
     if (at == ~0ull) return;
     const float best = tr_logit(at);
     if (!(best < INFINITY)) return;
     int cut = TR_BINS;                      // the bin in which the cut lies; past the last: everything stays
-    tr_fill_table(table);
     if (mode != TR_ALL) {
         u64 mine = 0;
 #pragma unroll
@@ -820,6 +822,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
     if (isnan(inv_t)) return;
     const int mode = tr_mode(a, sp, of), groups = sp.parts * TR_GROUPS;
     // everything that hangs on nothing else is asked for at once
+    const u64 part_best = tr_part_best(sp, row);
     const bool drawn = inv_t > 0.f, sums = drawn && (mode == TR_ALL || mode == TR_WEIGHT);
     const u64 front = mode == TR_WEIGHT && drawn ? sp.sought[2 * row] : 0, sought = mode == TR_WEIGHT && drawn ? sp.sought[2 * row + 1] : 0;
     int n = drawn ? sp.listed[row] : 0;
@@ -830,6 +833,7 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         for (int i = 0; i < TOPS; ++i)
             tops[i] = tid + i * TR_THREADS < groups ? sp.tops[(size_t)row * groups + tid + i * TR_THREADS] : ~0ull;
     }
+    tr_fill_table(s.table);
 #pragma unroll
     for (int i = 0; i < TR_BUCKETS / TR_THREADS; ++i) {
         const int b = tid + i * TR_THREADS;
@@ -837,14 +841,13 @@ trunc_pick_kernel(TruncArgs a, TruncSpace sp) {
         s.bucket_sum[b] = on ? sp.sums[(size_t)row * sp.buckets + b] : 0;
         s.bucket_count[b] = on ? sp.counts[(size_t)row * sp.buckets + b] : 0;
     }
-    const u64 first = tr_best(sp, row);
+    const u64 first = tr_wave_min(part_best);
     const float best = first == ~0ull ? 0.f : tr_logit(first);
     TruncResult r;
     if (tr_decided(first, best, inv_t, r)) {
         if (tid == 0) r.store(a, row);
         return;
     }
-    tr_fill_table(s.table);
     const TruncWeights weigh(best, inv_t, bits, s.table);
     const double least = tr_least(of, bits);
     const unsigned k = mode == TR_FEW || mode == TR_COUNT ? (unsigned)of.k : 0;
