@@ -1352,11 +1352,11 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
        [0, 1)) or, without it, the number that :func:`sample` draws for (``seed``, ``rng_key``, ``rng_step``).
 
     Weights are held to 2^-45 of the best one's for vocabularies of up to 131,072 (half as finely for every doubling) and added up
-    exactly; tokens of less than half of that keep their place in the order and are never drawn, and a ``min_p`` below an eighth of it is
-    none.  Rows whose ``inv_temperature`` is
-    not above 0 take the best token, and rows where it is no number are passed over: what stands in the outputs stays.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability among
-    them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1, no
-    tokens and -inf.  ``host_tokens`` as in :func:`sample`."""
+    exactly; tokens of less than half of that keep their place in the order and are never drawn, and a ``min_p`` below an eighth of
+    it is none.  Rows whose ``inv_temperature`` is not above 0 take the best token, and rows where it is no number are passed over:
+    what stands in the outputs stays.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability
+    among them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1,
+    no tokens and -inf.  Vocabularies of up to 2^24.  ``host_tokens`` as in :func:`sample`."""
     what = "sample_truncated"
     native = _launches(logits)
     code = native.sample_truncated(logits, out_tokens, inv_temperature, top_k, top_p, min_p, uniform, rng_key, rng_step, kept, logprob,

@@ -564,3 +564,61 @@ def test_two_graphs_of_draws(gpu):
             K.sample_truncated(x, eager, top_k=torch.full((rows,), 5 + 60 * i, dtype=torch.int32, device=gpu), **kw)
             torch.cuda.synchronize()
             assert torch.equal(outs[i], eager)
+
+
+def test_sample_truncated_largest_vocabulary(gpu):
+    """2^24 tokens and not one more; weights are held to 2^-37 there."""
+    rng = np.random.default_rng(24)
+    vocab = 1 << 24
+    x = (rng.standard_normal((2, vocab)) * 2).astype(np.float32)
+    x[:, rng.integers(0, vocab, 50)] = rng.uniform(11, 16, 50)
+    got = draw_on(gpu, x, np.full(2, 0.9, np.float32), [0, 1000], np.asarray([0.3, 0.8], np.float32), [0, 0], np.asarray([0.25, 0.9], np.float32))
+    for r, (k, p, u) in enumerate(((0, 0.3, 0.25), (1000, 0.8, 0.9))):
+        token, n, lp = plain.truncated(x[r], np.float32(0.9), k, float(np.float32(p)), 0, float(np.float32(u)))
+        assert (int(got[0][r]), int(got[1][r])) == (token, n)
+        assert abs(float(got[2][r]) - lp) <= 2.0 ** -24 * abs(lp) + 2.0 ** -37 * vocab       # (a rounding, and vocab weights of 2^-38 of the best one's)
+    one = torch.zeros(1, dtype=torch.int32, device=gpu)
+    with pytest.raises(KernelError):
+        K.sample_truncated(torch.zeros(1, vocab + 1, device=gpu), one, inv_temperature=torch.ones(1, device=gpu), uniform=torch.zeros(1, device=gpu))
+
+
+@pytest.mark.parametrize("vocab", [700, 9000])
+def test_sample_truncated_odd_uniform_numbers(gpu, vocab):
+    """Numbers outside [0, 1) and no numbers draw the first or the last token that stays, never one that does not."""
+    x = np.zeros((6, vocab), np.float32)
+    x[:, 100], x[:, 600] = 3, 4
+    u = np.asarray([-1, math.nan, -math.inf, 1, 7, math.inf], np.float32)
+    tokens, kept, _ = draw_on(gpu, x, np.ones(6, np.float32), np.full(6, 2), np.ones(6), np.zeros(6), u)
+    assert tokens.tolist() == [100] * 3 + [600] * 3 and kept.tolist() == [2] * 6
+
+
+def test_rows_past_2_31_elements(gpu):
+    """17,000 rows of 128,256: the last ones begin behind 2^31 elements, and are what they are alone."""
+    rows, vocab, seats = 17000, 128256, 17001
+    g = torch.Generator(device=gpu)
+    g.manual_seed(3)
+    last = torch.randn(3, vocab, generator=g, device=gpu) * 3
+    logits = torch.zeros(rows, vocab, dtype=torch.bfloat16, device=gpu)
+    logits[-3:] = last
+    marks, counts = torch.zeros(seats, vocab, dtype=torch.uint8, device=gpu), torch.zeros(seats, vocab, dtype=torch.int32, device=gpu)
+    tokens = torch.randint(0, vocab, (3 * 500,), generator=g, device=gpu).int()
+    K.count_tokens(marks, counts, torch.arange(3, device=gpu).repeat_interleave(500).int() + (seats - 3), tokens)
+    assert counts[-3:].sum().item() == 1500 and counts[:-3].any().item() is False
+    row_seat = torch.arange(rows, device=gpu).int() + 1
+    one = torch.full((rows,), 1.5, device=gpu)
+    out = torch.empty(rows, vocab, device=gpu)
+    K.adjust_logits(logits, out, row_seat=row_seat, marks=marks, counts=counts, repetition=one, presence=one, frequency=one)
+    alone = torch.empty(3, vocab, device=gpu)
+    K.adjust_logits(logits[-3:], alone, row_seat=torch.arange(3, device=gpu).int(), marks=marks[-3:].clone(), counts=counts[-3:].clone(),
+                    repetition=one[:3], presence=one[:3], frequency=one[:3])
+    assert torch.equal(out[-3:], alone) and not torch.equal(alone, logits[-3:].float())
+    assert (out[:-3] == 0).all()
+    u = torch.rand(rows, generator=g, device=gpu)
+    p, inv_t = torch.full((rows,), 0.9, device=gpu), torch.full((rows,), 0.8, device=gpu)
+    inv_t[:-3] = 0                                  # (greedy, but for the last)
+    drawn, kept = torch.empty(rows, dtype=torch.int32, device=gpu), torch.empty(rows, dtype=torch.int32, device=gpu)
+    K.sample_truncated(out, drawn, inv_temperature=inv_t, top_p=p, uniform=u, kept=kept)
+    few, few_kept = torch.empty(3, dtype=torch.int32, device=gpu), torch.empty(3, dtype=torch.int32, device=gpu)
+    K.sample_truncated(alone, few, inv_temperature=inv_t[-3:], top_p=p[-3:], uniform=u[-3:], kept=few_kept)
+    assert torch.equal(drawn[-3:], few) and torch.equal(kept[-3:], few_kept) and (kept[-3:] > 1).all()
+    assert (drawn[:-3] == 0).all() and (kept[:-3] == 1).all()
