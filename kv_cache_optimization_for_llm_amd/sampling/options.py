@@ -22,8 +22,8 @@ class SampleOptions:
     """``repetition_penalty``: None is the server's.  ``penalize_prompt``: the repetition penalty takes the prompt's tokens as emitted
     ones, too (the other two count what the request itself has said).  ``logit_bias``: token id -> what its logit gains (-inf bans it).
     ``grammar``: called with the tokens emitted so far before every token, says which ones may come next - None (all of them), a
-    truth value per token of the vocabulary, ids, or what :func:`pack_allowed` makes of them; a step that needs its answer waits for the
-    tokens of the step before.  A request of whose vocabulary nothing is left ends with the error ``invalid_logits``."""
+    truth value per token of the vocabulary, ids, or what :func:`pack_allowed` makes of them (:class:`AllowedWords`); a step that needs its
+    answer waits for the tokens of the step before.  A request of whose vocabulary nothing is left ends with the error ``invalid_logits``."""
 
     top_k: int = 0                                  # 0: all tokens
     top_p: float = 1.0
@@ -62,12 +62,28 @@ class SampleOptions:
         return (self.repetition_penalty not in (None, 1.0) or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0)
 
 
-def pack_allowed(allowed, vocab_size: int) -> Optional[np.ndarray]:
-    """int32 words of 32 tokens each (bit ``token % 32`` of word ``token / 32``) from a truth value per token, from token ids, or from
-    such words (an int32 or uint32 array of that length); ``None`` stays: everything is allowed."""
+class AllowedWords(np.ndarray):
+    """Allowed tokens as int32 words of 32 each (bit ``token % 32`` of word ``token / 32``): what :func:`pack_allowed` returns, or made of a
+    row of int32 or uint32 words.  Words say by their class that they are; every other array of whole numbers is a row of ids, whatever its
+    length."""
+
+    def __new__(cls, words):
+        a = np.asarray(words)
+        if a.ndim != 1 or a.dtype not in (np.int32, np.uint32):
+            raise ValueError("allowed words are a row of int32 or uint32")
+        return a.view(np.int32).view(cls)
+
+
+def pack_allowed(allowed, vocab_size: int) -> Optional[AllowedWords]:
+    """Words of 32 tokens each from a truth value per token, from token ids, or from such words (:class:`AllowedWords`); ``None`` stays:
+    everything is allowed."""
     if allowed is None:
         return None
     words = (vocab_size + 31) // 32
+    if isinstance(allowed, AllowedWords):
+        if allowed.shape != (words,) or allowed.dtype not in (np.int32, np.uint32):
+            raise ValueError(f"allowed words {allowed.shape} {allowed.dtype} are not {words} of 32 tokens each")
+        return allowed.view(np.int32)
     a = allowed if isinstance(allowed, np.ndarray) else np.asarray(list(allowed))
     if a.ndim != 1:
         raise ValueError("allowed tokens are a row of ids, of truth values, or of packed words")
@@ -76,9 +92,7 @@ def pack_allowed(allowed, vocab_size: int) -> Optional[np.ndarray]:
             raise ValueError(f"{a.shape[0]} truth values for a vocabulary of {vocab_size}")
         bits = np.zeros(words * 32, dtype=np.uint8)
         bits[:vocab_size] = a
-        return np.packbits(bits, bitorder="little").view(np.int32)
-    if isinstance(allowed, np.ndarray) and a.dtype in (np.int32, np.uint32) and a.shape[0] == words:
-        return a.view(np.int32)
+        return AllowedWords(np.packbits(bits, bitorder="little").view(np.int32))
     if a.shape[0] and not np.issubdtype(a.dtype, np.integer):
         raise ValueError("token ids must be whole numbers")
     ids = a.astype(np.int64)
@@ -86,4 +100,4 @@ def pack_allowed(allowed, vocab_size: int) -> Optional[np.ndarray]:
         raise ValueError(f"an allowed token is outside [0, {vocab_size})")
     bits = np.zeros(words * 32, dtype=np.uint8)
     bits[ids] = 1
-    return np.packbits(bits, bitorder="little").view(np.int32)
+    return AllowedWords(np.packbits(bits, bitorder="little").view(np.int32))

@@ -7,7 +7,7 @@ import pytest
 from kv_cache_optimization_for_llm_amd.cache.manager import CacheError, CacheManager
 from kv_cache_optimization_for_llm_amd.engine.scheduler import Request, Scheduler
 from kv_cache_optimization_for_llm_amd.parts.base import attention_cache_spec
-from kv_cache_optimization_for_llm_amd.sampling.options import SampleOptions, pack_allowed
+from kv_cache_optimization_for_llm_amd.sampling.options import AllowedWords, SampleOptions, pack_allowed
 
 
 @pytest.mark.parametrize("bad", [
@@ -88,3 +88,26 @@ def test_numbers_that_32_bits_do_not_hold_are_refused(bad):
 
 def test_a_ban_may_be_as_low_as_it_likes():
     assert SampleOptions(logit_bias={3: -1e300, 4: -float("inf")}).logit_bias[4] == -float("inf")
+
+
+@pytest.mark.parametrize("dtype", [np.int8, np.int16, np.int32, np.uint32, np.int64])
+def test_ids_of_any_type_and_number_are_ids(dtype):
+    """Also exactly as many as there are words of 32 tokens."""
+    for vocab, ids in ((20, [3]), (64, [3, 5]), (100, [0, 1, 2, 99]), (128, [3, 5, 7, 9]), (128, [1, 1, 2, 127])):
+        want = pack_allowed(sorted(set(ids)), vocab)
+        assert len(ids) == len(want) and np.array_equal(pack_allowed(np.asarray(ids, dtype), vocab), want)
+
+
+def test_words_say_that_they_are():
+    words = np.asarray([0b1010, -2], np.int32)
+    free = [t in (1, 3) or 33 <= t for t in range(64)]
+    for given in (AllowedWords(words), AllowedWords(words.view(np.uint32)), AllowedWords(np.repeat(words, 2)[::2])):
+        assert np.array_equal(pack_allowed(given, 64), pack_allowed(free, 64))
+    for vocab in (32, 65):
+        with pytest.raises(ValueError):
+            pack_allowed(AllowedWords(words), vocab)
+    with pytest.raises(ValueError):
+        pack_allowed(AllowedWords(words).astype(np.int64), 64)
+    for bad in (words.astype(np.int64), words[None], [1.5, 2]):
+        with pytest.raises(ValueError):
+            AllowedWords(bad)
