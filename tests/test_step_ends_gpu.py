@@ -622,3 +622,38 @@ def test_rows_past_2_31_elements(gpu):
     K.sample_truncated(alone, few, inv_temperature=inv_t[-3:], top_p=p[-3:], uniform=u[-3:], kept=few_kept)
     assert torch.equal(drawn[-3:], few) and torch.equal(kept[-3:], few_kept) and (kept[-3:] > 1).all()
     assert (drawn[:-3] == 0).all() and (kept[:-3] == 1).all()
+
+
+def near_borders(rng, least, most):
+    """(logit of the second token below the first's 0, inverse temperature, number, whether the number is above the first's share): pairs
+    whose first one's share of both weights lies ``least`` to ``most`` beside a number of 24 bits."""
+    below, inv_t = rng.uniform(0.2, 2.5, 1 << 24).astype(np.float32), rng.uniform(0.4, 1.6, 1 << 24).astype(np.float32)
+    part = (below * inv_t.astype(np.float64)) * (128 / math.log(2)) % 1
+    hard = np.abs(part - 0.5) < 0.1             # (between two of a table's powers of 2^(1/128), where a series is worst)
+    below, inv_t = below[hard], inv_t[hard]
+    share = 1 / (1 + np.exp(-below.astype(np.longdouble) * inv_t.astype(np.longdouble)))        # (80 bits)
+    u = np.round(share * 2 ** 24) / 2 ** 24
+    far = np.abs(u - share)
+    on = np.nonzero((far > least) & (far < most))[0]
+    return -below[on], inv_t[on], u[on].astype(np.float32), (u > share)[on]
+
+
+@pytest.mark.parametrize("vocab", [40, 5000, 60000, 131072])
+def test_weights_are_as_exact_as_stated(gpu, vocab):
+    """Two tokens and a border within 2e-13 of a number: a weight off by 2^-45 of the best one's moves the first one's share by w0 / (w0 +
+    w1)^2 of that, below 2^-45, and the number times the sum of both is rounded by 2^-53 of it; what is further away than 4e-14 (2^-45 is
+    2.9e-14) falls on the side that 80 bits have it on."""
+    second, inv_t, u, above = near_borders(np.random.default_rng(11), 4e-14, 2e-13)
+    n = len(u)
+    assert n >= 16 and 4 <= above.sum() <= n - 4
+    x = np.full((n, vocab), -np.inf, np.float32)
+    a, b = vocab // 3, vocab - 2
+    x[:, a], x[:, b] = 0, second
+    none = np.zeros(n)
+    tokens, kept, _ = draw_on(gpu, x, inv_t, none, none + 1, none, u)
+    assert (kept == 2).all() and np.array_equal(tokens.numpy(), np.where(above, b, a))         # the first whose sum exceeds u S
+    tokens, kept, _ = draw_on(gpu, x, inv_t, none, u, none, none)
+    assert np.array_equal(kept.numpy(), np.where(above, 2, 1)) and (tokens == a).all()         # the shortest with at least p S
+    x[:, 7] = -200                                                                             # (nothing, behind both)
+    kept = draw_on(gpu, x, inv_t, none + 2, u, none, none)[1]
+    assert np.array_equal(kept.numpy(), np.where(above, 2, 1))
