@@ -4,6 +4,8 @@ from __future__ import annotations
 from dataclasses import dataclass, replace
 from typing import Dict, Iterable, List, Optional, Sequence, Union
 
+import torch
+
 from ..sampling.options import SampleOptions, pack_allowed
 from ..sampling.sampler import OptionRow, SampleRow, Sampler
 from .batch import StepEntry
@@ -73,7 +75,9 @@ class Runner:
     def _on_release(self, seq) -> None:
         if seq.request.options is not None:
             self._grammars -= seq.request.options.grammar is not None
-        self.engine.unbind_request(engine_key(seq.request))
+        key = engine_key(seq.request)
+        if self.engine.has_request(key) and self.engine.seat_of(key) == seq.seat:
+            self.engine.unbind_request(key)         # (a request whose name was another's stays out of that one's way)
 
     def submit(self, tokens: Sequence[int], max_new_tokens: int, *, request_id: Optional[int] = None,
                n_seqs: int = 1, temperature: Optional[float] = None, options: Optional[SampleOptions] = None) -> int:
@@ -104,6 +108,17 @@ class Runner:
         events, self._kept = self._kept, []
         events.extend(self._resolve_in_flight())
         events.extend(self.scheduler.cancel(request_id))
+        return events
+
+    def cancel_all(self) -> List[Event]:
+        """Ends every request (:meth:`cancel`) and waits until the device is done with what was launched for them: behind it the
+        engine is as it was before they came, and this runner may go."""
+        events: List[Event] = []
+        for request_id in self.live_requests():
+            events.extend(self.cancel(request_id))
+        events.extend(self._kept + self._resolve_in_flight())
+        self._kept = []
+        torch.cuda.current_stream(self.engine.device).synchronize()
         return events
 
     def live_requests(self) -> List[int]:
@@ -205,7 +220,8 @@ class LLM:
                  ignore_eos: Optional[bool] = None, repetition_penalty: Optional[float] = None,
                  options: Union[None, SampleOptions, Sequence[Optional[SampleOptions]]] = None, return_reasons: bool = False):
         """Generates for every prompt (token ids in, token ids out), batched continuously.  ``options``: what the requests ask of
-        their sampling, one for all of them or one each (None: the server's)."""
+        their sampling, one for all of them or one each (None: the server's).  What a grammar raises comes out of here; no request of
+        the call is left behind then."""
         opts = ServeOptions(**vars(self.serve_options))
         if temperature is not None:
             opts.temperature = temperature
@@ -222,11 +238,15 @@ class LLM:
         ids = [runner.submit(p, max_new_tokens, options=o) for p, o in zip(prompts, each)]
         out: Dict[int, List[int]] = {i: [] for i in ids}
         reasons: Dict[int, str] = {}
-        for ev in runner.run_until_idle():
-            if ev.kind == "token":
-                out[ev.request_id].append(ev.token)
-            elif ev.kind in ("done", "rejected"):
-                reasons[ev.request_id] = ev.reason
+        try:
+            for ev in runner.run_until_idle():
+                if ev.kind == "token":
+                    out[ev.request_id].append(ev.token)
+                elif ev.kind in ("done", "rejected"):
+                    reasons[ev.request_id] = ev.reason
+        except BaseException:
+            runner.cancel_all()
+            raise
         self.last_runner = runner
         results = [out[i] for i in ids]
         return (results, [reasons.get(i) for i in ids]) if return_reasons else results

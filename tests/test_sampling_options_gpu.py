@@ -9,7 +9,7 @@ import plain_llama as plain
 import plain_step_ends as ends
 from kv_cache_optimization_for_llm_amd.cache.manager import CacheManager
 from kv_cache_optimization_for_llm_amd.engine.batch import build_batch
-from kv_cache_optimization_for_llm_amd.engine.engine import EngineOptions
+from kv_cache_optimization_for_llm_amd.engine.engine import EngineError, EngineOptions
 from kv_cache_optimization_for_llm_amd.engine.runner import LLM, Runner, ServeOptions
 from kv_cache_optimization_for_llm_amd.parts.base import attention_cache_spec
 from kv_cache_optimization_for_llm_amd.sampling.options import SampleOptions, pack_allowed
@@ -269,3 +269,61 @@ def test_steps_of_more_entries_than_a_launch_takes(model_dirs, gpu, dtype, monke
     few = LLM(model_dirs["A"], EngineOptions(dtype=dtype, max_seqs=4, max_seq_len=64))
     assert few.generate(prompts, 10, ignore_eos=True) == want
     few.engine.cache.check()
+
+
+# ---------------------------------------------------------------- what a grammar raises
+@pytest.mark.parametrize("ahead", [False, True])
+@pytest.mark.parametrize("at", [0, 1, 5])
+def test_generation_goes_on_after_a_grammar_that_raised(model_dirs, gpu, at, ahead):
+    """Out of generate, too: seats, pages and names come back, whatever was in flight."""
+    llm = LLM(model_dirs["A"], EngineOptions(dtype="bfloat16", max_seqs=3, max_seq_len=64), ServeOptions(run_ahead=ahead))
+    prompts = prompts_for(256, [5, 30, 9, 12, 7], 2)
+    want = llm.generate(prompts, 8, ignore_eos=True, temperature=0.7, seed=4)
+
+    def raises(out):
+        if len(out) == at:
+            raise KeyError("no such state")
+
+    def misnames(out):
+        return [3, 256] if len(out) == at else None
+    for grammar, error in ((raises, KeyError), (misnames, ValueError)):
+        for place in (0, 4):            # in the first steps, and in a seat that another request had
+            options = [SampleOptions(grammar=grammar) if i == place else None for i in range(5)]
+            with pytest.raises(error):
+                llm.generate(prompts, 8, ignore_eos=True, temperature=0.7, seed=4, options=options)
+            cache = llm.engine.cache
+            assert cache.free_seats == 3 and all(g.free_pages() == g.num_pages for g in cache.groups)
+            cache.check()
+            assert llm.generate(prompts, 8, ignore_eos=True, temperature=0.7, seed=4) == want
+
+
+def test_generate_leaves_another_runners_requests_alone(model_dirs, gpu):
+    """A call whose requests would have names that are taken is refused, and the one that has the name goes on."""
+    llm = LLM(model_dirs["A"], EngineOptions(dtype="bfloat16", max_seqs=3, max_seq_len=64))
+    prompts = prompts_for(256, [5, 9], 2)
+    want = llm.generate(prompts, 8, ignore_eos=True)
+    runner = Runner(llm.engine, ServeOptions(ignore_eos=True))
+    assert [runner.submit(p, 8) for p in prompts] == [0, 1]
+    events = runner.step()
+    with pytest.raises(EngineError):
+        llm.generate(prompts, 8, ignore_eos=True)
+    assert llm.engine.cache.free_seats == 1
+    while not runner.idle():
+        events += runner.step()
+    assert [[e.token for e in events if e.kind == "token" and e.request_id == i] for i in (0, 1)] == want
+    llm.engine.cache.check()
+
+
+def test_cancel_all(model_dirs, gpu):
+    llm = LLM(model_dirs["A"], EngineOptions(dtype="bfloat16", max_seqs=2, max_seq_len=64))
+    prompts = prompts_for(256, [5, 9, 4], 2)
+    want = llm.generate(prompts[:1], 8, ignore_eos=True)
+    runner = Runner(llm.engine, ServeOptions(ignore_eos=True))
+    assert runner.cancel_all() == []
+    for p in prompts:
+        runner.submit(p, 8)
+    events = runner.step() + runner.step() + runner.cancel_all()
+    assert sorted(e.request_id for e in events if e.kind == "done" and e.reason == "cancelled") == [0, 1, 2] and runner.idle()
+    assert [e.token for e in events if e.kind == "token" and e.request_id == 0] == want[0][:2]
+    assert llm.engine.cache.free_seats == 2
+    llm.engine.cache.check()
