@@ -375,7 +375,8 @@ class CacheManager:
     def check_mapped(self, seat: int, start: int, count: int, group: int) -> None:
         """Raises unless positions ``start .. start + count - 1`` have a page."""
         g = self.groups[group]
-        if count > 0 and (g.table_host[seat, start // self.page_size:(start + count - 1) // self.page_size + 1] < 0).any():
+        lo, hi = start // self.page_size, (start + count - 1) // self.page_size + 1
+        if count > 0 and (lo < 0 or hi > self.max_blocks or (g.table_host[seat, lo:hi] < 0).any()):
             raise CacheError(f"seat {seat}: positions {start}..{start + count - 1} are not all mapped "
                              f"in group {group}")
 

@@ -111,3 +111,15 @@ def test_words_say_that_they_are():
     for bad in (words.astype(np.int64), words[None], [1.5, 2]):
         with pytest.raises(ValueError):
             AllowedWords(bad)
+
+
+def test_positions_outside_the_table_are_refused():
+    m = cache(max_len=62)               # 16 blocks of 4
+    seat = m.admit("a")
+    assert m.grow(seat, 62)
+    m.check_mapped(seat, 0, 64, 0)
+    m.check_mapped(seat, 63, 1, 0)
+    m.check_mapped(seat, 64, 0, 0)
+    for start, count in ((60, 5), (60, 10), (64, 1), (100, 3), (-1, 1), (-1, 64), (-8, 2), (0, 1 << 40)):
+        with pytest.raises(CacheError):
+            m.check_mapped(seat, start, count, 0)
