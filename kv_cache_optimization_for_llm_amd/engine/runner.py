@@ -63,13 +63,14 @@ class Runner:
 
     # the scheduler owns seats; the engine only needs to know which request sits where
     def _on_admit(self, seq) -> None:
-        self.engine.bind_request(engine_key(seq.request), seq.seat)
         options = seq.request.options
+        if options is not None:
+            self._grammars += options.grammar is not None       # (in front of what may raise: _on_release counts it down in any case)
+        self.engine.bind_request(engine_key(seq.request), seq.seat)
         emitted = seq.prompt[len(seq.prompt) - seq.request.resumed_tokens:] if seq.request.resumed_tokens else ()
         if options is None:
             self.sampler.reset_seat(seq.seat, emitted)
         else:
-            self._grammars += options.grammar is not None
             self.sampler.reset_seat(seq.seat, emitted, seq.prompt[:len(seq.prompt) - seq.request.resumed_tokens], options)
 
     def _on_release(self, seq) -> None:

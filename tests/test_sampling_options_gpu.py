@@ -327,3 +327,26 @@ def test_cancel_all(model_dirs, gpu):
     assert [e.token for e in events if e.kind == "token" and e.request_id == 0] == want[0][:2]
     assert llm.engine.cache.free_seats == 2
     llm.engine.cache.check()
+
+
+def test_a_grammar_sees_real_tokens_after_a_request_was_refused(model_dirs, gpu):
+    """A request whose name another runner's has is refused when it is seated; the grammars that come later are still asked with the
+    tokens' values, not with their places in a step in flight."""
+    llm = LLM(model_dirs["A"], EngineOptions(dtype="bfloat16", max_seqs=3, max_seq_len=64))
+    want = llm.generate([[4, 5]], 6, ignore_eos=True)[0]
+    other, runner = (Runner(llm.engine, ServeOptions(ignore_eos=True)) for _ in range(2))
+    other.submit([1, 2, 3], 6)
+    other.step()
+    seen = []
+
+    def grammar(out):
+        seen.append(list(out))
+    runner.submit([1, 2, 3], 6, options=SampleOptions(grammar=lambda out: None))
+    with pytest.raises(EngineError):
+        runner.step()
+    runner.cancel(0)
+    runner.submit([4, 5], 6, options=SampleOptions(grammar=grammar))
+    tokens = [e.token for e in runner.run_until_idle() if e.kind == "token"]
+    assert tokens == want and seen == [tokens[:i] for i in range(6)]
+    other.cancel_all()
+    llm.engine.cache.check()
