@@ -194,6 +194,7 @@ extern "C" int kva_adjust_logits(const long long *address, float *out, long long
     if (rows == 0) return KVA_OK;
     KVA_REQUIRE((marks == nullptr) == (row_seat == nullptr) && (allowed == nullptr) == (allowed_row == nullptr),
                 "adjust_logits: marks and seats, grammars and the rows' numbers of them go together");
+    KVA_REQUIRE(biases >= 0 && biases <= INT_MAX - AL_THREADS, "adjust_logits: %d biases", biases);
     KVA_REQUIRE(biases == 0 || (bias_start != nullptr && bias_token != nullptr && bias_value != nullptr), "adjust_logits: a part of the biases is missing");
     const AdjustArgs a{logits, out, in_stride, out_stride, vocab, row_seat, seats, marks, counts, repetition, presence, frequency, bias_start,
                        bias_token, bias_value, biases, allowed_row, allowed, grammars, (vocab + 31) / 32};
@@ -223,7 +224,7 @@ count_tokens_kernel(unsigned char *__restrict__ marks, int *__restrict__ counts,
 
 extern "C" int kva_count_tokens(unsigned char *marks, int *counts, int seats, int vocab, const int *of, const int *tokens, int n,
                                 hipStream_t stream) {
-    KVA_REQUIRE(n >= 0 && seats > 0 && vocab > 0, "count_tokens: bad sizes");
+    KVA_REQUIRE(n >= 0 && n <= INT_MAX - 255 && seats > 0 && vocab > 0, "count_tokens: bad sizes seats=%d vocab=%d tokens=%d", seats, vocab, n);
     if (n == 0) return KVA_OK;
     KVA_REQUIRE(marks != nullptr && of != nullptr && tokens != nullptr, "count_tokens: marks, seats and tokens are needed");
     hipLaunchKernelGGL(count_tokens_kernel, dim3((n + 255) / 256), dim3(256), 0, stream, marks, counts, seats, vocab, of, tokens, n);

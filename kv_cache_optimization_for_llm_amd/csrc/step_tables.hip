@@ -61,10 +61,10 @@ grow_tables_kernel(GrowArgs a) {
     if (before + need > a.num_pages) return;            // not all of its pages are there: it takes none
     const int *src = a.pages + before;
     int *dst = a.table + (size_t)a.seats[e] * a.blocks + a.held[e];
-    for (int j = 4 * threadIdx.x; j < need; j += 4 * ST_THREADS) {
+    for (long long j = 4 * threadIdx.x; j < need; j += 4 * ST_THREADS) {
         if (j + 3 < need) *reinterpret_cast<st_i32x4 *>(dst + j) = *reinterpret_cast<const st_i32x4 *>(src + j);
         else
-            for (int i = j; i < need; ++i) dst[i] = src[i];
+            for (long long i = j; i < need; ++i) dst[i] = src[i];
     }
 }
 

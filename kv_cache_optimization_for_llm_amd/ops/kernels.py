@@ -1196,6 +1196,20 @@ def mark_tokens(mask: torch.Tensor, seats: torch.Tensor, tokens: torch.Tensor) -
           "mark_tokens")
 
 
+_MOST = (1 << 31) - 1           # what the C entries count sizes in
+
+
+def _size(what: str, name: str, n) -> int:
+    """A whole number that the C entries take as it is (a larger one would reach them without its upper bits)."""
+    try:
+        whole = int(n)
+    except (TypeError, ValueError, OverflowError):
+        whole = None
+    if whole is None or whole != n or abs(whole) > _MOST:
+        raise KernelError(f"{what}: {name} {n!r} is not a whole number of 32 bits")
+    return whole
+
+
 def _at(what: str, name: str, t: Optional[torch.Tensor], dtype: torch.dtype, shape: tuple, device: int) -> int:
     """The address of a contiguous tensor of this type and shape on the device that the launch goes to; 0 for no tensor."""
     if t is None:
@@ -1208,6 +1222,8 @@ def _at(what: str, name: str, t: Optional[torch.Tensor], dtype: torch.dtype, sha
         raise KernelError(f"{what}: {name} is {t.dtype}, expected {dtype}")
     if t.layout is not torch.strided or not t.is_contiguous():
         raise KernelError(f"{what}: {name} must be contiguous")
+    if any(n > _MOST for n in t.shape):
+        raise KernelError(f"{what}: {name} is {tuple(t.shape)}, sizes are counted in 32 bits")
     if t.get_device() != device:
         raise KernelError(f"{what}: {name} is on {t.device}, the launch goes to " + (f"cuda:{device}" if device >= 0 else "no GPU"))
     return t.data_ptr()
@@ -1240,6 +1256,8 @@ def _rows_of(what: str, name: str, t: torch.Tensor) -> tuple:
         raise KernelError(f"{what}: the elements of a row of {name} must lie next to each other")
     if rows > 1 and stride < cols:
         raise KernelError(f"{what}: rows of {name} overlap")
+    if rows > _MOST or cols > _MOST:
+        raise KernelError(f"{what}: {name} is {tuple(t.shape)}, sizes are counted in 32 bits")
     return t.data_ptr(), rows, cols, stride if rows > 1 else cols, dtype_code(t.dtype), t.get_device()
 
 
@@ -1410,6 +1428,7 @@ def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, le
     if seats.dim() != 1 or pages.dim() != 1 or table.dim() != 2:
         raise KernelError(f"{what}: a table [rows, blocks], a seat, held blocks and a length per request, and a row of pages")
     n, size, i32, entries = seats.shape, table.shape, torch.int32, seats.shape[0]
+    page_size = _size(what, "page_size", page_size)
     if offsets is None:
         offsets = torch.empty(entries + 1, dtype=i32, device=table.device)
     address = _addresses(what, "table seats held lengths pages offsets",
@@ -1418,7 +1437,7 @@ def grow_tables(table: torch.Tensor, seats: torch.Tensor, held: torch.Tensor, le
     _here(what, table.get_device())
     if entries == 0:
         return offsets.zero_()
-    check(hip_lib().kva_grow_tables(address.buffer_info()[0], size[0], size[1], entries, int(page_size), pages.shape[0], _stream()), what)
+    check(hip_lib().kva_grow_tables(address.buffer_info()[0], size[0], size[1], entries, page_size, pages.shape[0], _stream()), what)
     return offsets
 
 
@@ -1439,6 +1458,7 @@ def step_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, 
     if lengths.dim() != 1 or positions.dim() != 1 or len(slots) != len(tables) or any(t.dim() != 2 for t in tables):
         raise KernelError(f"{what}: a length per entry, a position per token, tables [rows, blocks] and as many arrays of slots")
     n, tokens, i32 = lengths.shape, positions.shape, torch.int32
+    page_size = _size(what, "page_size", page_size)
     spec = (lengths.get_device(), lengths, i32, n, starts, i32, n, seats, i32, n, q_start, i32, (n[0] + 1,), positions, i32, tokens,
             tok_seat, i32, tokens)
     sizes = array("q")
@@ -1447,7 +1467,7 @@ def step_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, 
         sizes.extend(t.shape)
     address = _addresses(what, "lengths starts seats q_start positions tok_seat" + " table slots" * len(tables), spec)
     _here(what, spec[0])
-    check(hip_lib().kva_step_rows(address.buffer_info()[0], sizes.buffer_info()[0], n[0], len(tables), int(page_size), tokens[0], _stream()), what)
+    check(hip_lib().kva_step_rows(address.buffer_info()[0], sizes.buffer_info()[0], n[0], len(tables), page_size, tokens[0], _stream()), what)
 
 
 _MAX_SPLITS = None

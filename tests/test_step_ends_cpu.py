@@ -184,3 +184,41 @@ def test_a_launch_needs_its_tensors():
                  lambda: lib.kva_sample_truncated(at, 64, 40, 2, 40, 0, 0, 0, 0)):
         with pytest.raises(KernelError):
             check(call(), "a launch")
+
+
+def meta(*shape, dtype=torch.int32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+MANY = (1 << 32) + 3            # 3, to who looks at 32 bits of it
+
+
+@pytest.mark.parametrize("call", [
+    lambda: K.adjust_logits(meta(MANY, 1, dtype=torch.float32), meta(MANY, 1, dtype=torch.float32)),
+    lambda: K.adjust_logits(meta(2, MANY, dtype=torch.float32), meta(2, MANY, dtype=torch.float32)),
+    lambda: K.adjust_logits(f32(2, 40), f32(2, 40), bias=(i32(3), meta(MANY), meta(MANY, dtype=torch.float32))),
+    lambda: K.adjust_logits(meta(2, 40, dtype=torch.float32), meta(2, 40, dtype=torch.float32), row_seat=meta(2),
+                            marks=meta(MANY, 40, dtype=torch.uint8)),
+    lambda: K.sample_truncated(meta(MANY, 1, dtype=torch.float32), meta(MANY), inv_temperature=meta(MANY, dtype=torch.float32),
+                               uniform=meta(MANY, dtype=torch.float32)),
+    lambda: K.count_tokens(meta(MANY, 9, dtype=torch.uint8), None, meta(3), meta(3)),
+    lambda: K.count_tokens(meta(3, 9, dtype=torch.uint8), None, meta(MANY), meta(MANY)),
+    lambda: K.grow_tables(meta(MANY, 8), meta(3), meta(3), meta(3), 16, meta(9)),
+    lambda: K.grow_tables(meta(4, 8), meta(3), meta(3), meta(3), 16, meta(MANY)),
+    lambda: K.grow_tables(meta(4, 8), meta(3), meta(3), meta(3), MANY, meta(9)),
+    lambda: K.grow_tables(meta(4, 8), meta(3), meta(3), meta(3), 2.5, meta(9)),
+    lambda: K.step_rows(meta(3), meta(3), meta(3), [meta(4, 8)], -MANY, meta(4), meta(5), meta(5), [meta(5)]),
+    lambda: K.step_rows(meta(3), meta(3), meta(3), [meta(4, 8)], "16", meta(4), meta(5), meta(5), [meta(5)]),
+    lambda: K.step_rows(meta(3), meta(3), meta(3), [meta(MANY, 8)], 16, meta(4), meta(5), meta(5), [meta(5)]),
+    lambda: K.step_rows(meta(3), meta(3), meta(3), [meta(4, 8)], 16, meta(4), meta(MANY), meta(MANY), [meta(MANY)])])
+def test_sizes_that_32_bits_do_not_hold_are_refused(call):
+    with pytest.raises(KernelError, match="32 bits"):
+        call()
+
+
+def test_sizes_that_a_launch_cannot_count_are_refused():
+    lib = hip_lib()
+    for call in (lambda: lib.kva_count_tokens(64, 0, 2, 9, 64, 64, (1 << 31) - 255, 0),
+                 lambda: lib.kva_adjust_logits(array("q", [64] * 11).buffer_info()[0], 64, 40, 64, 0, 40, 2, 40, 2, (1 << 31) - 1, 1, 0)):
+        with pytest.raises(KernelError, match="bad sizes|biases"):
+            check(call(), "a launch")
