@@ -139,6 +139,14 @@ def _align(n: int, a: int = 4) -> int:
     return (n + a - 1) // a * a
 
 
+def make_rows(lengths: torch.Tensor, starts: torch.Tensor, seats: torch.Tensor, cache_tables: Sequence[torch.Tensor], page_size: int,
+              q_start: torch.Tensor, positions: torch.Tensor, tok_seat: torch.Tensor, slots: Sequence[torch.Tensor]) -> None:
+    """:func:`~..ops.kernels.step_rows` of as many cache groups as there are: a launch takes some of them."""
+    for g in range(0, max(1, len(cache_tables)), K.MAX_STEP_GROUPS):
+        some = slice(g, g + K.MAX_STEP_GROUPS)
+        K.step_rows(lengths, starts, seats, cache_tables[some], page_size, q_start, positions, tok_seat, slots[some])
+
+
 def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequence[Sequence[int]],
                 wants: Sequence[Sequence[int]], slot_maps: Optional[Sequence[Sequence[np.ndarray]]],
                 device, tables: Sequence[torch.Tensor] = (), page_size: int = 0) -> StepBatch:
@@ -195,8 +203,8 @@ def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequen
     if made:
         rows = torch.empty((2 + G, _align(max(1, T))), dtype=torch.int32, device=device)[:, :T]
         d_positions, d_tok_seat, d_slots = rows[0], rows[1], [rows[2 + g] for g in range(G)]
-        K.step_rows(view("lengths"), view("entry_start_pos"), view("entry_seat"), tables, page_size, view("entry_q_start"),
-                    d_positions, d_tok_seat, d_slots)
+        make_rows(view("lengths"), view("entry_start_pos"), view("entry_seat"), tables, page_size, view("entry_q_start"),
+                  d_positions, d_tok_seat, d_slots)
     else:
         d_positions, d_tok_seat, d_slots = view("positions"), view("tok_seat"), [view(f"slots{g}") for g in range(G)]
 

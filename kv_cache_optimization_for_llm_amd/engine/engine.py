@@ -19,7 +19,7 @@ from ..cache.manager import CacheManager
 from ..cache.manager import page_bytes as cache_page_bytes
 from ..config.model_config import read_config_json
 from ..models.builder import Model, spec_for_config
-from ..ops.kernels import MAX_STEP_ENTRIES, MAX_STEP_GROUPS
+from ..ops.kernels import MAX_STEP_ENTRIES
 from ..ops.library import KernelLibraryError, hip_lib
 from ..weights.loader import load_tensors
 from ..weights.random_init import random_tensors_on_device
@@ -172,8 +172,7 @@ class Engine:
         if options.use_graphs and self.dtype == torch.bfloat16 and self.model.graph_safe():
             from .graphs import DecodeGraphs, PortionGraphs
             self.graphs = DecodeGraphs(self.model, self.cache, self.device, self.feedback)
-            if len(groups) <= MAX_STEP_GROUPS:
-                self.portion_graphs = PortionGraphs(self.model, self.cache, self.device, self.feedback)
+            self.portion_graphs = PortionGraphs(self.model, self.cache, self.device, self.feedback)
 
     # ------------------------------------------------------------------ requests
     def has_request(self, request_id) -> bool:
@@ -276,7 +275,7 @@ class Engine:
 
     def _batch(self, seats, starts, toks, wants, slot_maps) -> StepBatch:
         groups = self.cache.groups
-        if slot_maps is None and (len(seats) > MAX_STEP_ENTRIES or len(groups) > MAX_STEP_GROUPS):
+        if slot_maps is None and len(seats) > MAX_STEP_ENTRIES:
             slot_maps = [[self.cache.slot_mapping(seat, start, len(arr), g.index)
                           for seat, start, arr in zip(seats, starts, toks)] for g in groups]
         batch = build_batch(seats, starts, toks, wants, slot_maps, self.device, [g.table_dev for g in groups], self.cache.page_size)

@@ -27,7 +27,7 @@ import torch
 from collections import OrderedDict
 
 from ..ops import kernels as K
-from .batch import StepBatch, attention_work_items
+from .batch import StepBatch, attention_work_items, make_rows
 
 
 def context_bucket(max_context: int) -> int:
@@ -214,8 +214,8 @@ class _PortionSlot:
         self.dev.copy_(self.staging, non_blocking=True)
         self.copied.record()
         b = self.batch
-        K.step_rows(self.entry_len, b.entry_start_pos, b.entry_seat, [g.table_dev for g in cache.groups], cache.page_size,
-                    self.made_q_start, b.positions, b.tok_seat, b.slot_mapping)
+        make_rows(self.entry_len, b.entry_start_pos, b.entry_seat, [g.table_dev for g in cache.groups], cache.page_size,
+                  self.made_q_start, b.positions, b.tok_seat, b.slot_mapping)
 
 
 class PortionGraphs:

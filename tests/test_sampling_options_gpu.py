@@ -350,3 +350,27 @@ def test_a_grammar_sees_real_tokens_after_a_request_was_refused(model_dirs, gpu)
     assert tokens == want and seen == [tokens[:i] for i in range(6)]
     other.cancel_all()
     llm.engine.cache.check()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_models_of_more_cache_groups_than_a_launch_takes(tmp_path, gpu, dtype):
+    """Eleven windows of their own: portions beside each other, eagerly and (bf16) replayed from their graphs, are the plain model's."""
+    import bonusun_util as U
+    from kv_cache_optimization_for_llm_amd.engine.engine import Engine
+    cfg = {"architecture": "Bonusun", "vocab": 101, "width": 64, "norm": {"eps": 0.05}, "residual_mult": 0.7, "layers": [
+        U.attention_layer(U.attention(2, 1, 32, 32, 0.2, rot=(32, 1000.0), window=9 + 3 * i), U.dense(48)) for i in range(11)]}
+    folder, state = U.write_model(str(tmp_path / "m"), cfg, 3)
+    eng = Engine(folder, EngineOptions(dtype=dtype, page_size=16, cache_tokens=1024, max_seqs=4, max_seq_len=256, max_batch_tokens=256))
+    assert len(eng.cache.groups) == 11 and (eng.portion_graphs is not None) == (dtype == "bfloat16")
+    steps, requests = [], {}
+    for turn in range(5):
+        new = {f"{x}{turn}": U.prompt(cfg, 72, 60 + 10 * turn + i) for i, x in enumerate("ab")}
+        requests.update(new)
+        for lo in range(0, 72, 24):
+            steps.append({"entries": [{"id": r, "tokens": t[lo:lo + 24], "want": [0, 23]} for r, t in new.items()],
+                          "end": list(new) if lo == 48 else []})
+    rows, routes = U.run_steps(eng, steps, cfg)
+    want = U.expected_rows(cfg, state, requests, routes, dtype)
+    U.assert_rows(rows, want, dtype, "portions")
+    assert dtype == "float32" or eng.portion_graphs.replays > 0
+    eng.cache.check()
