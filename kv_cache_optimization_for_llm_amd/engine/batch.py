@@ -155,7 +155,7 @@ def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequen
     ``slot_maps[g][e]`` is the slot array of entry ``e`` in cache group ``g``.  Without them, what a token's row holds (position, seat,
     slot in every group of ``tables``, the groups' block tables on the device) is made there from the entries' lengths
     (:func:`~..ops.kernels.step_rows`); the host has no copy of it then (us of host time, slot maps included, host / device: 64 entries
-    of 8 tokens 341 / 167, 32 of 128 276 / 175, one of 8,192 213 / 191, one of 512 47 / 55)."""
+    of 8 tokens 362 / 163, 32 of 128 238 / 127, one of 8,192 126 / 97, one of 512 45 / 45)."""
     E = len(seats)
     lens = [len(t) for t in token_lists]
     T = int(sum(lens))

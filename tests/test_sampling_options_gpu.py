@@ -374,3 +374,21 @@ def test_models_of_more_cache_groups_than_a_launch_takes(tmp_path, gpu, dtype):
     U.assert_rows(rows, want, dtype, "portions")
     assert dtype == "float32" or eng.portion_graphs.replays > 0
     eng.cache.check()
+
+
+def test_short_portions_alone_are_made_by_the_host(model_dirs, gpu, monkeypatch):
+    """Where a launch costs the host more than the rows themselves; the same logits either way."""
+    from kv_cache_optimization_for_llm_amd.engine import batch, engine
+    from kv_cache_optimization_for_llm_amd.engine.batch import StepEntry
+    made, step_rows = [], batch.K.step_rows
+    monkeypatch.setattr(batch.K, "step_rows", lambda *args: (made.append(len(args[0])), step_rows(*args)))
+    prompt = prompts_for(256, [400], 7)[0]
+    got = []
+    for most in (256, 0):
+        monkeypatch.setattr(engine, "HOST_ROWS", most)
+        eng = engine.Engine(model_dirs["A"], EngineOptions(dtype="float32", max_seqs=4, max_seq_len=512))
+        assert len(eng.cache.groups) == 1
+        for entries in ([("a", 0, 2)], [("a", 2, 100)], [("a", 100, 357)], [("b", 0, 300)], [("c", 0, 5), ("d", 0, 9)]):
+            got.append(eng.step([StepEntry(r, prompt[i:j], [j - i - 1]) for r, i, j in entries]).clone())
+    assert made == [1, 1, 2] + [1, 1, 1, 1, 2]
+    assert all(torch.equal(a, b) for a, b in zip(got[:5], got[5:]))
