@@ -19,7 +19,7 @@
 
 #define AL_THREADS 256
 #define AL_WAVES (AL_THREADS / KVA_WAVE)
-#define AL_UNITS 1
+#define AL_TILE (4 * AL_THREADS)
 
 typedef float al_f32x4 __attribute__((ext_vector_type(4), aligned(4)));         // (rows start at any multiple of their type)
 typedef uint16_t al_u16x4 __attribute__((ext_vector_type(4), aligned(2)));
@@ -43,35 +43,31 @@ struct AdjustArgs {
     int grammars, words;
 };
 
-// grid (tiles, rows); a tile is UNITS x 1,024 tokens
-template <typename T, int UNITS, bool STREAMED>
+// grid (tiles, rows); a tile is 1,024 tokens, four neighbouring ones a thread
+template <typename T, bool STREAMED>
 __global__ void __launch_bounds__(AL_THREADS)
 adjust_logits_kernel(AdjustArgs a) {
     __shared__ int hit_token[AL_THREADS];
     __shared__ float hit_value[AL_THREADS];
     __shared__ int hits_of[AL_WAVES];
     const int row = blockIdx.y, tid = threadIdx.x, lane = tid % KVA_WAVE, wave = tid / KVA_WAVE, vocab = a.vocab;
-    const int tile0 = blockIdx.x * (UNITS * 4 * AL_THREADS), tile1 = min(vocab, tile0 + UNITS * 4 * AL_THREADS);
+    const int tile0 = blockIdx.x * AL_TILE, tile1 = min(vocab, tile0 + AL_TILE), t = tile0 + 4 * tid;
     const T *in = reinterpret_cast<const T *>(a.logits) + row * a.in_stride;
-    float l[UNITS][4];
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        const int t = tile0 + 4 * (u * AL_THREADS + tid);
-        if (t + 3 < vocab) {
-            if constexpr (sizeof(T) == 4) {
-                const al_f32x4 *p = reinterpret_cast<const al_f32x4 *>(in + t);
-                const al_f32x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
-                l[u][0] = v.x, l[u][1] = v.y, l[u][2] = v.z, l[u][3] = v.w;
-            } else {
-                const al_u16x4 *p = reinterpret_cast<const al_u16x4 *>(in + t);
-                const al_u16x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
-                l[u][0] = bf16_bits_to_float(v.x), l[u][1] = bf16_bits_to_float(v.y);
-                l[u][2] = bf16_bits_to_float(v.z), l[u][3] = bf16_bits_to_float(v.w);
-            }
+    float l[4];
+    if (t + 3 < vocab) {
+        if constexpr (sizeof(T) == 4) {
+            const al_f32x4 *p = reinterpret_cast<const al_f32x4 *>(in + t);
+            const al_f32x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
+            l[0] = v.x, l[1] = v.y, l[2] = v.z, l[3] = v.w;
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) l[u][i] = t + i < vocab ? to_float(in[t + i]) : 0.f;
+            const al_u16x4 *p = reinterpret_cast<const al_u16x4 *>(in + t);
+            const al_u16x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
+            l[0] = bf16_bits_to_float(v.x), l[1] = bf16_bits_to_float(v.y);
+            l[2] = bf16_bits_to_float(v.z), l[3] = bf16_bits_to_float(v.w);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[i] = t + i < vocab ? to_float(in[t + i]) : 0.f;
     }
     // a row that names a seat or a grammar that is not there gets no token at all
     bool lost = false;
@@ -83,31 +79,26 @@ adjust_logits_kernel(AdjustArgs a) {
             const int *counts = a.counts != nullptr ? a.counts + (size_t)seat * vocab : nullptr;
             const float rep = a.repetition != nullptr ? a.repetition[row] : 1.f;
             const float pres = a.presence != nullptr ? a.presence[row] : 0.f, freq = a.frequency != nullptr ? a.frequency[row] : 0.f;
+            unsigned m = 0;
+            if (t + 3 < vocab) {
+                const al_u8x4 *p = reinterpret_cast<const al_u8x4 *>(marks + t);
+                const al_u8x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
+                m = (v.x != 0) | (v.y != 0) << 1 | (v.z != 0) << 2 | (v.w != 0) << 3;
+            } else {
 #pragma unroll
-            for (int u = 0; u < UNITS; ++u) {
-                const int t = tile0 + 4 * (u * AL_THREADS + tid);
-                unsigned m = 0;
-                if (t + 3 < vocab) {
-                    const al_u8x4 *p = reinterpret_cast<const al_u8x4 *>(marks + t);
-                    const al_u8x4 v = STREAMED ? __builtin_nontemporal_load(p) : *p;
-                    m = (v.x != 0) | (v.y != 0) << 1 | (v.z != 0) << 2 | (v.w != 0) << 3;
-                } else {
+                for (int i = 0; i < 4; ++i)
+                    if (t + i < vocab && marks[t + i] != 0) m |= 1u << i;
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (t + i < vocab && marks[t + i] != 0) m |= 1u << i;
+            for (int i = 0; i < 4; ++i) {
+                if (!(m >> i & 1)) continue;
+                float x = l[i];
+                if (rep != 1.f) x = x > 0.f ? x / rep : x * rep;
+                if (counts != nullptr) {
+                    const int c = counts[t + i];
+                    if (c > 0) x -= fmaf(freq, (float)c, pres);
                 }
-                if (m == 0) continue;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!(m >> i & 1)) continue;
-                    float x = l[u][i];
-                    if (rep != 1.f) x = x > 0.f ? x / rep : x * rep;
-                    if (counts != nullptr) {
-                        const int c = counts[t + i];
-                        if (c > 0) x -= fmaf(freq, (float)c, pres);
-                    }
-                    l[u][i] = x;
-                }
+                l[i] = x;
             }
         }
     }
@@ -134,14 +125,12 @@ adjust_logits_kernel(AdjustArgs a) {
             __syncthreads();
             for (int h = 0; h < hits; ++h) {
                 const int rel = hit_token[h] - tile0;
-                if ((rel >> 2) % AL_THREADS != tid) continue;
-                const int unit = (rel >> 2) / AL_THREADS, which = rel & 3;
+                if (rel >> 2 != tid) continue;
+                const int which = rel & 3;
                 const float b = hit_value[h];
 #pragma unroll
-                for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (u == unit && j == which) l[u][j] += b;
+                for (int j = 0; j < 4; ++j)
+                    if (j == which) l[j] += b;
             }
             __syncthreads();
         }
@@ -152,28 +141,24 @@ adjust_logits_kernel(AdjustArgs a) {
         if (g >= a.grammars || g < -1) lost = true;
         else if (g >= 0) allowed = a.allowed + (size_t)g * a.words;
     }
+    if (t >= vocab) return;
     float *out = a.out + row * a.out_stride;
+    unsigned bits = 15;
+    if (allowed != nullptr) bits = allowed[t / 32] >> t % 32;
+    if (lost) bits = 0;
+    al_f32x4 v;
+    v.x = bits & 1 ? l[0] : -INFINITY;
+    v.y = bits & 2 ? l[1] : -INFINITY;
+    v.z = bits & 4 ? l[2] : -INFINITY;
+    v.w = bits & 8 ? l[3] : -INFINITY;
+    al_f32x4 *to = reinterpret_cast<al_f32x4 *>(out + t);
+    if (t + 3 < vocab) {
+        if (STREAMED) __builtin_nontemporal_store(v, to);
+        else *to = v;
+    } else
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        const int t = tile0 + 4 * (u * AL_THREADS + tid);
-        if (t >= vocab) continue;
-        unsigned bits = 15;
-        if (allowed != nullptr) bits = allowed[t / 32] >> t % 32;
-        if (lost) bits = 0;
-        al_f32x4 v;
-        v.x = bits & 1 ? l[u][0] : -INFINITY;
-        v.y = bits & 2 ? l[u][1] : -INFINITY;
-        v.z = bits & 4 ? l[u][2] : -INFINITY;
-        v.w = bits & 8 ? l[u][3] : -INFINITY;
-        al_f32x4 *to = reinterpret_cast<al_f32x4 *>(out + t);
-        if (t + 3 < vocab) {
-            if (STREAMED) __builtin_nontemporal_store(v, to);
-            else *to = v;
-        } else
-#pragma unroll
-            for (int i = 0; i < 3; ++i)
-                if (t + i < vocab) out[t + i] = v[i];
-    }
+        for (int i = 0; i < 3; ++i)
+            if (t + i < vocab) out[t + i] = v[i];
 }
 
 // address [11], the host's: of row_seat, marks, counts, repetition, presence, frequency, the biases' starts, tokens and values, allowed_row
@@ -198,12 +183,11 @@ extern "C" int kva_adjust_logits(const long long *address, float *out, long long
     KVA_REQUIRE(biases == 0 || (bias_start != nullptr && bias_token != nullptr && bias_value != nullptr), "adjust_logits: a part of the biases is missing");
     const AdjustArgs a{logits, out, in_stride, out_stride, vocab, row_seat, seats, marks, counts, repetition, presence, frequency, bias_start,
                        bias_token, bias_value, biases, allowed_row, allowed, grammars, (vocab + 31) / 32};
-    const int tile = AL_UNITS * 4 * AL_THREADS;
     const long long touched = (long long)rows * vocab * ((dtype == KVA_F32 ? 4 : 2) + 4 + (row_seat != nullptr ? 1 : 0));
     const bool streamed = touched > 256ll << 20;
-    const dim3 grid((vocab + tile - 1) / tile, rows), block(AL_THREADS);
-    const auto kernel = dtype == KVA_F32 ? (streamed ? adjust_logits_kernel<float, AL_UNITS, true> : adjust_logits_kernel<float, AL_UNITS, false>)
-                                         : (streamed ? adjust_logits_kernel<bf16_t, AL_UNITS, true> : adjust_logits_kernel<bf16_t, AL_UNITS, false>);
+    const dim3 grid((vocab + AL_TILE - 1) / AL_TILE, rows), block(AL_THREADS);
+    const auto kernel = dtype == KVA_F32 ? (streamed ? adjust_logits_kernel<float, true> : adjust_logits_kernel<float, false>)
+                                         : (streamed ? adjust_logits_kernel<bf16_t, true> : adjust_logits_kernel<bf16_t, false>);
     hipLaunchKernelGGL(kernel, grid, block, 0, stream, a);
     KVA_CHECK_LAUNCH("adjust_logits");
     return KVA_OK;
