@@ -46,8 +46,6 @@ class StepBatch:
     entry_q_start: torch.Tensor      # [E + 1] first row of each entry (last = T)
     entry_start_pos: torch.Tensor    # [E] position of the entry's first token
     # host copies of the same
-    h_positions: np.ndarray = field(repr=False, default=None)
-    h_tok_seat: np.ndarray = field(repr=False, default=None)
     h_entry_seat: np.ndarray = field(repr=False, default=None)
     h_entry_q_start: np.ndarray = field(repr=False, default=None)
     h_entry_start_pos: np.ndarray = field(repr=False, default=None)
@@ -154,8 +152,8 @@ def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequen
 
     ``slot_maps[g][e]`` is the slot array of entry ``e`` in cache group ``g``.  Without them, what a token's row holds (position, seat,
     slot in every group of ``tables``, the groups' block tables on the device) is made there from the entries' lengths
-    (:func:`~..ops.kernels.step_rows`); the host has no copy of it then (us of host time, slot maps included, host / device: 64 entries
-    of 8 tokens 362 / 163, 32 of 128 238 / 127, one of 8,192 126 / 97, one of 512 45 / 45)."""
+    (:func:`~..ops.kernels.step_rows`; us of host time, slot maps included, host / device: 64 entries of 8 tokens 362 / 163, 32 of 128
+    238 / 127, one of 8,192 126 / 97, one of 512 45 / 45)."""
     E = len(seats)
     lens = [len(t) for t in token_lists]
     T = int(sum(lens))
@@ -163,11 +161,6 @@ def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequen
     q_start = np.zeros(E + 1, dtype=np.int32)
     np.cumsum(lens, out=q_start[1:])
     token_ids = np.concatenate([np.asarray(t, dtype=np.int32) for t in token_lists]) if T else np.zeros(0, np.int32)
-    positions = tok_seat = None
-    if not made:
-        positions = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, lens)]) \
-            if T else np.zeros(0, np.int32)
-        tok_seat = np.repeat(np.asarray(seats, dtype=np.int32), lens)
     wanted: List[int] = []
     for e, w in enumerate(wants):
         for i in w:
@@ -184,7 +177,8 @@ def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequen
     if made:
         segs["lengths"] = np.asarray(lens, dtype=np.int32)
     else:
-        segs["positions"], segs["tok_seat"] = positions, tok_seat
+        segs["positions"] = np.concatenate([np.arange(s, s + n, dtype=np.int32) for s, n in zip(starts, lens)]) if T else np.zeros(0, np.int32)
+        segs["tok_seat"] = np.repeat(np.asarray(seats, dtype=np.int32), lens)
         for g in range(G):
             segs[f"slots{g}"] = np.concatenate(slot_maps[g]).astype(np.int32) if T else np.zeros(0, np.int32)
     offsets, total = {}, 0
@@ -214,8 +208,7 @@ def build_batch(seats: Sequence[int], starts: Sequence[int], token_lists: Sequen
         logit_rows=view("logit_rows"), slot_mapping=d_slots,
         entry_seat=view("entry_seat"), entry_q_start=view("entry_q_start"),
         entry_start_pos=view("entry_start_pos"),
-        h_positions=positions, h_tok_seat=tok_seat, h_entry_seat=segs["entry_seat"],
-        h_entry_q_start=q_start, h_entry_start_pos=segs["entry_start_pos"],
+        h_entry_seat=segs["entry_seat"], h_entry_q_start=q_start, h_entry_start_pos=segs["entry_start_pos"],
         logits_for_all_rows=wanted == list(range(T)),
         max_q_len=max(lens) if lens else 0, min_q_len=min(lens) if lens else 0,
         max_context=max((s + n for s, n in zip(starts, lens)), default=0),
