@@ -30,7 +30,7 @@
 // sought is the next turn's; the row is read again in every turn (out of LDS up to 16,384 tokens).
 //
 // us in a graph.  Vocabulary 128,256: 1 row of a p 21, of a k 17; 64 rows of p 0.9 49 (7.2 + 18 + 17 + 9.2 for the four kernels), of a k up to 50 24 (7.4 + 1.8 + 1.8 +
-// 14.2: 33 MB are 6.4 us at a copy's rate); 256 rows of p 0.98 at a temperature of 2, which keep most of the vocabulary, 117 (21 + 33 + 59 + 11: the
+// 14.2: 33 MB are 6.4 us at a copy's rate); 256 rows of p 0.98 at a temperature of 2, which keep most of the vocabulary, 118 (21 + 34 + 59 + 10: the
 // first reads 131 MB at 6.2 TB/s, the next two weigh every token); rows of nearly equal logits 410 to 480.  One launch, against four: 1,024 tokens 10 / 16
 // to 25, 2,048 13 to 15 / 17 to 22, 4,096 16 to 21 / 17 to 29, 8,192 28 to 31 / 18 to 25.
 #include "common.h"

@@ -1286,7 +1286,7 @@ def adjust_logits(logits: torch.Tensor, out: torch.Tensor, *, row_seat: Optional
     * ``allowed`` int32 ``[grammars, ceil(vocab / 32)]`` with ``allowed_row`` (-1: everything): the logit of a token whose bit
       (``token % 32`` of word ``token / 32``) is not set becomes -inf.
 
-    A row that names a seat or a grammar that is not there gets -inf everywhere: no token can be taken from it."""
+    A row that names a seat or a grammar that is not there gets -inf everywhere: no token can be taken from it.  Up to 65,535 rows."""
     what = "adjust_logits"
     native = _launches(logits)
     code = native.adjust_logits(logits, out, row_seat, marks, counts, repetition, presence, frequency, bias, allowed_row, allowed,
@@ -1374,7 +1374,7 @@ def sample_truncated(logits: torch.Tensor, out_tokens: torch.Tensor, *, inv_temp
     it is none.  Rows whose ``inv_temperature`` is not above 0 take the best token, and rows where it is no number are passed over:
     what stands in the outputs stays.  ``kept`` (int32) gets how many tokens stayed, ``logprob`` (fp32) the token's log-probability
     among them (0 of a single one).  A row without a logit above -inf, and one at a temperature whose largest is +inf, gets -1,
-    no tokens and -inf.  Vocabularies of up to 2^24.  ``host_tokens`` as in :func:`sample`."""
+    no tokens and -inf.  Up to 65,535 rows, vocabularies of up to 2^24.  ``host_tokens`` as in :func:`sample`."""
     what = "sample_truncated"
     native = _launches(logits)
     code = native.sample_truncated(logits, out_tokens, inv_temperature, top_k, top_p, min_p, uniform, rng_key, rng_step, kept, logprob,

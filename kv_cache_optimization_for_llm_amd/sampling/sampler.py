@@ -314,7 +314,7 @@ class Sampler:
                 grammars.append(packed)
         biases = [sorted((o.logit_bias or {}).items()) if o is not None else [] for o in opts]
         total_biases = sum(map(len, biases))
-        # one upload: ten numbers a row, the biases, the grammars
+        # one upload: eleven numbers a row, where each one's biases begin, the biases, the grammars (and another with the penalties)
         size = 11 * n + (n + 1) + 2 * total_biases + len(grammars) * words
         # (a block of torch's pinned memory is not handed out again before the copy has left it)
         staging = torch.empty(size, dtype=torch.int32, pin_memory=True)
